@@ -74,6 +74,7 @@ typedef uint16_t wm_bf16;
 #define WKV_FP4_UE8M0_B32 3 /* PackedRows 'fp4_ue8m0'                                         */
 #define WKV_MXFP8_B32 4     /* mx.quantize(mode="mxfp8") chunks (fp8_cache.py:112)             */
 #define WKV_MXFP4_B32 5     /* mx.quantize(mode="mxfp4") index copy (fp8_cache.py:116)         */
+#define WKV_BF16 6          /* bf16 rows as they are (paged cache only)                      */
 
 /* Message for the last failing call on this thread ("" if none). */
 WM_API const char *w_last_error(void);
@@ -236,6 +237,86 @@ WM_API int wkv_dequantize(const uint8_t *payload, const void *scales, int64_t ro
 WM_API int wkv_gather_dequantize(const uint8_t *payload, const void *scales, int64_t rows,
                           const int32_t *row_idx, int64_t n, int D, int fmt, wm_bf16 *out,
                           wm_stream_t stream);
+
+/* ----------------------------------------------------- paged KV cache ----- */
+
+/* A paged cache tensor is a pool [n_pages, Hkv, page_size, D] of rows: bf16
+ * (fmt WKV_BF16), or e4m3 bytes with scales [n_pages, Hkv, page_size, D/64]
+ * float32 (WKV_FP8_F32_B64) or [n_pages, Hkv, page_size, D/32] E8M0
+ * (WKV_MXFP8_B32).  D is 64, 128 or 256, page_size a multiple of 16.  Entry e
+ * of sequence b is slot e % page_size of page page_table[b, e / page_size]
+ * (page_table int32 [B, max_pages]; entries behind a sequence's length are not
+ * read).  lengths int32 [B] holds the entries of each sequence; the capacity of
+ * a sequence is max_pages * page_size.  Lengths, tables and counts live on the
+ * device and are read by the kernels, so a captured call follows them.  No call
+ * reads or writes through a page id outside [0, n_pages).
+ * The reference keeps dense per-sequence caches (mlx-lm KVCache,
+ * runtime/deepseek_v4_ssd/qwen_quantized_cache.py:6-20); these calls serve
+ * batches of sequences of different lengths from one pool. */
+
+/* Write new tokens: k, v bf16 [T, Hkv, D] (k_stride, v_stride values between
+ * tokens, multiples of 8), packed by sequence: the tokens of sequence b are
+ * cu_seqlens[b] .. cu_seqlens[b+1]-1 (int32 [B+1]) and become its last entries,
+ * lengths[b] counting them already.  Quantized rows are the bytes of
+ * wkv_quantize.  Tokens outside cu_seqlens' range, entries outside the capacity
+ * and pages out of range are skipped.  Optional arrays [B, Hkv, capacity]:
+ * mass float32 gets 0 and positions int32 the token's position (seen[b] counts
+ * the sequence's tokens including the new ones) at the written entries. */
+WM_API int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride, int64_t v_stride,
+                            const int32_t *cu_seqlens, int T, int B, int Hkv, int D, void *k_cache, void *v_cache,
+                            void *k_scales, void *v_scales, int fmt, int n_pages, int page_size,
+                            const int32_t *page_table, int max_pages, const int32_t *lengths, float *mass,
+                            int32_t *positions, const int32_t *seen, wm_stream_t stream);
+
+/* Reduce every sequence longer than `budget` to `budget` entries, for each head
+ * by itself: entries with position >= seen[b] - recent or position < sinks stay
+ * (recent + sinks <= budget), then those of the largest mass, ties to the lower
+ * entry.  Kept entries behind the budget move into the freed entries before it,
+ * in order; the others do not move.  mass, positions [B, Hkv, capacity] are
+ * updated in place (mass_out == mass and positions_out == positions) or written
+ * to arrays of their own; lengths_out [B] (not lengths) gets min(length, budget).
+ * A sequence with a length or a page id out of range is left as it is.  Pages
+ * shared between sequences must not be evicted from.  Workspace:
+ * wkv_evict_workspace_size(B, Hkv, min(budget, capacity)). */
+WM_API size_t wkv_evict_workspace_size(int B, int Hkv, int budget);
+WM_API int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k_scales, void *v_scales, int fmt,
+                           int n_pages, int page_size, const int32_t *page_table, int max_pages, const int32_t *lengths,
+                           const int32_t *seen, const float *mass, const int32_t *positions, int budget, int recent,
+                           int sinks, float *mass_out, int32_t *positions_out, int32_t *lengths_out, void *workspace,
+                           size_t ws_bytes, wm_stream_t stream);
+
+/* Attention of one token per sequence over the paged cache: for query head h of
+ * kv head h / (Hq / Hkv), s_j = scale * q.k_j over the lengths[b] entries,
+ *   lse = log sum_j exp(s_j),   out = sum_j exp(s_j - lse) v_j.
+ * q bf16 [B, Hq, D] (q_stride values between sequences), out bf16 [B, Hq, D],
+ * lse float32 [B, Hq] or NULL.  mass (float32 [B, Hkv, capacity] or NULL):
+ * every entry's weight, summed over its query heads, is added to it.  A
+ * sequence of length 0 gets zeros and lse -inf; one whose length is outside
+ * [0, capacity] or that reaches a page id outside [0, n_pages) gets NaN.
+ * Workspace: wattn_decode_workspace_size (with a mass array it also holds the
+ * scores, 4 bytes per entry of the capacity and query head, heads rounded up to
+ * 8 or a multiple of 16 per kv head); calls that share one must not overlap. */
+WM_API size_t wattn_decode_workspace_size(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages,
+                                          int with_mass);
+WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int D, const void *k_cache,
+                        const void *v_cache, const void *k_scales, const void *v_scales, int fmt, int n_pages,
+                        int page_size, const int32_t *page_table, int max_pages, const int32_t *lengths, float scale,
+                        wm_bf16 *out, float *lse, float *mass, void *workspace, size_t ws_bytes, wm_stream_t stream);
+
+/* Attention of packed prompts.  q bf16 [Tq, Hq, D], k, v bf16 [Tk, Hkv, D] with
+ * q_stride, k_stride, v_stride values between tokens (multiples of 8; heads are
+ * dense, so slices of one projection's output can be passed as they are).
+ * Sequence b has the rows cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1 and the keys
+ * cu_seqlens_k[b] .. cu_seqlens_k[b+1]-1 (int32 [B+1], on the device).  With
+ * causal != 0 row i of nq sees the keys j <= i + nk - nq: a prompt its own
+ * tokens, a continuation also its history; else all nk keys.  out bf16
+ * [Tq, Hq, D]; lse float32 [Tq, Hq] or NULL (natural logarithm).  A row that sees
+ * no key gets zeros and lse -inf; rows outside every sequence are not written.
+ * D is 64, 128 or 256.  Uses no workspace.  */
+WM_API int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q_stride, int64_t k_stride,
+                        int64_t v_stride, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int B, int Tq,
+                        int Tk, int Hq, int Hkv, int D, float scale, int causal, wm_bf16 *out, float *lse,
+                        wm_stream_t stream);
 
 /* --------------------------------------------------------------- router --- */
 

@@ -1,0 +1,180 @@
+"""Argument checks of the attention and paged-cache calls, and the paged cache's
+host side, without a GPU: every refusal comes before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+import whallm_b200 as W
+from whallm_b200 import _lib as L
+
+P = ctypes.c_void_p(1 << 20)          # an aligned address that no refused call touches
+ODD = ctypes.c_void_p((1 << 20) + 2)
+
+
+def expect(name, args, msg, code=L.WM_ERR_INVALID):
+    rc = getattr(L.lib(), name)(*args)
+    assert rc == code, (name, rc, L.last_error())
+    if msg:
+        assert msg in L.last_error(), L.last_error()
+
+
+def append_args(**c):
+    d = dict(k=P, v=P, ks=512, vs=512, cu=P, T=4, B=2, Hkv=4, D=128, kc=P, vc=P, ksc=None, vsc=None, fmt=L.WKV_BF16, n=8, page=16,
+             table=P, width=4, lengths=P, mass=None, pos=None, seen=None, stream=None)
+    return tuple({**d, **c}.values())
+
+
+def evict_args(**c):
+    d = dict(B=2, Hkv=4, D=128, kc=P, vc=P, ksc=None, vsc=None, fmt=L.WKV_BF16, n=8, page=16, table=P, width=4, lengths=P, seen=P,
+             mass=P, pos=P, budget=32, recent=4, sinks=4, mo=P, po=P, lo=ctypes.c_void_p(1 << 21), ws=P, bytes=1 << 20, stream=None)
+    return tuple({**d, **c}.values())
+
+
+def decode_args(**c):
+    d = dict(q=P, qs=1024, B=2, Hq=8, Hkv=4, D=128, kc=P, vc=P, ksc=None, vsc=None, fmt=L.WKV_BF16, n=8, page=16, table=P, width=4,
+             lengths=P, scale=0.1, out=P, lse=None, mass=None, ws=P, bytes=1 << 30, stream=None)
+    return tuple({**d, **c}.values())
+
+
+def prompt_args(**c):
+    d = dict(q=P, k=P, v=P, qs=1024, ks=512, vs=512, cq=P, ck=P, B=2, Tq=8, Tk=8, Hq=8, Hkv=4, D=128, scale=0.1, causal=1, out=P,
+             lse=None, stream=None)
+    return tuple({**d, **c}.values())
+
+
+@pytest.mark.parametrize("name,make", [("wkv_paged_append", append_args), ("wkv_paged_evict", evict_args),
+                                       ("wattn_decode", decode_args)])
+def test_pool_refusals(name, make):
+    expect(name, make(fmt=L.WKV_FP8_UE8M0_B32), "paged cache rows are")
+    expect(name, make(fmt=L.WKV_MXFP4_B32), "paged cache rows are")
+    expect(name, make(D=96), "head dimension 64, 128 or 256")
+    expect(name, make(page=24), "multiple of 16")
+    expect(name, make(page=0), "multiple of 16")
+    expect(name, make(B=-1), "negative or empty shape")
+    expect(name, make(Hkv=0), "negative or empty shape")
+    expect(name, make(page=1 << 20, width=1 << 12), "at most 2^31 - 1 entries")
+    expect(name, make(kc=None), "missing cache or page table")
+    expect(name, make(table=None), "missing cache or page table")
+    expect(name, make(ksc=P), "bf16 rows take none")
+    expect(name, make(fmt=L.WKV_MXFP8_B32, ksc=P), "quantized rows need scales")
+    expect(name, make(vc=ODD), "16-byte aligned")
+
+
+def test_append_refusals():
+    f = "wkv_paged_append"
+    expect(f, append_args(T=-1), "negative token count")
+    expect(f, append_args(k=None), "missing input")
+    expect(f, append_args(ks=511), "16-byte aligned and hold")
+    expect(f, append_args(vs=504), "16-byte aligned and hold")
+    expect(f, append_args(v=ODD), "16-byte aligned and hold")
+    expect(f, append_args(pos=P), "token counts")
+    expect(f, append_args(T=0), None, L.WM_OK)
+    expect(f, append_args(B=0), None, L.WM_OK)
+
+
+def test_evict_refusals():
+    f = "wkv_paged_evict"
+    expect(f, evict_args(budget=0), "budget")
+    expect(f, evict_args(budget=8, recent=6, sinks=3), "budget")
+    expect(f, evict_args(recent=-1), "budget")
+    expect(f, evict_args(mass=None), "missing array")
+    expect(f, evict_args(lo=P), "array of their own")
+    expect(f, evict_args(mo=ctypes.c_void_p(1 << 21)), "both in place")
+    expect(f, evict_args(bytes=8), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, evict_args(B=0), None, L.WM_OK)
+    assert L.lib().wkv_evict_workspace_size(2, 4, 32) == 2 * 4 * 2 * 32 * 4
+    assert L.lib().wkv_evict_workspace_size(0, 4, 32) == 0
+
+
+def test_decode_refusals():
+    f = "wattn_decode"
+    expect(f, decode_args(Hq=6), "multiple of the key-value heads")
+    expect(f, decode_args(Hq=0), "multiple of the key-value heads")
+    for s in (0.0, -1.0, float("nan"), float("inf")):
+        expect(f, decode_args(scale=s), "positive and finite")
+    expect(f, decode_args(q=None), "missing input or output")
+    expect(f, decode_args(qs=1000), "4-byte aligned")
+    expect(f, decode_args(bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, decode_args(B=0), None, L.WM_OK)
+    size = L.lib().wattn_decode_workspace_size
+    assert size(2, 6, 4, 128, L.WKV_BF16, 16, 4, 0) == 0 and size(2, 8, 4, 100, L.WKV_BF16, 16, 4, 0) == 0
+    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 1) - size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 0) == 2 * 4 * 64 * 8 * 4
+
+
+def test_prompt_refusals():
+    f = "wattn_prompt"
+    expect(f, prompt_args(Hq=6), "multiple of the key-value heads")
+    expect(f, prompt_args(Tq=-1), "multiple of the key-value heads")
+    expect(f, prompt_args(D=80), "head dimension")
+    expect(f, prompt_args(scale=0.0), "positive and finite")
+    expect(f, prompt_args(out=None), "missing input or output")
+    expect(f, prompt_args(ck=None), "missing input or output")
+    expect(f, prompt_args(ks=500), "16-byte aligned and hold")
+    expect(f, prompt_args(qs=1028), "16-byte aligned and hold")
+    expect(f, prompt_args(k=ODD), "16-byte aligned and hold")
+    expect(f, prompt_args(Tq=0), None, L.WM_OK)
+
+
+def test_python_refusals():
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)    # noqa: E731
+    pool = (bf(4, 2, 16, 64), bf(4, 2, 16, 64), i32(3, 2), i32(3))
+    with pytest.raises(ValueError, match="format"):
+        W.decode_attention(bf(3, 4, 64), *pool, fmt="fp8_ue8m0")
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        W.decode_attention(bf(3, 4, 64), *pool)
+    with pytest.raises(ValueError, match="scales"):
+        W.decode_attention(bf(3, 4, 64), pool[0].to(torch.uint8), pool[1].to(torch.uint8), *pool[2:], fmt="mxfp8")
+    with pytest.raises(ValueError, match="of one shape"):
+        W.decode_attention(bf(3, 4, 64), pool[0].float(), *pool[1:])
+    with pytest.raises(ValueError, match="page_table"):
+        W.decode_attention(bf(3, 4, 64), pool[0], pool[1], pool[2].long(), pool[3])
+    with pytest.raises(ValueError, match="take no scales"):
+        W.paged_evict(pool[0], pool[1], pool[2], pool[3], None, None, pool[3], 4, k_scales=bf(1))
+    with pytest.raises(ValueError, match=r"bf16 \[tokens, heads, D\]"):
+        W.prompt_attention(bf(3, 4, 64).float(), bf(3, 2, 64), bf(3, 2, 64), i32(2))
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        W.prompt_attention(bf(3, 4, 64), bf(3, 2, 64), bf(3, 2, 64), i32(2))
+
+
+def test_paged_cache_hands_out_pages():
+    c = W.PagedKVCache(3, 2, 64, n_pages=10, page_size=16, max_pages=5, device="cpu")
+    assert c.mass is None and c.page_table.tolist() == [[-1] * 5] * 3
+    c.reserve([17, 0, 1])
+    assert c.free_pages == 7 and (c.page_table[0, :2] >= 0).all() and (c.page_table[0, 2:] == -1).all()
+    assert (c.page_table[1] == -1).all()
+    used = [p for p in c.page_table.flatten().tolist() if p >= 0]
+    assert len(set(used)) == 3 and all(0 <= p < 10 for p in used)
+    before = c.page_table.clone()
+    c.reserve([32, 0, 16])                       # already there
+    assert torch.equal(c.page_table, before) and c.free_pages == 7
+    with pytest.raises(ValueError, match="page table"):
+        c.reserve([81, 0, 0])
+    with pytest.raises(ValueError, match="out of pages"):
+        c.reserve([80, 80, 80])
+    with pytest.raises(ValueError, match="counts"):
+        c.reserve([1, 1])
+    with pytest.raises(ValueError, match="counts"):
+        c.reserve([1, -1, 0])
+    assert torch.equal(c.page_table, before) and c.free_pages == 7   # a refused call changes nothing
+    c.clear(0)
+    assert c.free_pages == 9 and (c.page_table[0] == -1).all()
+    c.reserve([80, 64, 0])
+    assert c.free_pages == 0
+
+
+def test_paged_cache_refusals():
+    for bad in (dict(dimension=96), dict(page_size=24), dict(fmt="mxfp4"), dict(batch=0), dict(n_pages=0), dict(max_pages=0)):
+        with pytest.raises(ValueError):
+            W.PagedKVCache(**{**dict(batch=1, heads=2, dimension=64, n_pages=2, device="cpu"), **bad})
+    c = W.PagedKVCache(2, 2, 64, n_pages=2, device="cpu", fmt="fp8_f32_b64")
+    assert c.key_scales.shape == (2, 2, 64, 1) and c.keys.dtype == torch.uint8
+    with pytest.raises(ValueError, match="track"):
+        c.evict(8)
+    x = torch.zeros((2, 2, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="sum of counts"):
+        c.append(x, x, [1, 2])
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        c.append(x, x)
+    assert c.offsets == [0, 0]                   # the refused call added no entry

@@ -2,7 +2,8 @@
 
 A drop-in for the hot path of baha2046/Whallm's MLX runtime: router top-k,
 permute-by-expert, the fused MXFP4 / affine-4 SwiGLU expert FFN with the
-top-k weighted combine, and the FP8/FP4 KV-cache row formats.  All arithmetic
+top-k weighted combine, the FP8/FP4 KV-cache row formats, and a paged KV
+cache with its attention.  All arithmetic
 runs in ``libwhallm_b200.so`` (hand-written sm_100a CUDA behind a C ABI,
 ``include/whallm_b200.h``); this package is the Python host side that keeps
 the reference's call signatures.
@@ -18,6 +19,7 @@ from .router import Gate, qwen_route, route, stable_topk_indices, topk_scores  #
 
 from .linear import MXFP8Linear, expand_block_scales, mx_linear  # noqa: F401
 from .loader import load_expert_layer, load_installed_experts, read_layout  # noqa: F401
-from .kvcache import MXFP8PoolingCache, PackedRows, QSAQuantizedCache  # noqa: F401
+from .attention import decode_attention, paged_append, paged_evict, prompt_attention  # noqa: F401
+from .kvcache import MXFP8PoolingCache, PackedRows, PagedKVCache, QSAQuantizedCache  # noqa: F401
 
 __version__ = "0.1.0"

@@ -24,7 +24,7 @@ WM_ERR_WORKSPACE = -4
 WM_OUT_F32, WM_OUT_BF16 = 0, 1
 WM_SCORE_SOFTMAX, WM_SCORE_SIGMOID, WM_SCORE_SQRTSOFTPLUS, WM_SCORE_NONE, WM_SCORE_SOFTMAX_BF16 = 0, 1, 2, 3, 4
 WM_UP_GATE, WM_GATE_UP = 0, 1
-WKV_FP8_F32_B64, WKV_FP8_UE8M0_B32, WKV_FP4_E4M3_B16, WKV_FP4_UE8M0_B32, WKV_MXFP8_B32, WKV_MXFP4_B32 = range(6)
+WKV_FP8_F32_B64, WKV_FP8_UE8M0_B32, WKV_FP4_E4M3_B16, WKV_FP4_UE8M0_B32, WKV_MXFP8_B32, WKV_MXFP4_B32, WKV_BF16 = range(7)
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -60,6 +60,13 @@ SIGNATURES = {
     "wkv_fp8_dequantize": [_P, _P, _I, _I, _I, _I, _P, _P],
     "wkv_dequantize": [_P, _P, _I64, _I, _I, _P, _P],
     "wkv_gather_dequantize": [_P, _P, _I64, _P, _I64, _I, _I, _P, _P],
+    "wkv_paged_append": [_P, _P, _I64, _I64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P],
+    "wkv_evict_workspace_size": [_I, _I, _I],
+    "wkv_paged_evict": [_I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ,
+                        _P],
+    "wattn_decode_workspace_size": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "wattn_decode": [_P, _I64, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _F, _P, _P, _P, _P, _SZ, _P],
+    "wattn_prompt": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
     "wmoe_router_topk": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _P],
     "wmoe_topk_scores": [_P, _P, _I, _I, _I, _I, _F, _F, _P, _P, _P],
     "wmoe_router_topk_static": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P],
@@ -77,7 +84,8 @@ SIGNATURES = {
                                  _SZ, _P],
 }
 _RESTYPE = {"w_last_error": ctypes.c_char_p, "wmoe_workspace_size": ctypes.c_size_t,
-            "wkv_scores_workspace_size": ctypes.c_size_t, "wmx_linear_workspace_size": ctypes.c_size_t}
+            "wkv_scores_workspace_size": ctypes.c_size_t, "wmx_linear_workspace_size": ctypes.c_size_t,
+            "wkv_evict_workspace_size": ctypes.c_size_t, "wattn_decode_workspace_size": ctypes.c_size_t}
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,728 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   s_j = scale q.k_j,  lse = log sum_j exp(s_j),  out = sum_j exp(s_j - lse) v_j
+//
+// for the G = Hq / Hkv query heads of each key-value head at once.  The call is
+// HBM bound: every cached row is read once, 4 D bytes (bf16) per entry and head
+// against 4 D G operations.
+//
+// Work split.  The entries of all (sequence, head) pairs form one line of units
+// of 64 keys; every CTA takes an equal share of the line, found from the
+// lengths on the device (no host copy, so a captured call follows the lengths).
+// A CTA that meets the end of a pair writes its part (running maximum, sum and
+// unnormalised output) and goes on with the next pair; a second kernel joins
+// the parts of each pair with weights 2^(m_part - m).  Ragged batches are
+// balanced to one unit, and one long sequence fills the GPU.
+//
+// A warp owns 16 keys of each unit.  It streams their rows through its own ring
+// of cp.async stages, so the main loop has no block-wide barrier; rows behind
+// the length are filled with zeros and never read.  Scores are computed as
+// K Q^T with the keys on the M side of m16n8k16 (8 query heads cost one N = 8
+// tile; padding heads to M = 16 would double the arithmetic of small groups),
+// and O^T = V^T P^T likewise: the score fragment, rounded to bf16, turns into
+// the B operand by one 8x8 transpose in registers.  Maximum, sum and output are
+// 32-bit; P is rounded to bf16 once, the type of V, an error of at most 2^-8 of
+// each weight that the sum over keys averages out.
+//
+// e4m3 rows are widened to bf16 exactly.  A key's block scales multiply its
+// partial scores, a value's block scales its weight before the rounding, so no
+// dequantized row is ever rounded.
+#include <algorithm>
+
+#include "wm_paged.cuh"
+#include "wm_tc.cuh"
+
+using wm_paged::Pool;
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kTile = 16;               // keys of a warp's tile
+constexpr int kUnit = kWarps * kTile;   // keys of a unit of work
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct DecodeArgs {
+  Pool pool;
+  const wm_bf16 *q;
+  int64_t q_stride;                     // between sequences; heads are dense
+  const int32_t *lengths;
+  int B, Hq, G, NC;                     // query heads, heads per kv head, chunks of query heads per kv head
+  float scale2;                         // scale * log2(e)
+  wm_bf16 *out;                         // [B, Hq, D]
+  float *lse;                           // [B, Hq] or null
+  float *mass;                          // [B, Hkv, capacity] or null
+  float *part_o, *part_m, *part_l;      // parts: [slots][heads of a chunk][D] and [slots][heads of a chunk]
+  float *scores;                        // [pairs][capacity][heads of a chunk], with mass only
+  int n_cta;                            // CTAs the line is split over
+};
+
+__device__ __forceinline__ int64_t units_of(const DecodeArgs &a, int b) {
+  const int64_t len = a.lengths[b], cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  return len <= 0 ? 0 : ((len < cap ? len : cap) + kUnit - 1) / kUnit;
+}
+
+// Units before sequence `upto` (all of them for upto = B), summed by one warp.
+__device__ __forceinline__ int64_t warp_units(const DecodeArgs &a, int upto) {
+  int64_t s = 0;
+  for (int b = threadIdx.x & 31; b < upto; b += 32) s += units_of(a, b);
+#pragma unroll
+  for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+  return s;
+}
+
+// CTAs that take part: each has at least one unit, so every part between a
+// pair's first and last is written.
+__device__ __forceinline__ int64_t parts_of(const DecodeArgs &a, int64_t total) {
+  return total < a.n_cta ? total : a.n_cta;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// two e4m3 codes (low half of w) -> two bf16, exact (4 significant bits, exponents -9 to 8)
+__device__ __forceinline__ uint32_t e4m3x2_bf16x2(uint32_t w) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(w)));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  return bf16x2(f.x, f.y);
+}
+
+template <int D, int FMT, int NH>
+struct Shape {
+  static constexpr int kRow = wm_paged::row_bytes(FMT, D);        // bytes of a row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kScale = wm_paged::scale_bytes(FMT, D);    // bytes of a row's scales
+  static constexpr int kBlocks = FMT == WKV_BF16 ? 1 : (FMT == WKV_FP8_F32_B64 ? D / 64 : D / 32);
+  static constexpr int kStage = 2 * kTile * (kRow + kScale);      // keys, values and their scales
+  // at least 64 KB in flight per SM with two CTAs (one for 256 x bf16)
+  static constexpr int kStages = D == 64 && FMT != WKV_BF16 ? 4 : 3;
+  static constexpr int kHeads = 8 * NH;
+  static constexpr int kMerge = kWarps * kHeads * D * 4;          // the warps' outputs when a part ends
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+};
+
+// 16-byte piece c of row r: an XOR of the piece with the row (pairs of rows for
+// 64-byte rows) spreads the eight rows of an 8x8 block over all banks.
+template <int kRow>
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+  if constexpr (kRow >= 128) return static_cast<uint32_t>(r * kRow + ((c ^ (r & 7)) << 4));
+  const uint32_t a = static_cast<uint32_t>(r * kRow + (c << 4));
+  return a ^ ((a >> 3) & 0x70u);
+}
+
+template <int D, int FMT, int NH>
+__global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
+  using S = Shape<D, FMT, NH>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i2 = (lane & 3) * 2;
+  uint8_t *ring = smem + warp * (S::kStages * S::kStage);
+  const uint32_t ring_u = wm_tc::smem_u32(ring);
+  WM_PDL_WAIT();
+  WM_PDL_LAUNCH();                                    // the join may be placed; it waits for this kernel's end
+
+  // this CTA's share [u, u_end) of the line of units
+  const int PH = a.pool.Hkv * a.NC;
+  const int64_t total = warp_units(a, a.B) * PH;
+  const int64_t n_cta = parts_of(a, total);
+  if (blockIdx.x >= n_cta) return;
+  int64_t u = total * blockIdx.x / n_cta;
+  const int64_t u_end = total * (blockIdx.x + 1) / n_cta;
+  int b = 0;
+  int64_t base = 0;                                   // line position of sequence b
+  for (int b0 = 0;; b0 += 32) {                       // the sequence that holds unit u
+    const int64_t mine = b0 + lane < a.B ? units_of(a, b0 + lane) * PH : 0;
+    int64_t s = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + s > u);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      b = b0 + l;
+      base += __shfl_sync(0xffffffffu, s - mine, l);
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, s, 31);
+  }
+
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  while (u < u_end) {
+    const int64_t nu = units_of(a, b);
+    if (nu == 0 || u >= base + nu * PH) {             // next sequence
+      base += nu * PH;
+      ++b;
+      continue;
+    }
+    const int hc = static_cast<int>((u - base) / nu);               // kv head and chunk of its query heads
+    const int64_t unit0 = (u - base) - hc * nu;
+    const int64_t unit1 = unit0 + (u_end - u) < nu ? unit0 + (u_end - u) : nu;
+    u += unit1 - unit0;
+    const int h = hc / a.NC, c = hc - h * a.NC;
+    const int64_t pair = static_cast<int64_t>(b) * PH + hc;
+    const int len = static_cast<int>(a.lengths[b] < cap ? a.lengths[b] : cap);
+    const int32_t *table = a.pool.table + static_cast<int64_t>(b) * a.pool.max_pages;
+
+    // tiles of this warp: 16 keys at (unit * 4 + warp) * 16
+    const int t0 = static_cast<int>(unit0) * kWarps + warp;
+    int n = static_cast<int>(unit1 - unit0);
+    if (n > 0 && (static_cast<int64_t>(t0) + static_cast<int64_t>(n - 1) * kWarps) * kTile >= len) --n;
+    bool bad = false;
+
+    // query fragments (the B operand: k = dimension, n = head), zero for heads past the group
+    constexpr int KS = D / 16;
+    uint32_t qf[NH][KS][2];
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) {
+      const int hg = c * S::kHeads + nh * 8 + g;
+      const wm_bf16 *qp = a.q + b * a.q_stride + static_cast<int64_t>(h * a.G + hg) * D;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        // e4m3 fragments hold four neighbouring values where bf16 ones hold two pairs eight apart
+        const int d0 = FMT == WKV_BF16 ? 16 * ks + i2 : 16 * ks + 2 * i2;
+        const int d1 = FMT == WKV_BF16 ? d0 + 8 : d0 + 2;
+        qf[nh][ks][0] = hg < a.G ? *reinterpret_cast<const uint32_t *>(qp + d0) : 0u;
+        qf[nh][ks][1] = hg < a.G ? *reinterpret_cast<const uint32_t *>(qp + d1) : 0u;
+      }
+    }
+
+    float o[D / 16][NH][4];
+    float m[NH][2], l[NH][2];
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[mt][nh][j] = 0.0f;
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) {
+      m[nh][0] = m[nh][1] = kNegInf;
+      l[nh][0] = l[nh][1] = 0.0f;
+    }
+
+    int pages = 0;                                    // lane i: page of tile (32 * block + i)
+    auto issue = [&](int i) {
+      if (i < n) {
+        if ((i & 31) == 0) {
+          const int64_t key = (static_cast<int64_t>(t0) + static_cast<int64_t>(i + lane) * kWarps) * kTile;
+          pages = i + lane < n ? table[key / a.pool.page_size] : 0;
+        }
+        int page = __shfl_sync(0xffffffffu, pages, i & 31);
+        const int key = (t0 + i * kWarps) * kTile;
+        const int rows = min(kTile, len - key);
+        const bool ok = page >= 0 && page < a.pool.n_pages;
+        bad |= !ok;
+        const int64_t row = ok ? (static_cast<int64_t>(page) * a.pool.Hkv + h) * a.pool.page_size + key % a.pool.page_size : 0;
+        const uint32_t st = ring_u + (i % S::kStages) * S::kStage;
+        const uint8_t *kp = static_cast<const uint8_t *>(a.pool.k) + row * S::kRow;
+        const uint8_t *vp = static_cast<const uint8_t *>(a.pool.v) + row * S::kRow;
+#pragma unroll
+        for (int x = 0; x < kTile * S::kChunks / 32; ++x) {
+          const int r = (x * 32 + lane) / S::kChunks, cc = (x * 32 + lane) % S::kChunks;
+          const int take = ok && r < rows ? 16 : 0;
+          const int64_t off = take ? (r * S::kChunks + cc) * 16 : 0;
+          cp16(st + swz<S::kRow>(r, cc), kp + off, take);
+          cp16(st + kTile * S::kRow + swz<S::kRow>(r, cc), vp + off, take);
+        }
+        if constexpr (S::kScale > 0) {
+          constexpr int per = kTile * S::kScale / 16; // 16-byte pieces of a tile's scales
+          const int which = lane / per, cc = lane % per;
+          if (which < 2) {
+            const int take = ok ? max(0, min(16, rows * S::kScale - cc * 16)) : 0;
+            const uint8_t *sp = static_cast<const uint8_t *>(which ? a.pool.vs : a.pool.ks) + row * S::kScale + (take ? cc * 16 : 0);
+            cp16(st + 2 * kTile * S::kRow + which * (kTile * S::kScale) + cc * 16, sp, take);
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) issue(i);
+    for (int i = 0; i < n; ++i) {
+      issue(i + S::kStages - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+      __syncwarp();
+      const uint32_t kt = ring_u + (i % S::kStages) * S::kStage, vt = kt + kTile * S::kRow;
+      const uint8_t *sc = ring + (i % S::kStages) * S::kStage + 2 * kTile * S::kRow;
+      auto scale_of = [&](int which, int r, int blk) {
+        const uint8_t *p = sc + which * (kTile * S::kScale) + r * S::kScale;
+        if constexpr (FMT == WKV_FP8_F32_B64) return reinterpret_cast<const float *>(p)[blk];
+        else return wm_e8m0(p[blk]);
+      };
+
+      // scores: rows are keys (g, g + 8), columns heads (i2, i2 + 1)
+      float s[NH][4];
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[nh][j] = 0.0f;
+      const int lr = lane & 15, lc = lane >> 4;
+      if constexpr (FMT == WKV_BF16) {
+        float s2[NH][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t f[4];
+          ldsm4(f, kt + swz<S::kRow>(lr, 2 * ks + lc));
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) mma((ks & 1) ? s2[nh] : s[nh], f, qf[nh][ks][0], qf[nh][ks][1]);
+        }
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[nh][j] += s2[nh][j];
+      } else {
+        constexpr int per = D / 16 / S::kBlocks;      // 16-value pieces of a scale block: 4 or 2
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk) {
+          float t[NH][4] = {};
+#pragma unroll
+          for (int x = 0; x < per; x += 2) {
+            const int ks = blk * per + x;
+            uint32_t f[4];
+            ldsm4(f, kt + swz<S::kRow>(lr, ks + lc));
+            // f[0], f[1]: rows g, g + 8 of piece ks; f[2], f[3]: of piece ks + 1
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t w0 = f[2 * y], w1 = f[2 * y + 1];
+              const uint32_t fa[4] = {e4m3x2_bf16x2(w0), e4m3x2_bf16x2(w1), e4m3x2_bf16x2(w0 >> 16), e4m3x2_bf16x2(w1 >> 16)};
+#pragma unroll
+              for (int nh = 0; nh < NH; ++nh) mma(t[nh], fa, qf[nh][ks + y][0], qf[nh][ks + y][1]);
+            }
+          }
+          const float s0 = scale_of(0, g, blk), s1 = scale_of(0, g + 8, blk);
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) {
+            s[nh][0] = fmaf(t[nh][0], s0, s[nh][0]);
+            s[nh][1] = fmaf(t[nh][1], s0, s[nh][1]);
+            s[nh][2] = fmaf(t[nh][2], s1, s[nh][2]);
+            s[nh][3] = fmaf(t[nh][3], s1, s[nh][3]);
+          }
+        }
+      }
+      const int key = (t0 + i * kWarps) * kTile;
+      const int rows = min(kTile, len - key);
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) {
+        s[nh][0] = g < rows ? s[nh][0] * a.scale2 : kNegInf;
+        s[nh][1] = g < rows ? s[nh][1] * a.scale2 : kNegInf;
+        s[nh][2] = g + 8 < rows ? s[nh][2] * a.scale2 : kNegInf;
+        s[nh][3] = g + 8 < rows ? s[nh][3] * a.scale2 : kNegInf;
+      }
+      if (a.scores) {
+        float *sp = a.scores + (pair * cap + key) * S::kHeads + i2;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+          if (g < rows) *reinterpret_cast<float2 *>(sp + g * S::kHeads + nh * 8) = make_float2(s[nh][0], s[nh][1]);
+          if (g + 8 < rows) *reinterpret_cast<float2 *>(sp + (g + 8) * S::kHeads + nh * 8) = make_float2(s[nh][2], s[nh][3]);
+        }
+      }
+
+      // running maximum; the output is rescaled only when some head's maximum grew
+      float mx[NH][2];
+      bool grew = false;
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x = fmaxf(s[nh][j], s[nh][j + 2]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          mx[nh][j] = fmaxf(x, m[nh][j]);
+          grew |= mx[nh][j] > m[nh][j];
+        }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float f = mx[nh][j] > m[nh][j] ? ex2(m[nh][j] - mx[nh][j]) : 1.0f;
+            l[nh][j] *= f;
+            m[nh][j] = mx[nh][j];
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) {
+              o[mt][nh][j] *= f;
+              o[mt][nh][j + 2] *= f;
+            }
+          }
+      }
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) {
+        s[nh][0] = ex2(s[nh][0] - m[nh][0]);
+        s[nh][1] = ex2(s[nh][1] - m[nh][1]);
+        s[nh][2] = ex2(s[nh][2] - m[nh][0]);
+        s[nh][3] = ex2(s[nh][3] - m[nh][1]);
+        l[nh][0] += s[nh][0] + s[nh][2];
+        l[nh][1] += s[nh][1] + s[nh][3];
+      }
+
+      // output: rows are value dimensions, columns heads
+      if constexpr (FMT == WKV_BF16) {
+        uint32_t p[NH][2];
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+          p[nh][0] = transpose8(bf16x2(s[nh][0], s[nh][1]));
+          p[nh][1] = transpose8(bf16x2(s[nh][2], s[nh][3]));
+        }
+        const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+          uint32_t f[4];
+          ldsm4t(f, vt + swz<S::kRow>(vr, 2 * mt + vc));
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) mma(o[mt][nh], f, p[nh][0], p[nh][1]);
+        }
+      } else {
+        constexpr int per = D / 16 / S::kBlocks;
+        const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk) {
+          const float s0 = scale_of(1, g, blk), s1 = scale_of(1, g + 8, blk);
+          uint32_t p[NH][2];
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) {
+            p[nh][0] = transpose8(bf16x2(s[nh][0] * s0, s[nh][1] * s0));
+            p[nh][1] = transpose8(bf16x2(s[nh][2] * s1, s[nh][3] * s1));
+          }
+#pragma unroll
+          for (int x = 0; x < per; x += 2) {
+            const int mt = blk * per + x;
+            uint32_t f[4];
+            ldsm4t(f, vt + swz<S::kRow>(vr, mt + vc));
+            // f[0], f[2]: piece mt, keys 0-7 and 8-15; f[1], f[3]: piece mt + 1.  A register holds
+            // dimensions 2g, 2g + 1 of two keys: row g of the tile is dimension 2g, row g + 8 is 2g + 1
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t w0 = __byte_perm(f[y], 0u, 0x3120), w1 = __byte_perm(f[y + 2], 0u, 0x3120);
+              const uint32_t fa[4] = {e4m3x2_bf16x2(w0), e4m3x2_bf16x2(w0 >> 16), e4m3x2_bf16x2(w1), e4m3x2_bf16x2(w1 >> 16)};
+#pragma unroll
+              for (int nh = 0; nh < NH; ++nh) mma(o[mt + y][nh], fa, p[nh][0], p[nh][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // the part of this CTA: merge the four warps
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x = l[nh][j];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        l[nh][j] = x;
+      }
+    if (bad)                                          // a page out of range: the sequence's outputs are NaN
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) l[nh][0] = l[nh][1] = __uint_as_float(0x7fc00000u);
+    if (g == 0)
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sm_m[warp][nh * 8 + i2 + j] = m[nh][j];
+          sm_l[warp][nh * 8 + i2 + j] = l[nh][j];
+        }
+    __syncthreads();                                  // all rings are drained
+    float *mg = reinterpret_cast<float *>(smem);      // [warp][head][D]
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int hd = nh * 8 + i2 + j;
+        const float top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
+        const float f = m[nh][j] == kNegInf ? (n > 0 ? 1.0f : 0.0f) : ex2(m[nh][j] - top);
+        float *row = mg + (warp * S::kHeads + hd) * D;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+          const int d0 = FMT == WKV_BF16 ? 16 * mt + g : 16 * mt + 2 * g, d1 = FMT == WKV_BF16 ? d0 + 8 : d0 + 1;
+          row[d0] = o[mt][nh][j] * f;
+          row[d1] = o[mt][nh][j + 2] * f;
+        }
+      }
+    __syncthreads();
+    const int64_t slot = blockIdx.x + pair;
+    for (int x = threadIdx.x; x < S::kHeads * D / 4; x += kWarps * 32) {
+      const float4 *p = reinterpret_cast<const float4 *>(mg) + x;
+      float4 r = p[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 y = p[w * (S::kHeads * D / 4)];
+        r.x += y.x; r.y += y.y; r.z += y.z; r.w += y.w;
+      }
+      reinterpret_cast<float4 *>(a.part_o + slot * (S::kHeads * D))[x] = r;
+    }
+    if (threadIdx.x < S::kHeads) {
+      const int hd = threadIdx.x;
+      const float top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += sm_m[w][hd] == kNegInf ? sm_l[w][hd] : sm_l[w][hd] * ex2(sm_m[w][hd] - top);
+      a.part_m[slot * S::kHeads + hd] = top;
+      a.part_l[slot * S::kHeads + hd] = sum;
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the parts of a pair: block (pair, head) for the output, and with a mass
+// array blocks (pair, kHeads + x) that add the weights of a run of keys.
+constexpr int kJoin = 128;             // threads
+constexpr int kRun = 2048;             // keys of a mass block
+
+template <int NH>
+__global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int D) {
+  constexpr int kHeads = 8 * NH;
+  __shared__ float s_lse2[kHeads];
+  const int PH = a.pool.Hkv * a.NC;
+  const int64_t pair = blockIdx.x;
+  const int b = static_cast<int>(pair / PH), hc = static_cast<int>(pair - static_cast<int64_t>(b) * PH);
+  const int h = hc / a.NC, c = hc - h * a.NC;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  WM_PDL_WAIT();
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  const int64_t total = warp_units(a, a.B) * PH, nu = units_of(a, b);
+  const int64_t first = warp_units(a, b) * PH + hc * nu;
+  const int len = a.lengths[b];
+  const bool bad = len < 0 || len > cap;
+  const float nan = __uint_as_float(0x7fc00000u);
+  // CTAs that hold units first .. first + nu - 1
+  const int64_t n_cta = parts_of(a, total);
+  const int64_t i0 = nu ? ((first + 1) * n_cta - 1) / total : 0, i1 = nu ? ((first + nu) * n_cta - 1) / total : -1;
+  const float *pm = a.part_m + (i0 + pair) * kHeads, *pl = a.part_l + (i0 + pair) * kHeads;
+  const int np = static_cast<int>(i1 - i0 + 1);
+  auto stats = [&](int hd, float &top, float &sum) {  // by one warp
+    top = kNegInf;
+    for (int i = lane; i < np; i += 32) top = fmaxf(top, pm[i * kHeads + hd]);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    sum = 0.0f;
+    for (int i = lane; i < np; i += 32) {
+      const float mi = pm[i * kHeads + hd];
+      sum += pl[i * kHeads + hd] * (mi == kNegInf ? 1.0f : ex2(mi - top));
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  };
+
+  if (blockIdx.y < kHeads) {
+    const int hd = blockIdx.y, hg = c * kHeads + hd;
+    if (hg >= a.G) return;
+    float top, sum;
+    stats(hd, top, sum);
+    const int64_t head = static_cast<int64_t>(b) * a.Hq + h * a.G + hg;
+    const float inv = bad ? nan : (np > 0 ? 1.0f / sum : 0.0f);
+    if (a.lse && threadIdx.x == 0) a.lse[head] = bad ? nan : (np > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
+    const float *po = a.part_o + ((i0 + pair) * kHeads + hd) * D;
+    for (int d = threadIdx.x * 2; d < D; d += kJoin * 2) {
+      float x = 0.0f, y = 0.0f;
+      for (int i = 0; i < np; ++i) {
+        const float mi = pm[i * kHeads + hd];
+        const float f = mi == kNegInf ? 1.0f : ex2(mi - top);
+        const float2 v = *reinterpret_cast<const float2 *>(po + static_cast<int64_t>(i) * kHeads * D + d);
+        x = fmaf(v.x, f, x);
+        y = fmaf(v.y, f, y);
+      }
+      reinterpret_cast<uint32_t *>(a.out + head * D + d)[0] = bf16x2(x * inv, y * inv);
+    }
+    return;
+  }
+  // mass: sum over the kv head's query heads; one chunk at a time adds (chunk 0's block does all of them)
+  const int64_t k0 = static_cast<int64_t>(blockIdx.y - kHeads) * kRun;
+  if (c != 0 || bad || k0 >= len) return;
+  const int64_t k1 = k0 + kRun < len ? k0 + kRun : len;
+  float *mass = a.mass + (static_cast<int64_t>(b) * a.pool.Hkv + h) * cap;
+  float acc[kRun / kJoin];
+#pragma unroll
+  for (int x = 0; x < kRun / kJoin; ++x) acc[x] = 0.0f;
+  for (int cc = 0; cc < a.NC; ++cc) {
+    const int64_t f2 = first + cc * nu;
+    const int64_t j0 = ((f2 + 1) * n_cta - 1) / total, j1 = ((f2 + nu) * n_cta - 1) / total;
+    const float *qm = a.part_m + (j0 + pair + cc) * kHeads, *ql = a.part_l + (j0 + pair + cc) * kHeads;
+    const int nq = static_cast<int>(j1 - j0 + 1);
+    __syncthreads();
+    for (int hd = warp; hd < kHeads; hd += kJoin / 32) {
+      float top = kNegInf, sum = 0.0f;
+      for (int i = lane; i < nq; i += 32) top = fmaxf(top, qm[i * kHeads + hd]);
+#pragma unroll
+      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int i = lane; i < nq; i += 32) {
+        const float mi = qm[i * kHeads + hd];
+        sum += ql[i * kHeads + hd] * (mi == kNegInf ? 1.0f : ex2(mi - top));
+      }
+#pragma unroll
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane == 0) s_lse2[hd] = top + log2f(sum);
+    }
+    __syncthreads();
+    const int live = min(kHeads, a.G - cc * kHeads);
+    const float *sc = a.scores + (pair + cc) * cap * kHeads;
+#pragma unroll
+    for (int x = 0; x < kRun / kJoin; ++x) {
+      const int64_t key = k0 + x * kJoin + threadIdx.x;
+      if (key < k1)
+        for (int hd = 0; hd < live; ++hd) acc[x] += ex2(sc[key * kHeads + hd] - s_lse2[hd]);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < kRun / kJoin; ++x) {
+    const int64_t key = k0 + x * kJoin + threadIdx.x;
+    if (key < k1) mass[key] += acc[x];
+  }
+}
+
+int chunk_heads(int G) { return G <= 8 ? 8 : 16; }
+
+// CTAs the line of units is split over: what fits on the GPU at once, and no
+// more than there are units when every sequence is at capacity.
+template <int D, int FMT, int NH>
+int grid_of(int64_t most_units) {
+  using S = Shape<D, FMT, NH>;
+  const int per_sm = std::max(1, std::min(4, (225 * 1024) / (S::kSmem + 1024 + 8 * S::kHeads * kWarps)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most_units, static_cast<int64_t>(per_sm) * wm::sm_count())));
+}
+
+template <int D, int FMT, int NH>
+int launch(DecodeArgs &a, cudaStream_t stream) {
+  using S = Shape<D, FMT, NH>;
+  auto kern = k_attn_decode<D, FMT, NH>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e == cudaSuccess) e = wm::launch_pdl(kern, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  const unsigned runs = a.mass ? static_cast<unsigned>((cap + kRun - 1) / kRun) : 0u;
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC), S::kHeads + runs);
+  e = wm::launch_pdl(k_attn_join<NH>, grid, dim3(kJoin), 0, stream, a, D);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
+  return wm::check_launch("wattn_decode");
+}
+
+// Runs f.template operator()<D, FMT, NH>() for the call's shape.
+template <typename F>
+auto dispatch(int D, int fmt, int G, F &&f) {
+#define WM_ATTN_NH(d, x) return G <= 8 ? f.template operator()<d, x, 1>() : f.template operator()<d, x, 2>()
+#define WM_ATTN_FMT(d)                                          \
+  if (fmt == WKV_BF16) WM_ATTN_NH(d, WKV_BF16);                 \
+  if (fmt == WKV_FP8_F32_B64) WM_ATTN_NH(d, WKV_FP8_F32_B64);   \
+  WM_ATTN_NH(d, WKV_MXFP8_B32)
+  if (D == 64) { WM_ATTN_FMT(64); }
+  if (D == 128) { WM_ATTN_FMT(128); }
+  WM_ATTN_FMT(256);
+#undef WM_ATTN_FMT
+#undef WM_ATTN_NH
+}
+
+struct GridOf {
+  int64_t most;
+  template <int D, int FMT, int NH>
+  int operator()() const { return grid_of<D, FMT, NH>(most); }
+};
+struct Launch {
+  DecodeArgs &a;
+  cudaStream_t stream;
+  template <int D, int FMT, int NH>
+  int operator()() const { return launch<D, FMT, NH>(a, stream); }
+};
+
+struct Plan {
+  int NC, heads, n_cta;
+  int64_t pairs, slots, cap;
+  size_t off_m, off_l, off_s, bytes;
+};
+
+Plan plan_of(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages, bool with_mass) {
+  Plan p{};
+  const int G = Hq / Hkv;
+  p.heads = chunk_heads(G);
+  p.NC = (G + p.heads - 1) / p.heads;
+  p.pairs = static_cast<int64_t>(B) * Hkv * p.NC;
+  p.cap = static_cast<int64_t>(max_pages) * page_size;
+  p.n_cta = dispatch(D, fmt, G, GridOf{p.pairs * ((p.cap + kUnit - 1) / kUnit)});
+  p.slots = p.n_cta + p.pairs;
+  auto up = [](size_t x) { return (x + 255) & ~size_t{255}; };
+  p.off_m = up(static_cast<size_t>(p.slots) * p.heads * D * 4);
+  p.off_l = p.off_m + up(static_cast<size_t>(p.slots) * p.heads * 4);
+  p.off_s = p.off_l + up(static_cast<size_t>(p.slots) * p.heads * 4);
+  p.bytes = p.off_s + (with_mass ? static_cast<size_t>(p.pairs) * p.cap * p.heads * 4 : 0);
+  return p;
+}
+
+bool shape_ok(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages) {
+  return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && (D == 64 || D == 128 || D == 256) && wm_paged::is_paged_fmt(fmt) &&
+         page_size > 0 && max_pages >= 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t wattn_decode_workspace_size(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages, int with_mass) {
+  if (!shape_ok(B, Hq, Hkv, D, fmt, page_size, max_pages)) return 0;
+  return plan_of(B, Hq, Hkv, D, fmt, page_size, max_pages, with_mass != 0).bytes;
+}
+
+int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int D, const void *k_cache, const void *v_cache,
+                 const void *k_scales, const void *v_scales, int fmt, int n_pages, int page_size, const int32_t *page_table,
+                 int max_pages, const int32_t *lengths, float scale, wm_bf16 *out, float *lse, float *mass, void *workspace,
+                 size_t ws_bytes, wm_stream_t stream) {
+  wm::clear_error();
+  Pool pool{const_cast<void *>(k_cache), const_cast<void *>(v_cache), const_cast<void *>(k_scales),
+            const_cast<void *>(v_scales), page_table, n_pages, page_size, max_pages, Hkv};
+  if (int rc = wm_paged::check_pool(pool, B, D, fmt)) return rc;
+  WM_REQUIRE(Hq > 0 && Hq % Hkv == 0, "decode attention: the query heads must be a multiple of the key-value heads");
+  WM_REQUIRE(scale > 0.0f && scale <= 3.4028234663852886e38f, "decode attention: the scale must be positive and finite");
+  if (B == 0) return WM_OK;
+  WM_REQUIRE(q && lengths && out, "decode attention: missing input or output");
+  WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && q_stride % 2 == 0 && wm::aligned(q, 4) && wm::aligned(out, 4),
+             "decode attention: query rows must be 4-byte aligned and hold Hq * D values");
+  const Plan p = plan_of(B, Hq, Hkv, D, fmt, page_size, max_pages, mass != nullptr);
+  WM_REQUIRE(p.pairs <= INT32_MAX && (p.cap + kRun - 1) / kRun <= 65000, "decode attention: batch or capacity too large");
+  if (ws_bytes < p.bytes) return wm::fail(WM_ERR_WORKSPACE, "decode attention: workspace too small");
+  WM_REQUIRE(workspace && wm::aligned(workspace, 256), "decode attention: the workspace must be 256-byte aligned");
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  DecodeArgs a{pool, q, q_stride, lengths, B, Hq, Hq / Hkv, p.NC, scale * kLog2e, out, lse, mass,
+               reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + p.off_m), reinterpret_cast<float *>(ws + p.off_l),
+               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.n_cta};
+  return dispatch(D, fmt, a.G, Launch{a, stream});
+}
+
+}  // extern "C"

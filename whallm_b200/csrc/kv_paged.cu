@@ -1,0 +1,399 @@
+// Paged key-value cache: append (bf16 or quantized rows) and eviction by
+// accumulated attention weight.  Compiled with -fmad=false, as formats.cu: the
+// quantized rows are the bytes of wkv_quantize.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "wm_kvfp8.cuh"
+#include "wm_paged.cuh"
+
+namespace cg = cooperative_groups;
+using wm_paged::Pool;
+
+namespace {
+
+// ------------------------------------------------------------------ append --
+//
+// One thread moves 16 values (two 16-byte loads) of a token's key or value row
+// to its slot; a quantized row's scale blocks are 2 or 4 adjacent lanes, as in
+// k_kv_fp8_quantize.  A token finds its sequence by binary search in
+// cu_seqlens: a step of at most ~10 cached loads that hides under the row's own
+// loads.  HBM bound: 2 B read and 2 B (1 B + scale) written per value.
+
+template <int FMT>
+__global__ void __launch_bounds__(256) k_paged_append(const wm_bf16 *__restrict__ k, const wm_bf16 *__restrict__ v,
+                                                      int64_t k_stride, int64_t v_stride, int64_t n16, int per_tok,
+                                                      int per_row, const int32_t *__restrict__ cu, int B,
+                                                      const int32_t *__restrict__ lengths, Pool pool,
+                                                      float *__restrict__ mass, int32_t *__restrict__ positions,
+                                                      const int32_t *__restrict__ seen) {
+  const bool is_v = blockIdx.y != 0;
+  const wm_bf16 *src = is_v ? v : k;
+  const int64_t stride = is_v ? v_stride : k_stride;
+  uint8_t *cache = static_cast<uint8_t *>(is_v ? pool.v : pool.k);
+  void *scales = is_v ? pool.vs : pool.ks;
+  const int lane = threadIdx.x & 31;
+  constexpr int G = FMT == WKV_BF16 ? 1 : wm_kv::Fp8Fmt<FMT == WKV_BF16 ? WKV_MXFP8_B32 : FMT>::kG / 2;
+  const unsigned gmask = ((1u << G) - 1u) << (lane & ~(G - 1));
+  // the G lanes of a scale block hold one row: they take every branch together
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n16; i += (int64_t)gridDim.x * blockDim.x) {
+    const int t = static_cast<int>(i / per_tok);
+    const int c = static_cast<int>(i - static_cast<int64_t>(t) * per_tok);
+    const int h = c / per_row, cr = c - h * per_row;
+    const uint4 *p = reinterpret_cast<const uint4 *>(src + t * stride) + 2 * c;
+    const uint4 u[2] = {__ldcs(p), __ldcs(p + 1)};
+    // the last b with cu[b] <= t
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
+    }
+    const int b = lo, end = __ldg(cu + b + 1);
+    if (t < __ldg(cu + b) || t >= end) continue;       // behind the last sequence: not a token
+    const int64_t e = static_cast<int64_t>(__ldg(lengths + b)) - (end - t);
+    const int64_t cap = static_cast<int64_t>(pool.max_pages) * pool.page_size;
+    if (e < 0 || e >= cap) continue;
+    const int pi = static_cast<int>(e / pool.page_size), slot = static_cast<int>(e - static_cast<int64_t>(pi) * pool.page_size);
+    const int page = __ldg(pool.table + static_cast<int64_t>(b) * pool.max_pages + pi);
+    if (page < 0 || page >= pool.n_pages) continue;
+    const int64_t row = (static_cast<int64_t>(page) * pool.Hkv + h) * pool.page_size + slot;
+    const int64_t chunk = row * per_row + cr;
+    if constexpr (FMT == WKV_BF16) {
+      uint4 *d = reinterpret_cast<uint4 *>(cache) + 2 * chunk;
+      d[0] = u[0];
+      d[1] = u[1];
+    } else {
+      wm_kv::kv_fp8_quant<FMT, 16>(u, chunk, gmask, lane, cache, scales);
+    }
+    if (!is_v && cr == 0) {
+      const int64_t at = (static_cast<int64_t>(b) * pool.Hkv + h) * cap + e;
+      if (mass) mass[at] = 0.0f;
+      if (positions) positions[at] = __ldg(seen + b) - (end - t);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- evict --
+//
+// One cluster of CTAs per (sequence, head).  Every entry gets a 32-bit key
+// whose unsigned order is (protected, weight); the budget-th largest key is
+// found by a radix select of three digits (11, 11 and 10 bits), its ties go to
+// the lowest entries, and the r-th kept entry behind the budget moves into the
+// r-th hole before it.  Attention does not depend on the order of its keys, so
+// nothing that stays is copied, sources and destinations never overlap, and no
+// move waits for another.  The CTAs of a cluster hold a slice of the keys each
+// in shared memory and add their digit counts over distributed shared memory:
+// weights and positions are read from memory once.
+// Bound by the latency of its eight cluster-wide steps for short caches, by the
+// reads of weights and positions and by the moved rows for long ones.
+
+constexpr int kET = 512;           // threads
+constexpr int kBins = 2048;        // bins of a digit
+constexpr int kKeySmem = 40960;    // keys held per CTA (160 KB); longer slices read them again
+
+struct EvictArgs {
+  Pool pool;
+  const int32_t *lengths, *seen;
+  const float *mass;
+  const int32_t *positions;
+  float *mass_out;
+  int32_t *positions_out, *lengths_out;
+  int32_t *lists;                  // [B * Hkv][2][budget]: holes, then tails
+  int budget, recent, sinks, row16, scale_bytes, key_cap;
+};
+
+__device__ __forceinline__ uint32_t evict_key(float m, int32_t pos, int32_t from, int32_t sinks) {
+  if (pos >= from || pos < sinks) return 0xffffffffu;
+  if (m != m) return 0xfffffffeu;
+  const uint32_t u = __float_as_uint(m + 0.0f);        // -0 becomes +0
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+
+// Exclusive sum over the block's threads; *total gets the whole sum.
+__device__ __forceinline__ int block_scan(int x, int *warp_sums, int *total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int s = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += o;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[w] = s;
+  __syncthreads();
+  int base = 0, all = 0;
+#pragma unroll
+  for (int j = 0; j < kET / 32; ++j) {
+    const int v = warp_sums[j];
+    if (j < w) base += v;
+    all += v;
+  }
+  *total = all;
+  return base + s - x;
+}
+
+__global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
+  extern __shared__ uint32_t sk[];                     // [key_cap] keys of this CTA's slice
+  __shared__ uint32_t hist[2][kBins];
+  __shared__ int warp_sums[kET / 32];
+  __shared__ int counts[4];                            // this CTA's ties, holes, tails
+  __shared__ int pick[2];                              // chosen digit, keys above it
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), C = static_cast<int>(cluster.num_blocks());
+  const int bh = static_cast<int>(blockIdx.x) / C, b = bh / a.pool.Hkv, h = bh - b * a.pool.Hkv;
+  const int tid = threadIdx.x;
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  const int len = a.lengths[b];
+  const int n = a.budget;
+  const int32_t *table = a.pool.table + static_cast<int64_t>(b) * a.pool.max_pages;
+  const float *mass = a.mass + bh * cap;
+  const int32_t *pos = a.positions + bh * cap;
+  float *mass_out = a.mass_out + bh * cap;
+  int32_t *pos_out = a.positions_out + bh * cap;
+
+  // a length or a page out of range leaves the sequence as it is
+  bool bad = len < 0 || len > cap;
+  if (!bad) {
+    const int np = (len + a.pool.page_size - 1) / a.pool.page_size;
+    for (int i = tid; i < np; i += kET) bad |= table[i] < 0 || table[i] >= a.pool.n_pages;
+  }
+  bad = __syncthreads_or(bad);
+  const int live = bad ? (len < 0 ? 0 : static_cast<int>(len < cap ? len : cap)) : len;
+  const bool copy = mass_out != mass;
+  if (bad || len <= n) {
+    if (copy)
+      for (int i = rank * kET + tid; i < live; i += C * kET) {
+        mass_out[i] = mass[i];
+        pos_out[i] = pos[i];
+      }
+    if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = len;
+    return;                                            // every CTA of the cluster returns here together
+  }
+  if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = n;
+
+  // this CTA's slice of the entries
+  const int S = ((len + C - 1) / C + 3) & ~3;
+  const int s0 = min(rank * S, len), s1 = min(s0 + S, len);
+  const int32_t from = a.seen[b] - a.recent;
+  const bool held = S <= a.key_cap;
+  auto key_at = [&](int i) { return held ? sk[i - s0] : evict_key(mass[i], pos[i], from, a.sinks); };
+  for (int i = tid; i < kBins; i += kET) hist[0][i] = 0u;
+  __syncthreads();
+  for (int i = s0 + tid; i < s1; i += kET) {
+    const float m = mass[i];
+    const int32_t p = pos[i];
+    const uint32_t key = evict_key(m, p, from, a.sinks);
+    if (held) sk[i - s0] = key;
+    if (copy && i < n) {                               // a hole's copy is replaced after the last barrier
+      mass_out[i] = m;
+      pos_out[i] = p;
+    }
+    atomicAdd(&hist[0][key >> 21], 1u);
+  }
+
+  // radix select of the n-th largest key
+  uint32_t prefix = 0u, mask = 0u;
+  int need = n;
+  const int shifts[3] = {21, 10, 0};
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = shifts[pass];
+    uint32_t *hc = hist[pass & 1];
+    if (pass > 0) {
+      const uint32_t dm = pass == 1 ? 2047u : 1023u;
+      for (int i = s0 + tid; i < s1; i += kET) {
+        const uint32_t key = key_at(i);
+        if ((key & mask) == prefix) atomicAdd(&hc[(key >> shift) & dm], 1u);
+      }
+    }
+    uint32_t *hn = hist[(pass + 1) & 1];               // last read two barriers ago
+    cluster.sync();
+    if (pass < 2)
+      for (int i = tid; i < kBins; i += kET) hn[i] = 0u;
+    // thread t holds bins 2047 - 4t down to 2044 - 4t
+    const int at = kBins / 4 - 1 - tid;
+    uint4 sum = make_uint4(0u, 0u, 0u, 0u);
+    for (int r = 0; r < C; ++r) {
+      const uint4 x = reinterpret_cast<const uint4 *>(cluster.map_shared_rank(hc, r))[at];
+      sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+    }
+    const int c4[4] = {static_cast<int>(sum.w), static_cast<int>(sum.z), static_cast<int>(sum.y), static_cast<int>(sum.x)};
+    int total, before = block_scan(c4[0] + c4[1] + c4[2] + c4[3], warp_sums, &total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (before < need && need <= before + c4[j]) {
+        pick[0] = 4 * at + 3 - j;
+        pick[1] = before;
+      }
+      before += c4[j];
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(pick[0]) << shift;
+    mask |= (pass == 2 ? 1023u : 2047u) << shift;
+    need -= pick[1];
+  }
+  // keys above prefix stay, and the first `need` entries whose key is prefix
+
+  // ranks: each thread walks a run of consecutive entries
+  const int E = (s1 - s0 + kET - 1) / kET;
+  const int r0 = min(s0 + tid * E, s1), r1 = min(r0 + E, s1);
+  int ties = 0;
+  for (int i = r0; i < r1; ++i) ties += key_at(i) == prefix;
+  int total_ties, tie0 = block_scan(ties, warp_sums, &total_ties);
+  if (tid == 0) counts[0] = total_ties;
+  cluster.sync();
+  for (int r = 0; r < rank; ++r) tie0 += *cluster.map_shared_rank(&counts[0], r);
+  int holes = 0, tails = 0, tr = tie0;
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t key = key_at(i);
+    const bool keep = key > prefix || (key == prefix && tr++ < need);
+    holes += i < n && !keep;
+    tails += i >= n && keep;
+  }
+  int total_holes, total_tails;
+  int hole0 = block_scan(holes, warp_sums, &total_holes);
+  int tail0 = block_scan(tails, warp_sums, &total_tails);
+  if (tid == 0) {
+    counts[1] = total_holes;
+    counts[2] = total_tails;
+  }
+  cluster.sync();
+  int moves = 0;
+  for (int r = 0; r < C; ++r) {
+    const int x = *cluster.map_shared_rank(&counts[1], r);
+    const int y = *cluster.map_shared_rank(&counts[2], r);
+    if (r < rank) {
+      hole0 += x;
+      tail0 += y;
+    }
+    moves += x;
+  }
+  int32_t *hl = a.lists + static_cast<int64_t>(bh) * 2 * n, *tl = hl + n;
+  tr = tie0;
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t key = key_at(i);
+    const bool keep = key > prefix || (key == prefix && tr++ < need);
+    if (i < n && !keep) hl[hole0++] = i;
+    if (i >= n && keep) tl[tail0++] = i;
+  }
+  cluster.sync();                                      // also: no CTA leaves while its counts are read
+
+  const int ct = rank * kET + tid, CT = C * kET;
+  for (int r = ct; r < moves; r += CT) {
+    const int d = hl[r], s = tl[r];
+    mass_out[d] = mass[s];
+    pos_out[d] = pos[s];
+  }
+  auto row_of = [&](int e) {
+    const int pi = e / a.pool.page_size;
+    return (static_cast<int64_t>(table[pi]) * a.pool.Hkv + h) * a.pool.page_size + (e - pi * a.pool.page_size);
+  };
+  const int per = 2 * a.row16;                         // 16-byte pieces of a move: the key row's, then the value row's
+  const int64_t items = static_cast<int64_t>(moves) * per;
+  for (int64_t j = ct; j < items; j += CT) {
+    const int r = static_cast<int>(j / per);
+    int c = static_cast<int>(j - static_cast<int64_t>(r) * per);
+    uint4 *base = static_cast<uint4 *>(c < a.row16 ? a.pool.k : a.pool.v);
+    c = c < a.row16 ? c : c - a.row16;
+    base[row_of(hl[r]) * a.row16 + c] = base[row_of(tl[r]) * a.row16 + c];
+  }
+  if (a.scale_bytes) {
+    const int per2 = a.scale_bytes;                    // 2-byte pieces of both rows' scales
+    const int half = per2 / 2;
+    const int64_t sitems = static_cast<int64_t>(moves) * per2;
+    for (int64_t j = ct; j < sitems; j += CT) {
+      const int r = static_cast<int>(j / per2);
+      int c = static_cast<int>(j - static_cast<int64_t>(r) * per2);
+      uint16_t *base = static_cast<uint16_t *>(c < half ? a.pool.ks : a.pool.vs);
+      c = c < half ? c : c - half;
+      base[row_of(hl[r]) * half + c] = base[row_of(tl[r]) * half + c];
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride, int64_t v_stride, const int32_t *cu_seqlens,
+                     int T, int B, int Hkv, int D, void *k_cache, void *v_cache, void *k_scales, void *v_scales, int fmt,
+                     int n_pages, int page_size, const int32_t *page_table, int max_pages, const int32_t *lengths,
+                     float *mass, int32_t *positions, const int32_t *seen, wm_stream_t stream) {
+  wm::clear_error();
+  const Pool pool{k_cache, v_cache, k_scales, v_scales, page_table, n_pages, page_size, max_pages, Hkv};
+  if (int rc = wm_paged::check_pool(pool, B, D, fmt)) return rc;
+  WM_REQUIRE(T >= 0, "paged append: negative token count");
+  if (T == 0 || B == 0) return WM_OK;
+  WM_REQUIRE(k && v && cu_seqlens && lengths, "paged append: missing input");
+  WM_REQUIRE(k_stride >= static_cast<int64_t>(Hkv) * D && v_stride >= static_cast<int64_t>(Hkv) * D && k_stride % 8 == 0 &&
+                 v_stride % 8 == 0 && wm::aligned(k, 16) && wm::aligned(v, 16),
+             "paged append: token rows must be 16-byte aligned and hold Hkv * D values");
+  WM_REQUIRE(!positions || seen, "paged append: positions need the sequences' token counts");
+  const int per_row = D / 16, per_tok = Hkv * per_row;
+  const int64_t n16 = static_cast<int64_t>(T) * per_tok;
+  const int64_t want = (n16 + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, static_cast<int64_t>(wm::sm_count()) * 16)), 2);
+#define WM_APPEND(F)                                                                                                  \
+  k_paged_append<F><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, per_row, cu_seqlens, B, lengths, \
+                                              pool, mass, positions, seen)
+  if (fmt == WKV_BF16) WM_APPEND(WKV_BF16);
+  else if (fmt == WKV_FP8_F32_B64) WM_APPEND(WKV_FP8_F32_B64);
+  else WM_APPEND(WKV_MXFP8_B32);
+#undef WM_APPEND
+  return wm::check_launch("wkv_paged_append");
+}
+
+size_t wkv_evict_workspace_size(int B, int Hkv, int budget) {
+  if (B <= 0 || Hkv <= 0 || budget <= 0) return 0;
+  return static_cast<size_t>(B) * Hkv * 2 * budget * sizeof(int32_t);
+}
+
+int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k_scales, void *v_scales, int fmt, int n_pages,
+                    int page_size, const int32_t *page_table, int max_pages, const int32_t *lengths, const int32_t *seen,
+                    const float *mass, const int32_t *positions, int budget, int recent, int sinks, float *mass_out,
+                    int32_t *positions_out, int32_t *lengths_out, void *workspace, size_t ws_bytes, wm_stream_t stream) {
+  wm::clear_error();
+  const Pool pool{k_cache, v_cache, k_scales, v_scales, page_table, n_pages, page_size, max_pages, Hkv};
+  if (int rc = wm_paged::check_pool(pool, B, D, fmt)) return rc;
+  WM_REQUIRE(budget > 0 && recent >= 0 && sinks >= 0 && static_cast<int64_t>(recent) + sinks <= budget,
+             "evict: the budget must be positive and hold the recent and the first positions");
+  if (B == 0) return WM_OK;
+  WM_REQUIRE(lengths && seen && mass && positions && mass_out && positions_out && lengths_out, "evict: missing array");
+  WM_REQUIRE(lengths_out != lengths, "evict: the new lengths need an array of their own");
+  WM_REQUIRE((mass_out == mass) == (positions_out == positions), "evict: weights and positions are both in place or both not");
+  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
+  const int n = static_cast<int>(std::min<int64_t>(budget, std::max<int64_t>(cap, 1)));
+  if (ws_bytes < wkv_evict_workspace_size(B, Hkv, n)) return wm::fail(WM_ERR_WORKSPACE, "evict: workspace too small");
+  WM_REQUIRE(workspace && wm::aligned(workspace, 4), "evict: missing workspace");
+  const int64_t heads = static_cast<int64_t>(B) * Hkv;
+  // CTAs per (sequence, head): enough to fill the GPU, at least 2048 entries each, at most a portable cluster
+  int C = 1;
+  while (C < 8 && heads * C * 2 <= 2 * wm::sm_count() && cap > 2048 * C) C *= 2;
+  const int64_t slice = ((cap + C - 1) / C + 3) & ~int64_t{3};
+  const int key_cap = static_cast<int>(std::min<int64_t>(slice, kKeySmem));
+  const size_t smem = static_cast<size_t>(key_cap) * 4;
+  WM_REQUIRE(heads * C <= INT32_MAX, "evict: too many sequences");
+  cudaError_t e = cudaFuncSetAttribute(k_paged_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeySmem * 4);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wkv_paged_evict: ") + cudaGetErrorString(e));
+  const EvictArgs args{pool, lengths, seen, mass, positions, mass_out, positions_out, lengths_out,
+                       static_cast<int32_t *>(workspace), n, recent, sinks, wm_paged::row_bytes(fmt, D) / 16,
+                       wm_paged::scale_bytes(fmt, D), key_cap};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(heads * C));
+  cfg.blockDim = dim3(kET);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(C);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, k_paged_evict, args);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wkv_paged_evict: ") + cudaGetErrorString(e));
+  return wm::check_launch("wkv_paged_evict");
+}
+
+}  // extern "C"

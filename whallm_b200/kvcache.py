@@ -1,4 +1,7 @@
-"""Qwen QSA affine-quantized KV cache on the device.
+"""KV caches on the device: Qwen QSA affine-quantized, V4.1 packed rows, MXFP8
+pooled and paged.
+
+Qwen QSA affine-quantized KV cache.
 
 Mirrors ``QSAQuantizedCache`` (runtime/deepseek_v4_ssd/qwen_quantized_cache.py:6-57),
 itself mlx-lm's ``QuantizedKVCache`` with group 32 and 4 or 8 bits: every
@@ -411,3 +414,139 @@ class MXFP8PoolingCache:
         self.previous_window_kv, self.previous_window_gate = previous_kv, previous_gate
         if pooled is not None:
             self.update_and_fetch(pooled)
+
+
+# --------------------------------------------------------------------------
+# Paged cache: sequences of different lengths in one pool of pages
+# --------------------------------------------------------------------------
+
+from . import attention as _A  # noqa: E402
+
+
+class PagedKVCache:
+    """Keys and values of up to ``batch`` sequences in one pool of ``n_pages``
+    pages of ``page_size`` entries, read by ``attention.decode_attention``.
+
+    ``fmt`` is a format of ``attention.PAGED_FORMATS``; with ``track`` every
+    entry also has its position and the attention weight it received (``mass``),
+    by which ``evict`` reduces the sequences to a budget.  Pages are handed out
+    and taken back on the host; the device holds ``page_table``, ``lengths`` and
+    ``seen`` (tokens of each sequence, evicted ones included), which the kernels
+    read.  Unused table entries are -1.
+
+    ``append`` and ``evict`` change host state, so a captured step calls
+    ``attention.paged_append`` and ``decode_attention`` on these tensors instead,
+    over pages handed out beforehand with ``reserve``."""
+
+    def __init__(self, batch: int, heads: int, dimension: int, n_pages: int, page_size: int = 64,
+                 max_pages: int | None = None, fmt: str = "bf16", track: bool = False, device="cuda"):
+        if fmt not in _A.PAGED_FORMATS:
+            raise ValueError(f"paged cache format must be one of {sorted(_A.PAGED_FORMATS)}, got {fmt!r}")
+        if dimension not in (64, 128, 256) or page_size <= 0 or page_size % 16:
+            raise ValueError("paged cache needs a head dimension of 64, 128 or 256 and a page size divisible by 16")
+        if batch <= 0 or heads <= 0 or n_pages <= 0 or (max_pages is not None and max_pages <= 0):
+            raise ValueError("paged cache needs sequences, heads and pages")
+        self.batch, self.heads, self.dimension, self.page_size, self.fmt = batch, heads, dimension, page_size, fmt
+        self.max_pages = n_pages if max_pages is None else max_pages
+        dt = torch.bfloat16 if fmt == "bf16" else torch.uint8
+        rows = (n_pages, heads, page_size)
+        self.keys, self.values = (torch.empty((*rows, dimension), dtype=dt, device=device) for _ in range(2))
+        self.key_scales = self.value_scales = None
+        if fmt != "bf16":
+            sdt, blk = (torch.float32, 64) if fmt == "fp8_f32_b64" else (torch.uint8, 32)
+            self.key_scales, self.value_scales = (torch.empty((*rows, dimension // blk), dtype=sdt, device=device)
+                                                  for _ in range(2))
+        self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)
+        cap = (batch, heads, self.max_pages * page_size)
+        self.mass = torch.zeros(cap, dtype=torch.float32, device=device) if track else None
+        self.positions = torch.zeros(cap, dtype=torch.int32, device=device) if track else None
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._pages = [[] for _ in range(batch)]
+        self._len = [0] * batch
+        self._seen = [0] * batch
+
+    # -------------------------------------------------------------- pages --
+    @property
+    def offsets(self):
+        """Entries of each sequence."""
+        return list(self._len)
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _write_table(self, rows):
+        for b in rows:
+            row = self._pages[b] + [-1] * (self.max_pages - len(self._pages[b]))
+            self.page_table[b].copy_(torch.tensor(row, dtype=torch.int32))
+
+    def reserve(self, counts):
+        """Hand out the pages that ``counts[b]`` more entries of each sequence need."""
+        if len(counts) != self.batch or any(int(n) != n or n < 0 for n in counts):
+            raise ValueError("counts must give every sequence a number of new entries")
+        need = [-(-(n + int(c)) // self.page_size) for n, c in zip(self._len, counts)]
+        if max(need) > self.max_pages:
+            raise ValueError("a sequence would exceed its page table")
+        more = [max(0, n - len(p)) for n, p in zip(need, self._pages)]
+        if sum(more) > len(self._free):
+            raise ValueError("the paged cache is out of pages")
+        for b, n in enumerate(more):
+            self._pages[b] += [self._free.pop() for _ in range(n)]
+        self._write_table([b for b, n in enumerate(more) if n])
+
+    def clear(self, sequence: int):
+        """Forget a sequence and take back its pages."""
+        self._free += reversed(self._pages[sequence])
+        self._pages[sequence] = []
+        self._len[sequence] = self._seen[sequence] = 0
+        self._write_table([sequence])
+        self.lengths[sequence] = 0
+        self.seen[sequence] = 0
+
+    # ---------------------------------------------------------- operators --
+    def append(self, keys: torch.Tensor, values: torch.Tensor, counts=None):
+        """Add tokens bf16 [T, heads, D], packed by sequence: ``counts[b]`` of
+        sequence b (default: one each)."""
+        counts = [1] * self.batch if counts is None else [int(c) for c in counts]
+        if keys.shape != values.shape or tuple(keys.shape) != (sum(counts), self.heads, self.dimension):
+            raise ValueError("keys and values must be [sum of counts, heads, D] of the cache")
+        self.reserve(counts)
+        dev = self.lengths.device
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        cu = torch.tensor(cu, dtype=torch.int32).to(dev)
+        new = cu[1:] - cu[:-1]
+        lengths, seen = self.lengths + new, self.seen + new
+        _A.paged_append(keys, values, cu, self.keys, self.values, self.page_table, lengths, self.fmt, self.key_scales,
+                        self.value_scales, self.mass, self.positions, seen)
+        self.lengths.copy_(lengths)
+        self.seen.copy_(seen)
+        self._len = [n + c for n, c in zip(self._len, counts)]
+        self._seen = [n + c for n, c in zip(self._seen, counts)]
+
+    def attend(self, queries: torch.Tensor, scale: float | None = None, return_lse: bool = False, out=None):
+        """Attention of one token per sequence, bf16 [batch, query heads, D]; adds to ``mass`` if tracked."""
+        return _A.decode_attention(queries, self.keys, self.values, self.page_table, self.lengths, self.fmt,
+                                   self.key_scales, self.value_scales, scale, self.mass, return_lse, out)
+
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0):
+        """Keep ``budget`` entries per sequence and head (see ``attention.paged_evict``) and take back the
+        pages behind them."""
+        if self.mass is None:
+            raise ValueError("eviction needs a cache built with track=True")
+        _, _, lengths = _A.paged_evict(self.keys, self.values, self.page_table, self.lengths, self.mass, self.positions,
+                                       self.seen, budget, recent, sinks, self.fmt, self.key_scales, self.value_scales)
+        self.lengths.copy_(lengths)
+        keep = -(-int(budget) // self.page_size)
+        changed = []
+        for b in range(self.batch):
+            if self._len[b] > budget:
+                self._len[b] = int(budget)
+                self._free += reversed(self._pages[b][keep:])
+                if len(self._pages[b]) > keep:
+                    self._pages[b] = self._pages[b][:keep]
+                    changed.append(b)
+        self._write_table(changed)
