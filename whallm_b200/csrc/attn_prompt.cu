@@ -1,70 +1,728 @@
 // Attention of packed prompts: grouped heads, causal (aligned at the end, so new
-// tokens may continue a longer history) or full.
+// tokens may continue a longer history) or full, on the 5th-generation tensor
+// cores.
 //
 //   row i of a sequence with nq rows and nk keys sees the keys j <= i + nk - nq
 //   (causal) or all nk;  s_j = scale q.k_j,  lse = log sum_j exp(s_j),
 //   out = sum_j exp(s_j - lse) v_j;  a row that sees no key: out 0, lse -inf.
 //
-// One warp per (row, head) on CUDA cores, one pass with a running maximum.
+// Rows.  The query heads of one key-value head are packed with the tokens: packed
+// row R is token R / G, head R % G of the group.  A work item is kRows packed
+// rows of one (sequence, key-value head): with G = 8 a block of 256 rows is 32
+// tokens, so short prompts fill whole tiles, K and V are read once for all query
+// heads, and the two tiles of a block end at (almost) the same key.
+//
+// One pass over the keys with a running maximum and sum per row (32 bits).  Step
+// s of an item is: S = Q K^T (tcgen05, both operands from shared memory) into one
+// of two TMEM buffers; a softmax warpgroup, one thread per row, reads its row,
+// writes P = exp2(S scale log2e - m) as bf16 over S; O += P V with P from TMEM.
+// Up to D = 128 the block has two tiles of 128 rows and step s works on tile
+// s & 1 (two softmax warpgroups in turn, each with its own O); at D = 256 TMEM
+// holds one O of 256 columns, the block has one tile, step s takes the s-th
+// 64-key tile and the two warpgroups hand the running maximum to each other.
+// The MMA warp issues PV(s), S(s + 2), PV(s + 1), ...: instructions of one thread
+// execute in order, so S(s + 2) may overwrite the buffer that PV(s) read.
+//
+// The reference point m of a row moves only when its maximum grows by more than
+// 2^8 (P then stays below 2^8, harmless in bf16 and in 32-bit sums): O is rescaled
+// in TMEM a few times per item instead of once per step, by the softmax threads
+// themselves.  P is rounded to bf16 once, the type of V; the sum adds the
+// unrounded values.
+//
+// Keys and values come by TMA in the 128-byte swizzle, K with D along the rows
+// (K-major), V with the keys along the rows (its MN-major operand form, no
+// transpose anywhere).  Tiles with keys that some row of the block does not see
+// are special in V only: a hidden key has P = 0, but 0 times a value that is not
+// finite is NaN.  Two helper warps therefore clear, in those tiles, the rows
+// behind the sequence's end (another sequence's values) and every value that is
+// not finite; such values (there are none in a healthy model) are added to the
+// rows that do see them at the end.  The check hides under the step's softmax.
 #include <algorithm>
 
-#include "wm_common.cuh"
+#include "wm_tc.cuh"
 
 namespace {
 
+using wm_tc::elect_one;
+using wm_tc::mbar_arrive;
+using wm_tc::mbar_expect_tx;
+using wm_tc::mbar_init;
+using wm_tc::smem_u32;
+using wm_tc::tc_commit;
+using wm_tc::tc_fence_after;
+using wm_tc::tc_fence_before;
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kSlack = 8.0f;          // growth of a row's maximum (log2) before it is rescaled
+constexpr int kThreads = 384;           // two softmax warpgroups, one warpgroup of TMA, MMA and two helper warps
+constexpr int kHelpers = 64;
 
 struct PromptArgs {
-  const wm_bf16 *q, *k, *v;
-  int64_t q_stride, k_stride, v_stride;
+  const wm_bf16 *q, *v;
+  int64_t q_stride, v_stride;
   const int32_t *cu_q, *cu_k;
-  int B, Tq, Tk, Hq, Hkv, causal;
+  int B, Tq, Tk, Hq, Hkv, G, causal;
   float scale2;
   wm_bf16 *out;
   float *lse;
 };
 
 template <int D>
-__global__ void __launch_bounds__(256) k_attn_prompt_rows(PromptArgs a) {
-  constexpr int V = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t n = static_cast<int64_t>(a.Tq) * a.Hq;
-  for (int64_t x = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; x < n; x += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-    const int t = static_cast<int>(x / a.Hq), h = static_cast<int>(x - static_cast<int64_t>(t) * a.Hq), hk = h / (a.Hq / a.Hkv);
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_q[mid] <= t) lo = mid; else hi = mid;
-    }
-    const int q0 = a.cu_q[lo], q1 = a.cu_q[lo + 1];
-    if (t < q0 || t >= q1) continue;
-    const int k0 = max(a.cu_k[lo], 0), k1 = min(a.cu_k[lo + 1], a.Tk);
-    const int last = a.causal ? min(k1, k0 + (t - q0) + (k1 - k0) - (q1 - q0) + 1) : k1;
-    float q[V], o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      q[i] = wm_bf16_to_f32(a.q[t * a.q_stride + h * D + i * 32 + lane]) * a.scale2;
-      o[i] = 0.0f;
-    }
-    float m = -__builtin_huge_valf(), l = 0.0f;
-    for (int64_t j = k0; j < last; ++j) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) s = fmaf(q[i], wm_bf16_to_f32(a.k[j * a.k_stride + hk * D + i * 32 + lane]), s);
-#pragma unroll
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      const float top = fmaxf(m, s), f = m == top ? 1.0f : exp2f(m - top), p = exp2f(s - top);
-      m = top;
-      l = l * f + p;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], f, p * wm_bf16_to_f32(a.v[j * a.v_stride + hk * D + i * 32 + lane]));
-    }
-    const float inv = last > k0 ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) a.out[(static_cast<int64_t>(t) * a.Hq + h) * D + i * 32 + lane] = wm_f32_to_bf16(o[i] * inv);
-    if (a.lse && lane == 0) a.lse[x] = last > k0 ? (m + log2f(l)) * kLn2 : -__builtin_huge_valf();
+struct Cfg {
+  static constexpr bool kChain = D == 256;            // one tile, the warpgroups share its rows
+  static constexpr int kTiles = kChain ? 1 : 2;       // 128-row tiles of a block
+  static constexpr int kRows = 128 * kTiles;
+  static constexpr int kN = kChain ? 64 : 128;        // keys of a tile
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kSlot = kN * D * 2;            // one K or V tile
+  static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kOCol = 2 * kN;                // TMEM: two S / P buffers, then O
+  static constexpr int kPanel = kN * 128;             // 64 dimensions of a K or V tile
+};
+
+// One block of packed rows of one (sequence, key-value head).
+struct Item {
+  int valid;                // 0: no more work
+  int q0, k0;               // first row and key of the sequence
+  int nq, nk;
+  int h, blk;
+  int tiles, first;         // key tiles; the first of them that holds a key some row does not see
+  uint32_t odd[16];         // keys of tiles first .. first + 3 with values that are not finite (128 bits each)
+};
+
+struct Bars {
+  uint64_t item_full[2], item_empty[2], odd_ready[2];
+  uint64_t q_full, q_empty;
+  // an edge tile (values that some row does not see) lands on v_edge, not kv_full: the helpers wait for it, and the
+  // MMA warp for v_fixed.  Both advance only with edge tiles, so a phase cannot pass unseen
+  uint64_t kv_full[8], kv_empty[8], v_edge[8], v_fixed[8];
+  uint64_t s_full[2], p_ready[2], o_done[2], m_ready[2], o_free, both;
+};
+
+struct Shared {
+  Bars bar;
+  Item item[2];
+  uint32_t tmem;
+  int abort;
+  float m[128], l[2][128];  // D = 256: shared reference points, and each warpgroup's sums at the end
+};
+
+// The tiles start at a multiple of 1024 bytes.
+template <int D>
+constexpr int smem_bytes() { return Cfg<D>::kQBytes + Cfg<D>::kSlots * Cfg<D>::kSlot + static_cast<int>(sizeof(Shared)) + 896; }
+static_assert(smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "shared memory of a CTA");
+
+// Bounded wait of a whole warp: all its lanes return the same answer.  A wait
+// that runs out makes every other wait of the CTA end, too.
+__device__ __forceinline__ bool wait(Shared *sh, uint64_t *bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, wm_tc::mbar_try(bar, parity))) return true;
+  const unsigned long long t0 = wm_tc::gtimer();
+  while (true) {
+    for (int i = 0; i < 8; ++i)
+      if (__all_sync(0xffffffffu, wm_tc::mbar_try(bar, parity))) return true;
+    const bool late = wm_tc::gtimer() - t0 > wm_tc::kWaitNs;
+    if (late) *reinterpret_cast<volatile int *>(&sh->abort) = 1;
+    if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int *>(&sh->abort) != 0)) return false;
   }
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// MN-major operand in the 128-byte swizzle: rows of 64 MN values (128 B), groups
+// of 8 rows along K 1024 B apart, panels of 64 MN values `panel` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t panel) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(panel >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: bf16 x bf16 -> f32, M = 128; B MN-major for PV
+__host__ __device__ constexpr uint32_t idesc_bf16(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+#define WM_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define WM_U8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : WM_R8(r, 0), WM_R8(r, 8), WM_R8(r, 16), WM_R8(r, 24)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      WM_U8(r, 0), WM_U8(r, 8), WM_U8(r, 16), WM_U8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Keys that packed row R of a block sees (0 for rows behind the sequence).
+__device__ __forceinline__ int visible(const PromptArgs &a, int nq, int nk, int R) {
+  const int i = R / a.G;
+  if (!a.causal) return nk;
+  const int n = i + 1 + nk - nq;
+  return n < 0 ? 0 : (n < nk ? n : nk);
+}
+
+__device__ __forceinline__ void seq_bounds(const PromptArgs &a, int b, int &q0, int &nq, int &k0, int &nk) {
+  q0 = min(max(a.cu_q[b], 0), a.Tq);
+  nq = max(min(a.cu_q[b + 1], a.Tq) - q0, 0);
+  k0 = min(max(a.cu_k[b], 0), a.Tk);
+  nk = max(min(a.cu_k[b + 1], a.Tk) - k0, 0);
+}
+
+// Load positions of key tile j and value tile j within an item of n tiles: the
+// order in which the MMA warp needs them.
+template <int D>
+__device__ __forceinline__ int pos_k(int j) { return Cfg<D>::kChain ? (j == 0 ? 0 : 2 * j - 1) : 2 * j; }
+template <int D>
+__device__ __forceinline__ int pos_v(int j, int n) { return Cfg<D>::kChain ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; }
+
+// Work item number x by one warp: blocks of all sequences from the last block of
+// the last sequence backwards (within a causal sequence the longest first), heads
+// innermost.
+template <int D>
+__device__ __forceinline__ void find_item(const PromptArgs &a, int64_t x, Item *out) {
+  using C = Cfg<D>;
+  const int lane = threadIdx.x & 31;
+  int64_t blk = x / a.Hkv;
+  const int h = static_cast<int>(x - blk * a.Hkv);
+  for (int hi = a.B; hi > 0; hi -= 32) {              // lane l: sequence hi - 1 - l
+    const int b = hi - 1 - lane;
+    int q0 = 0, nq = 0, k0 = 0, nk = 0;
+    if (b >= 0) seq_bounds(a, b, q0, nq, k0, nk);
+    const int64_t mine = (static_cast<int64_t>(nq) * a.G + C::kRows - 1) / C::kRows;
+    int64_t s = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, s > blk);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        const int k = static_cast<int>(s - 1 - blk);  // block within the sequence, last first
+        const int R0 = k * C::kRows;
+        const int R1 = static_cast<int>(min(static_cast<int64_t>(R0) + C::kRows, static_cast<int64_t>(nq) * a.G)) - 1;
+        const int n0 = visible(a, nq, nk, R0), n1 = visible(a, nq, nk, R1);
+        out->valid = 1;
+        out->q0 = q0;
+        out->k0 = k0;
+        out->nq = nq;
+        out->nk = nk;
+        out->h = h;
+        out->blk = k;
+        out->tiles = (n1 + C::kN - 1) / C::kN;
+        out->first = n0 / C::kN;
+      }
+      if (lane < 16) out->odd[lane] = 0u;
+      return;
+    }
+    blk -= __shfl_sync(0xffffffffu, s, 31);
+  }
+  if (lane == 0) out->valid = 0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn_prompt(PromptArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using C = Cfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Shared &sh = *reinterpret_cast<Shared *>(smem + C::kQBytes + C::kSlots * C::kSlot);
+  const uint32_t q_s = smem_u32(smem), kv_s = q_s + C::kQBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    Bars &b = sh.bar;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&b.item_full[i], 1);
+      mbar_init(&b.item_empty[i], 8 + 1 + 2);         // softmax, MMA and helper warps
+      mbar_init(&b.odd_ready[i], kHelpers);
+      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_ready[i], 128);
+      mbar_init(&b.o_done[i], 1);
+      mbar_init(&b.m_ready[i], 128);
+    }
+    mbar_init(&b.q_full, kHelpers);
+    mbar_init(&b.q_empty, 1);
+    mbar_init(&b.o_free, 256);
+    mbar_init(&b.both, 256);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&b.kv_full[i], 1);
+      mbar_init(&b.kv_empty[i], 1);
+      mbar_init(&b.v_edge[i], 1);
+      mbar_init(&b.v_fixed[i], kHelpers);
+    }
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  Bars &bar = sh.bar;
+
+  if (warp >= 8) {
+    // 384 threads at 168 registers are launched: 256 x 208 + 128 x 88 is the same sum
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // ------------------------------------------------- items and TMA loads
+      int64_t g = 0;                                  // loads so far
+      uint32_t edge_ph = 0u, edge_last = 0u;          // per slot: phase of v_edge, and whether the last load was an edge tile
+      int it = 0;
+      for (int64_t x = blockIdx.x;; x += gridDim.x, ++it) {
+        const int sl = it & 1;
+        if (!wait(&sh, &bar.item_empty[sl], ((it >> 1) & 1) ^ 1)) break;
+        Item *item = &sh.item[sl];
+        find_item<D>(a, x, item);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.item_full[sl]);
+        if (!item->valid) break;
+        const int n = item->tiles, first = item->first;
+        bool ok = true;
+        for (int p = 0; ok && p < 2 * n; ++p, ++g) {
+          bool is_v;
+          int j;
+          if constexpr (C::kChain) {
+            is_v = p == 2 * n - 1 || (p >= 2 && (p & 1) == 0);
+            j = p == 0 ? 0 : (p == 2 * n - 1 ? n - 1 : ((p & 1) ? (p + 1) / 2 : (p - 2) / 2));
+          } else {
+            is_v = p & 1;
+            j = p >> 1;
+          }
+          const int slot = static_cast<int>(g % C::kSlots);
+          ok = wait(&sh, &bar.kv_empty[slot], static_cast<uint32_t>((g / C::kSlots) & 1) ^ 1);
+          const bool edge = is_v && j >= first;
+          if (ok && elect_one()) {
+            uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
+            mbar_expect_tx(full, C::kSlot);
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_3d(kv_s + slot * C::kSlot + d * C::kPanel, is_v ? &map_v : &map_k, d * 64, item->h, item->k0 + j * C::kN, full);
+            if (edge) mbar_arrive(&bar.kv_full[slot]);
+          }
+          if (ok) {
+            edge_ph ^= edge ? 1u << slot : 0u;
+            edge_last = edge ? edge_last | (1u << slot) : edge_last & ~(1u << slot);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+      // loads in flight when the others gave up must land before the CTA leaves
+      if (*reinterpret_cast<volatile int *>(&sh.abort))
+        for (int64_t i = g > C::kSlots ? g - C::kSlots : 0; i < g; ++i) {
+          const int slot = static_cast<int>(i % C::kSlots);
+          const bool edge = (edge_last >> slot) & 1u;
+          uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
+          const uint32_t ph = edge ? ((edge_ph >> slot) & 1u) ^ 1u : static_cast<uint32_t>((i / C::kSlots) & 1);
+          for (int tries = 0; tries < 1000 && !wm_tc::mbar_try(full, ph); ++tries) {}
+        }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------- MMAs
+      constexpr uint32_t id_s = idesc_bf16(C::kN, false), id_o = idesc_bf16(D, true);
+      int64_t g0 = 0;                                 // loads before this item
+      uint32_t fixed = 0u, pph = 0u;                  // phase bits: v_fixed per slot, p_ready per buffer
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int sl = it & 1;
+        ok = wait(&sh, &bar.item_full[sl], (it >> 1) & 1);
+        if (!ok) break;
+        const Item *item = &sh.item[sl];
+        const int n = item->tiles, first = item->first, valid = item->valid;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
+        if (!valid) break;
+        const int steps = n * C::kTiles;
+        ok = wait(&sh, &bar.q_full, it & 1);
+        if (!ok) break;
+        auto slot_of = [&](int64_t gg) { return static_cast<int>(gg % C::kSlots); };
+        auto phase_of = [&](int64_t gg) { return static_cast<uint32_t>((gg / C::kSlots) & 1); };
+        auto issue_s = [&](int s) {
+          const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1;
+          const int64_t gg = g0 + pos_k<D>(j);
+          if (!wait(&sh, &bar.kv_full[slot_of(gg)], phase_of(gg))) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t qa = q_s + w * (128 * D * 2), kb = kv_s + slot_of(gg) * C::kSlot;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(tmem + (s & 1) * C::kN, wm_tc::bdesc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32),
+                     wm_tc::bdesc_sw128(kb + (kk >> 2) * C::kPanel + (kk & 3) * 32), id_s, kk != 0);
+            tc_commit(&bar.s_full[s & 1]);
+            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[slot_of(gg)]);
+            if (s == steps - 1) tc_commit(&bar.q_empty);
+          }
+          __syncwarp();
+          return true;
+        };
+        if (steps == 0 && lane == 0) mbar_arrive(&bar.q_empty);       // nothing to read Q for
+        for (int s = 0; ok && s < 2 && s < steps; ++s) ok = issue_s(s);
+        if (ok && it > 0) ok = wait(&sh, &bar.o_free, (it - 1) & 1);  // the last item's O has been read
+        for (int s = 0; ok && s < steps; ++s) {
+          const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1, buf = s & 1;
+          const int64_t gg = g0 + pos_v<D>(j, n);
+          const int slot = slot_of(gg);
+          ok = wait(&sh, &bar.kv_full[slot], phase_of(gg));
+          if (ok && j >= first && w == 0) {
+            ok = wait(&sh, &bar.v_fixed[slot], (fixed >> slot) & 1u);
+            fixed ^= 1u << slot;
+          }
+          ok = ok && wait(&sh, &bar.p_ready[buf], (pph >> buf) & 1u);
+          pph ^= 1u << buf;
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t vb = kv_s + slot * C::kSlot, o = tmem + C::kOCol + w * D, p = tmem + buf * C::kN;
+#pragma unroll
+            for (int kk = 0; kk < C::kN / 16; ++kk)
+              wm_tc::tc_mma_ts(o, p + kk * 8, desc_mn(vb + kk * 2048, C::kPanel), id_o, (j | kk) != 0);
+            if (C::kChain || s >= steps - 2) tc_commit(&bar.o_done[buf]);
+            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[slot]);
+          }
+          __syncwarp();
+          if (s + 2 < steps) ok = issue_s(s + 2);
+        }
+        g0 += 2 * n;
+      }
+    } else {
+      // --------------------------------- query rows, and values of edge tiles
+      const int ht = tid - 320;
+      int64_t g0 = 0;
+      uint32_t edge_ph = 0u;
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int sl = it & 1;
+        ok = wait(&sh, &bar.item_full[sl], (it >> 1) & 1);
+        if (!ok) break;
+        Item *item = &sh.item[sl];
+        if (!item->valid) break;
+        const int n = item->tiles, first = item->first, nk = item->nk;
+        const int64_t rows = static_cast<int64_t>(item->nq) * a.G;
+        ok = wait(&sh, &bar.q_empty, (it & 1) ^ 1);
+        if (!ok) break;
+        const int R0 = item->blk * C::kRows;
+        constexpr int per = D / 8;                    // 16-byte pieces of a row
+        for (int x = ht; x < C::kRows * per; x += kHelpers) {
+          const int r = x / per, c = x % per;
+          const bool in = R0 + r < rows;
+          const int i = in ? (R0 + r) / a.G : 0, hg = in ? (R0 + r) - i * a.G : 0;
+          const wm_bf16 *src = a.q + (static_cast<int64_t>(item->q0) + i) * a.q_stride + static_cast<int64_t>(item->h * a.G + hg) * D + c * 8;
+          const uint32_t dst = q_s + (r >> 7) * (128 * D * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&bar.q_full);
+        for (int j = first; ok && j < n; ++j) {
+          const int64_t gg = g0 + pos_v<D>(j, n);
+          const int slot = static_cast<int>(gg % C::kSlots);
+          ok = wait(&sh, &bar.v_edge[slot], (edge_ph >> slot) & 1u);
+          if (!ok) break;
+          edge_ph ^= 1u << slot;
+          uint8_t *vt = smem + C::kQBytes + slot * C::kSlot;
+          const int live = nk - j * C::kN;
+          for (int x = ht; x < C::kSlot / 16; x += kHelpers) {
+            const int r = (x >> 3) % C::kN;           // key of this 16-byte piece
+            uint4 *p = reinterpret_cast<uint4 *>(vt) + x;
+            if (r >= live) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            const uint4 v = *p;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {             // exponent bits all ones
+              const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
+              odd |= lo | hi;
+              w[e] = (lo ? 0u : w[e] & 0xffffu) | (hi ? 0u : w[e] & 0xffff0000u);
+            }
+            if (odd) {
+              *p = make_uint4(w[0], w[1], w[2], w[3]);
+              if (j - first < 4) atomicOr(&item->odd[(j - first) * 4 + (r >> 5)], 1u << (r & 31));
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&bar.v_fixed[slot]);
+        }
+        mbar_arrive(&bar.odd_ready[sl]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
+        g0 += 2 * n;
+      }
+    }
+  } else {
+    // ------------------------------------------------- softmax, one row each
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int w = warp >> 2, r = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + lanes + w * C::kN;
+    const uint32_t o_t = tmem + lanes + C::kOCol + (C::kChain ? 0 : w * D);
+    uint32_t sph = 0u;                                // phase of this warpgroup's S
+    // D = 256: steps of the items before on each buffer, the phases of o_done and m_ready; else the
+    // items before that had keys, the phase of o_done
+    uint32_t done[2] = {0u, 0u};
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int sl = it & 1;
+      ok = wait(&sh, &bar.item_full[sl], (it >> 1) & 1);
+      if (!ok) break;
+      const Item *item = &sh.item[sl];
+      if (!item->valid) break;
+      const int n = item->tiles, first = item->first, nq = item->nq, nk = item->nk;
+      const int steps = n * C::kTiles;
+      const int R = item->blk * C::kRows + (C::kChain ? 0 : w * 128) + r;
+      const bool live = R < static_cast<int64_t>(nq) * a.G;
+      const int see = live ? visible(a, nq, nk, R) : 0;
+      float m = kNegInf, l = 0.0f;
+
+      for (int s = w; ok && s < steps; s += 2) {
+        const int j = C::kChain ? s : s >> 1;
+        ok = wait(&sh, &bar.s_full[w], sph);
+        if (!ok) break;
+        sph ^= 1u;
+        tc_fence_after();
+        uint32_t x[C::kN / 32][32];
+#pragma unroll
+        for (int c = 0; c < C::kN / 32; ++c) tmem_ld32(x[c], s_t + c * 32);
+        tmem_wait_ld();
+        if (j >= first) {
+          const int room = see - j * C::kN;
+#pragma unroll
+          for (int c = 0; c < C::kN; ++c)
+            if (c >= room) x[c >> 5][c & 31] = __float_as_uint(kNegInf);
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[0][c]);
+#pragma unroll
+        for (int c = 4; c < C::kN; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c >> 5][c & 31]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+        if constexpr (C::kChain) {
+          if (s > 0) {                                // the reference point as the other warpgroup left it
+            ok = wait(&sh, &bar.m_ready[w ^ 1], (done[w ^ 1] + ((s - 1) >> 1)) & 1u);
+            if (!ok) break;
+            const float mo = *reinterpret_cast<volatile float *>(&sh.m[r]);
+            if (mo != m) {
+              l *= m == kNegInf ? 0.0f : ex2(m - mo);
+              m = mo;
+            }
+          }
+        }
+        const bool grow = top > m + kSlack || (m == kNegInf && top > m);
+        const float f = grow ? (m == kNegInf ? 0.0f : ex2(m - top)) : 1.0f;
+        if (grow) {
+          m = top;
+          l *= f;
+        }
+        if constexpr (C::kChain) {
+          *reinterpret_cast<volatile float *>(&sh.m[r]) = m;
+          mbar_arrive(&bar.m_ready[w]);
+        }
+        // O holds PV of the steps before.  With two tiles S(s) followed PV(s - 2), the last one on this O, in
+        // the MMA warp's order, so it is complete; at D = 256 the last one is PV(s - 1)
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+          if constexpr (C::kChain) {
+            ok = wait(&sh, &bar.o_done[w ^ 1], (done[w ^ 1] + ((s - 1) >> 1)) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o, o_t + c);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(o_t + c, o);
+          }
+        }
+        const float base = m == kNegInf ? 0.0f : m;
+        const float2 sc = make_float2(a.scale2, a.scale2), nb = make_float2(-base, -base);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int h = 0; h < C::kN / 64; ++h) {        // 64 keys: 32 registers of P
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int c = h * 64 + 2 * i;
+            float2 e = wm_fma2(make_float2(__uint_as_float(x[c >> 5][c & 31]), __uint_as_float(x[(c + 1) >> 5][(c + 1) & 31])), sc, nb);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[i & 1] = wm_add2(sum[i & 1], e);
+            p[i] = bf16x2(e.x, e.y);
+          }
+          tmem_st32(s_t + h * 32, p);
+        }
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar.p_ready[w]);
+      }
+      if (!ok) break;
+
+      // --------------------------------------------------------- epilogue
+      if (steps > 0) {
+        const int last = C::kChain ? (steps - 1) & 1 : w;
+        ok = wait(&sh, &bar.o_done[last], (done[last] + (C::kChain ? (steps - 1) >> 1 : 0)) & 1u);
+        if (!ok) break;
+        done[0] += C::kChain ? (steps + 1) >> 1 : 1;
+        done[1] += C::kChain ? steps >> 1 : 1;
+      }
+      ok = wait(&sh, &bar.odd_ready[sl], (it >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if constexpr (C::kChain) {
+        // both warpgroups' sums at the last reference point; two phases of `both` per item
+        mbar_arrive(&bar.both);
+        ok = wait(&sh, &bar.both, 0);
+        if (!ok) break;
+        if (steps > 0) {
+          const float ml = *reinterpret_cast<volatile float *>(&sh.m[r]);
+          if (m != ml) l = m == kNegInf ? 0.0f : l * ex2(m - ml);
+          m = ml;
+        }
+        sh.l[w][r] = l;
+        mbar_arrive(&bar.both);
+        ok = wait(&sh, &bar.both, 1);
+        if (!ok) break;
+        l = sh.l[0][r] + sh.l[1][r];
+      }
+      uint32_t any = 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) any |= item->odd[i];
+      const float inv = see > 0 ? 1.0f / l : 0.0f;
+      const int i = R / a.G, hg = R - i * a.G;
+      const int64_t head = (static_cast<int64_t>(item->q0) + i) * a.Hq + item->h * a.G + hg;
+      constexpr int kCols = C::kChain ? D / 2 : D;    // at D = 256 each warpgroup writes half of every row
+      const int col0 = C::kChain ? w * kCols : 0;
+      for (int c = col0; c < col0 + kCols; c += 32) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(o, o_t + c);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (live && any) {                            // values that are not finite, for the rows that see them
+          for (int t = 0; t < 16; ++t)
+            for (uint32_t bits = item->odd[t]; bits; bits &= bits - 1) {
+              const int key = (first + (t >> 2)) * C::kN + (t & 3) * 32 + __ffs(bits) - 1;
+              if (key >= see) continue;
+              const wm_bf16 *vp = a.v + (static_cast<int64_t>(item->k0) + key) * a.v_stride + static_cast<int64_t>(item->h) * D + c;
+              for (int e = 0; e < 32; ++e) {
+                const float x = wm_bf16_to_f32(vp[e]);
+                if (!(fabsf(x) <= 3.4028234663852886e38f)) {
+#pragma unroll
+                  for (int y = 0; y < 32; ++y)
+                    if (y == e) o[y] = __float_as_uint(__uint_as_float(o[y]) + x);
+                }
+              }
+            }
+        }
+        uint4 *dst = reinterpret_cast<uint4 *>(a.out + head * D + c);
+#pragma unroll
+        for (int e = 0; live && e < 4; ++e) {
+          uint32_t y[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const float lo = __uint_as_float(o[8 * e + 2 * z]), hi = __uint_as_float(o[8 * e + 2 * z + 1]);
+            y[z] = see > 0 ? bf16x2(lo * inv, hi * inv) : 0u;
+          }
+          dst[e] = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+        __syncwarp();                                 // the TMEM loads are whole-warp instructions
+      }
+      if (live && a.lse && (!C::kChain || w == 0)) a.lse[head] = see > 0 ? (m + log2f(l)) * kLn2 : kNegInf;
+      tc_fence_before();
+      mbar_arrive(&bar.o_free);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
+    }
+  }
+  __syncthreads();
+  if (*reinterpret_cast<volatile int *>(&sh.abort)) { // a wait ran out: no result passes for one
+    const int64_t n = static_cast<int64_t>(a.Tq) * a.Hq * D;
+    for (int64_t i = tid; i < n; i += kThreads) a.out[i] = 0x7FC0;
+  }
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// [tokens, heads, D] bf16 with `stride` values between tokens, boxes of 64
+// dimensions x 1 head x `rows` tokens; tokens behind the last read as zeros.
+int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t tokens, int64_t stride, int rows) {
+  auto fn = wm_tc::encode_fn();
+  if (!fn) return wm::fail(WM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return wm::fail(WM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+  return WM_OK;
+}
+
+template <int D>
+int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t stream) {
+  using C = Cfg<D>;
+  CUtensorMap mk, mv;
+  // without keys no tile is loaded; the maps then describe one row of q
+  const bool any = a.Tk > 0;
+  if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, C::kN)) return rc;
+  if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, C::kN)) return rc;
+  // at most one partial block per sequence beyond the rows' own blocks
+  const int64_t most = (static_cast<int64_t>(a.Tq) * a.G / C::kRows + a.B) * a.Hkv;
+  const int grid = static_cast<int>(std::min<int64_t>(most, wm::sm_count()));
+  auto kern = k_attn_prompt<D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
+  kern<<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mk, mv);
+  return wm::check_launch("wattn_prompt");
 }
 
 }  // namespace
@@ -85,14 +743,12 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
                  v_stride >= static_cast<int64_t>(Hkv) * D && q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 &&
                  wm::aligned(q, 16) && wm::aligned(k, 16) && wm::aligned(v, 16) && wm::aligned(out, 16),
              "prompt attention: token rows must be 16-byte aligned and hold their heads");
-  const PromptArgs a{q, k, v, q_stride, k_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, causal,
+  WM_REQUIRE(static_cast<int64_t>(Tq) * (Hq / Hkv) <= INT32_MAX - 256, "prompt attention: too many rows per key-value head");
+  const PromptArgs a{q, v, q_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, Hq / Hkv, causal,
                      scale * kLog2e, out, lse};
-  const int64_t want = (static_cast<int64_t>(Tq) * Hq + 7) / 8;
-  const int grid = static_cast<int>(std::min<int64_t>(want, static_cast<int64_t>(wm::sm_count()) * 64));
-  if (D == 64) k_attn_prompt_rows<64><<<grid, 256, 0, stream>>>(a);
-  else if (D == 128) k_attn_prompt_rows<128><<<grid, 256, 0, stream>>>(a);
-  else k_attn_prompt_rows<256><<<grid, 256, 0, stream>>>(a);
-  return wm::check_launch("wattn_prompt");
+  if (D == 64) return launch<64>(a, k, k_stride, stream);
+  if (D == 128) return launch<128>(a, k, k_stride, stream);
+  return launch<256>(a, k, k_stride, stream);
 }
 
 }  // extern "C"
