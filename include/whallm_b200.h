@@ -294,8 +294,9 @@ WM_API int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, 
  * sequence of length 0 gets zeros and lse -inf; one whose length is outside
  * [0, capacity] or that reaches a page id outside [0, n_pages) gets NaN.
  * Workspace: wattn_decode_workspace_size (with a mass array it also holds the
- * scores, 4 bytes per entry of the capacity and query head, heads rounded up to
- * 8 or a multiple of 16 per kv head); calls that share one must not overlap. */
+ * scores, 4 bytes per entry of the capacity and query head, the heads of a kv
+ * head rounded up to 2, above 16 to a multiple of 16); calls that share one must
+ * not overlap. */
 WM_API size_t wattn_decode_workspace_size(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages,
                                           int with_mass);
 WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int D, const void *k_cache,

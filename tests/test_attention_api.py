@@ -99,7 +99,7 @@ def test_decode_refusals():
     expect(f, decode_args(B=0), None, L.WM_OK)
     size = L.lib().wattn_decode_workspace_size
     assert size(2, 6, 4, 128, L.WKV_BF16, 16, 4, 0) == 0 and size(2, 8, 4, 100, L.WKV_BF16, 16, 4, 0) == 0
-    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 1) - size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 0) == 2 * 4 * 64 * 8 * 4
+    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 1) - size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 0) == 2 * 4 * 64 * 2 * 4
 
 
 def test_prompt_refusals():

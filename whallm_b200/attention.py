@@ -25,70 +25,89 @@ import torch
 from . import _lib as L
 
 PAGED_FORMATS = {"bf16": L.WKV_BF16, "fp8_f32_b64": L.WKV_FP8_F32_B64, "mxfp8": L.WKV_MXFP8_B32}
-_INT = torch.int32
+_BF16, _F32, _INT, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+_NO_CPU = "whallm_b200 ops take CUDA tensors (no CPU fallback)"
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+# The checks below run on every call of a decode step, where the host's time is what counts for small
+# batches: they read each tensor attribute once, and addresses go to the library as plain integers.
 
 
-def _call(name, t, *args):
-    """Call an entry point on t's device and its current stream."""
-    if t.device.index == torch.cuda.current_device():
-        L.call(name, *args, L.stream_of(t))
+def _call(name, dev, *args):
+    """Call an entry point on device number ``dev`` and its current stream."""
+    if dev == torch.cuda.current_device():
+        L.call(name, *args, _raw_stream(dev))
     else:
-        with torch.cuda.device(t.device):
-            L.call(name, *args, L.stream_of(t))
+        with torch.cuda.device(dev):
+            L.call(name, *args, _raw_stream(dev))
 
 
-def _same_device(first, *tensors):
-    for t in tensors:
-        if t is not None and t.device != first.device:
-            raise ValueError("all tensors of a call must be on one device")
-
-
-def _ints(name, t, shape):
-    if t.dtype != _INT or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be int32 {list(shape)}")
+def _at(name, t, dtype, shape, dev):
+    """Address of a contiguous tensor of a given type, shape and device (None: 0)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {list(shape)}")
+    if t.get_device() != dev or not t.is_contiguous():
+        if not t.is_cuda:
+            raise ValueError(_NO_CPU)
+        if not t.is_contiguous():
+            raise ValueError("whallm_b200 ops take contiguous tensors")
+        raise ValueError("all tensors of a call must be on one device")
+    return t.data_ptr()
 
 
 def _tokens(name, t, heads=None):
     """bf16 [T, heads, D] whose heads are dense -> (T, heads, D, values between tokens)."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3:
+    if t.dtype != _BF16 or t.dim() != 3:
         raise ValueError(f"{name} must be bf16 [tokens, heads, D]")
     n, h, d = t.shape
+    s0, s1, s2 = t.stride()
     if heads is not None and h != heads:
         raise ValueError(f"{name} has {h} heads, expected {heads}")
     if not t.is_cuda:
-        raise ValueError("whallm_b200 ops take CUDA tensors (no CPU fallback)")
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+        raise ValueError(_NO_CPU)
+    if (s2 != 1 and d > 1) or (s1 != d and h > 1):
         raise ValueError(f"the heads of a token of {name} must be contiguous")
-    return n, h, d, (t.stride(0) if n > 1 else h * d)
+    return n, h, d, (s0 if n > 1 else h * d)
 
 
 def _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt):
-    """Check a paged cache's tensors -> (format id, n_pages, Hkv, page_size, D, B, max_pages)."""
-    if fmt not in PAGED_FORMATS:
+    """Check a paged cache's tensors -> (format id, n_pages, Hkv, page_size, D, B, max_pages, device, the
+    addresses of caches, scales and table)."""
+    f = PAGED_FORMATS.get(fmt)
+    if f is None:
         raise ValueError(f"paged cache format must be one of {sorted(PAGED_FORMATS)}, got {fmt!r}")
-    f = PAGED_FORMATS[fmt]
-    dt = torch.bfloat16 if f == L.WKV_BF16 else torch.uint8
-    if k_cache.dim() != 4 or k_cache.dtype != dt or v_cache.dtype != dt or v_cache.shape != k_cache.shape:
+    shape = k_cache.shape
+    dt = _BF16 if f == L.WKV_BF16 else _U8
+    if len(shape) != 4 or k_cache.dtype != dt or v_cache.dtype != dt or v_cache.shape != shape:
         raise ValueError(f"caches must be {dt} [n_pages, heads, page_size, D] of one shape")
-    pages, heads, size, d = k_cache.shape
+    pages, heads, size, d = shape
+    if page_table.dim() != 2 or page_table.dtype != _INT:
+        raise ValueError("page_table must be int32 [sequences, max_pages]")
+    tshape = page_table.shape
+    dev = k_cache.get_device()
     if f == L.WKV_BF16:
         if k_scales is not None or v_scales is not None:
             raise ValueError("bf16 caches take no scales")
+        ks = vs = None
     else:
-        sdt, blk = (torch.float32, 64) if f == L.WKV_FP8_F32_B64 else (torch.uint8, 32)
-        for s in (k_scales, v_scales):
-            if s is None or s.dtype != sdt or tuple(s.shape) != (pages, heads, size, d // blk):
-                raise ValueError(f"{fmt} caches need {sdt} scales [n_pages, heads, page_size, D/{blk}]")
-    if page_table.dim() != 2 or page_table.dtype != _INT:
-        raise ValueError("page_table must be int32 [sequences, max_pages]")
-    L.require_cuda(k_cache, v_cache, k_scales, v_scales, page_table)
-    _same_device(k_cache, v_cache, k_scales, v_scales, page_table)
-    return f, pages, heads, size, d, page_table.shape[0], page_table.shape[1]
+        sdt, blk = (_F32, 64) if f == L.WKV_FP8_F32_B64 else (_U8, 32)
+        sshape = (pages, heads, size, d // blk)
+        if k_scales is None or v_scales is None:
+            raise ValueError(f"{fmt} caches need {sdt} scales [n_pages, heads, page_size, D/{blk}]")
+        ks, vs = _at("k_scales", k_scales, sdt, sshape, dev), _at("v_scales", v_scales, sdt, sshape, dev)
+    at = (_at("k_cache", k_cache, dt, shape, dev), _at("v_cache", v_cache, dt, shape, dev), ks, vs,
+          _at("page_table", page_table, _INT, tshape, dev))
+    if dev < 0:
+        raise ValueError(_NO_CPU)
+    return f, pages, heads, size, d, tshape[0], tshape[1], dev, at
 
 
-def _per_entry(name, t, dtype, shape):
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != shape):
-        raise ValueError(f"{name} must be {dtype} {list(shape)}")
+def _on(dev, *tensors):
+    for t in tensors:
+        if t.get_device() != dev:
+            raise ValueError("all tensors of a call must be on one device")
 
 
 def _scale(scale, d):
@@ -108,25 +127,20 @@ def paged_append(k, v, cu_seqlens, k_cache, v_cache, page_table, lengths, fmt="b
     already.  Their ``mass`` (float32 [B, Hkv, capacity]) becomes 0 and their
     ``positions`` (int32, same shape) the token's position, ``seen`` int32 [B]
     counting every token of the sequence up to and including these."""
-    f, pages, heads, size, d, B, width = _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt)
+    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                               page_table, fmt)
     T, _, dk, ks = _tokens("k", k, heads)
     Tv, _, dv, vs = _tokens("v", v, heads)
     if dk != d or dv != d or Tv != T:
         raise ValueError("k and v must have one shape and the cache's head dimension")
-    _ints("cu_seqlens", cu_seqlens, (B + 1,))
-    _ints("lengths", lengths, (B,))
-    shape = (B, heads, width * size)
-    _per_entry("mass", mass, torch.float32, shape)
-    _per_entry("positions", positions, _INT, shape)
     if positions is not None and seen is None:
         raise ValueError("positions need the sequences' token counts (seen)")
-    if seen is not None:
-        _ints("seen", seen, (B,))
-    L.require_cuda(cu_seqlens, lengths, mass, positions, seen)
-    _same_device(k_cache, k, v, cu_seqlens, lengths, mass, positions, seen)
-    p = L.ptr
-    _call("wkv_paged_append", k, p(k), p(v), ks, vs, p(cu_seqlens), T, B, heads, d, p(k_cache), p(v_cache), p(k_scales),
-          p(v_scales), f, pages, size, p(page_table), width, p(lengths), p(mass), p(positions), p(seen))
+    _on(dev, k, v)
+    shape = (B, heads, width * size)
+    _call("wkv_paged_append", dev, k.data_ptr(), v.data_ptr(), ks, vs, _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev),
+          T, B, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width, _at("lengths", lengths, _INT, (B,), dev),
+          _at("mass", mass, _F32, shape, dev), _at("positions", positions, _INT, shape, dev),
+          _at("seen", seen, _INT, (B,), dev))
 
 
 def paged_evict(k_cache, v_cache, page_table, lengths, mass, positions, seen, budget, recent=0, sinks=0, fmt="bf16",
@@ -139,27 +153,21 @@ def paged_evict(k_cache, v_cache, page_table, lengths, mass, positions, seen, bu
     Without ``out``, mass and positions are updated in place; else ``out`` is
     ``(mass, positions, lengths)`` to write, which may share the input's mass and
     positions but not its lengths.  Returns (mass, positions, lengths)."""
-    f, pages, heads, size, d, B, width = _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt)
-    shape = (B, heads, width * size)
+    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                               page_table, fmt)
+    cap = width * size
+    shape = (B, heads, cap)
     new_mass, new_pos, new_len = out if out is not None else (mass, positions, torch.empty_like(lengths))
-    _ints("lengths", lengths, (B,))
-    _ints("new lengths", new_len, (B,))
-    _ints("seen", seen, (B,))
-    for m, q in ((mass, positions), (new_mass, new_pos)):
-        _per_entry("mass", m, torch.float32, shape)
-        _per_entry("positions", q, _INT, shape)
     budget, recent, sinks = int(budget), int(recent), int(sinks)
     if budget <= 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError("the budget must be positive and hold the recent and the first positions")
-    L.require_cuda(lengths, mass, positions, seen, new_mass, new_pos, new_len)
-    _same_device(k_cache, lengths, mass, positions, seen, new_mass, new_pos, new_len)
     budget = min(budget, 2**31 - 1)
-    nbytes = L.lib().wkv_evict_workspace_size(B, heads, min(budget, max(width * size, 1)))
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=k_cache.device)
-    p = L.ptr
-    _call("wkv_paged_evict", k_cache, B, heads, d, p(k_cache), p(v_cache), p(k_scales), p(v_scales), f, pages, size,
-          p(page_table), width, p(lengths), p(seen), p(mass), p(positions), budget, recent, sinks, p(new_mass), p(new_pos),
-          p(new_len), p(ws), ws.numel())
+    ws = torch.empty((2 * B * heads * max(1, min(budget, cap)),), dtype=_INT, device=k_cache.device)
+    _call("wkv_paged_evict", dev, B, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width,
+          _at("lengths", lengths, _INT, (B,), dev), _at("seen", seen, _INT, (B,), dev), _at("mass", mass, _F32, shape, dev),
+          _at("positions", positions, _INT, shape, dev), budget, recent, sinks, _at("new mass", new_mass, _F32, shape, dev),
+          _at("new positions", new_pos, _INT, shape, dev), _at("new lengths", new_len, _INT, (B,), dev), ws.data_ptr(),
+          4 * ws.numel())
     return new_mass, new_pos, new_len
 
 
@@ -173,25 +181,23 @@ def decode_attention(q, k_cache, v_cache, page_table, lengths, fmt="bf16", k_sca
     over the query heads of its key-value head.  ``scale`` defaults to D^-1/2.  A
     sequence without entries gets zeros (lse -inf); one whose length or pages are
     out of range gets NaN."""
-    f, pages, heads, size, d, B, width = _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt)
+    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                               page_table, fmt)
     Bq, Hq, dq, qs = _tokens("q", q)
     if Bq != B or dq != d or Hq % heads:
         raise ValueError("q must be [sequences, a multiple of the cache's heads, D]")
-    _ints("lengths", lengths, (B,))
-    _per_entry("mass", mass, torch.float32, (B, heads, width * size))
     scale = _scale(scale, d)
+    _on(dev, q)
+    device = q.device
     if out is None:
-        out = torch.empty((B, Hq, d), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (B, Hq, d):
-        raise ValueError("out must be bf16 [sequences, heads, D]")
-    L.require_cuda(lengths, mass, out)
-    _same_device(k_cache, q, lengths, mass, out)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty((B, Hq, d), dtype=_BF16, device=device)
+    lse = torch.empty((B, Hq), dtype=_F32, device=device) if return_lse else None
     nbytes = L.lib().wattn_decode_workspace_size(B, Hq, heads, d, f, size, width, mass is not None)
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
-    p = L.ptr
-    _call("wattn_decode", q, p(q), qs, B, Hq, heads, d, p(k_cache), p(v_cache), p(k_scales), p(v_scales), f, pages, size,
-          p(page_table), width, p(lengths), scale, p(out), p(lse), p(mass), p(ws), ws.numel())
+    ws = torch.empty((max(nbytes, 256),), dtype=_U8, device=device)
+    _call("wattn_decode", dev, q.data_ptr(), qs, B, Hq, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width,
+          _at("lengths", lengths, _INT, (B,), dev), scale, _at("out", out, _BF16, (B, Hq, d), dev),
+          lse.data_ptr() if return_lse else None, _at("mass", mass, _F32, (B, heads, width * size), dev), ws.data_ptr(),
+          nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -213,20 +219,17 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
         if Tk != Tq:
             raise ValueError("keys of another count than the rows need cu_seqlens_k")
         cu_seqlens_k = cu_seqlens
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
-        raise ValueError("cu_seqlens must be int32 [sequences + 1]")
     B = cu_seqlens.numel() - 1
-    _ints("cu_seqlens", cu_seqlens, (B + 1,))
-    _ints("cu_seqlens_k", cu_seqlens_k, (B + 1,))
+    if B < 0:
+        raise ValueError("cu_seqlens must be int32 [sequences + 1]")
     scale = _scale(scale, d)
+    dev, device = q.get_device(), q.device
+    _on(dev, k, v)
     if out is None:
-        out = torch.empty((Tq, Hq, d), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (Tq, Hq, d):
-        raise ValueError("out must be bf16 [tokens, heads, D]")
-    L.require_cuda(cu_seqlens, cu_seqlens_k, out)
-    _same_device(q, k, v, cu_seqlens, cu_seqlens_k, out)
-    lse = torch.empty((Tq, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    p = L.ptr
-    _call("wattn_prompt", q, p(q), p(k), p(v), qs, ks, vs, p(cu_seqlens), p(cu_seqlens_k), B, Tq, Tk, Hq, Hkv, d, scale,
-          int(bool(causal)), p(out), p(lse))
+        out = torch.empty((Tq, Hq, d), dtype=_BF16, device=device)
+    lse = torch.empty((Tq, Hq), dtype=_F32, device=device) if return_lse else None
+    _call("wattn_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
+          _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev), _at("cu_seqlens_k", cu_seqlens_k, _INT, (B + 1,), dev), B, Tq,
+          Tk, Hq, Hkv, d, scale, 1 if causal else 0, _at("out", out, _BF16, (Tq, Hq, d), dev),
+          lse.data_ptr() if return_lse else None)
     return (out, lse) if return_lse else out

@@ -54,7 +54,8 @@ struct DecodeArgs {
   float *lse;                           // [B, Hq] or null
   float *mass;                          // [B, Hkv, capacity] or null
   float *part_o, *part_m, *part_l;      // parts: [slots][heads of a chunk][D] and [slots][heads of a chunk]
-  float *scores;                        // [pairs][capacity][heads of a chunk], with mass only
+  float *scores;                        // [pairs][capacity][score_heads], with mass only
+  int score_heads;                      // a chunk's query heads, rounded up to 2
   int n_cta;                            // CTAs the line is split over
 };
 
@@ -344,11 +345,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
         s[nh][3] = g + 8 < rows ? s[nh][3] * a.scale2 : kNegInf;
       }
       if (a.scores) {
-        float *sp = a.scores + (pair * cap + key) * S::kHeads + i2;
+        const int sh = a.score_heads;
+        float *sp = a.scores + (pair * cap + key) * sh + i2;
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
-          if (g < rows) *reinterpret_cast<float2 *>(sp + g * S::kHeads + nh * 8) = make_float2(s[nh][0], s[nh][1]);
-          if (g + 8 < rows) *reinterpret_cast<float2 *>(sp + (g + 8) * S::kHeads + nh * 8) = make_float2(s[nh][2], s[nh][3]);
+          if (nh * 8 + i2 >= sh) continue;
+          if (g < rows) *reinterpret_cast<float2 *>(sp + g * sh + nh * 8) = make_float2(s[nh][0], s[nh][1]);
+          if (g + 8 < rows) *reinterpret_cast<float2 *>(sp + (g + 8) * sh + nh * 8) = make_float2(s[nh][2], s[nh][3]);
         }
       }
 
@@ -504,108 +507,170 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   }
 }
 
-// Joins the parts of a pair: block (pair, head) for the output, and with a mass
-// array blocks (pair, kHeads + x) that add the weights of a run of keys.
+// Joins the parts of a pair.  Blocks (pair, head) give the output; with a mass
+// array blocks (pair, heads + x) add the weights of a run of keys.  A pair has up
+// to one part per CTA: their factors go to shared memory first, so that the loads
+// of the parts' outputs are independent of one another (a first form that walked
+// the parts one by one took 9.8 us for 37 parts of 128 values).
 constexpr int kJoin = 128;             // threads
-constexpr int kRun = 2048;             // keys of a mass block
+constexpr int kRun = 512;              // keys of a mass block
 
-template <int NH>
-__global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int D) {
+// Factor of a part with maximum m under the pair's maximum: a part without a
+// finite score keeps its sum (zero, or NaN).
+__device__ __forceinline__ float part_factor(float m, float top) { return m == kNegInf ? 1.0f : ex2(m - top); }
+
+template <int D, int NH>
+__global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
   constexpr int kHeads = 8 * NH;
+  constexpr int kCols = D / 4, kGroups = kJoin / kCols;        // a thread sums 4 values over every kGroups-th part
+  __shared__ float s_f[kJoin], s_red[2][kJoin / 32];
+  __shared__ float4 s_o[kJoin];
+  __shared__ float2 s_st[kJoin];
   __shared__ float s_lse2[kHeads];
   const int PH = a.pool.Hkv * a.NC;
   const int64_t pair = blockIdx.x;
   const int b = static_cast<int>(pair / PH), hc = static_cast<int>(pair - static_cast<int64_t>(b) * PH);
   const int h = hc / a.NC, c = hc - h * a.NC;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (static_cast<int>(blockIdx.y) < heads ? c * kHeads + static_cast<int>(blockIdx.y) >= a.G : c != 0) return;
   WM_PDL_WAIT();
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
-  const int64_t total = warp_units(a, a.B) * PH, nu = units_of(a, b);
-  const int64_t first = warp_units(a, b) * PH + hc * nu;
+  int64_t total = 0, first = 0;                       // units of all sequences, and of those before b
+  for (int x = lane; x < a.B; x += 32) {
+    const int64_t n = units_of(a, x);
+    total += n;
+    first += x < b ? n : 0;
+  }
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, m);
+    first += __shfl_xor_sync(0xffffffffu, first, m);
+  }
+  const int64_t nu = units_of(a, b);
+  total *= PH;
+  first = first * PH + hc * nu;
   const int len = a.lengths[b];
   const bool bad = len < 0 || len > cap;
   const float nan = __uint_as_float(0x7fc00000u);
-  // CTAs that hold units first .. first + nu - 1
   const int64_t n_cta = parts_of(a, total);
-  const int64_t i0 = nu ? ((first + 1) * n_cta - 1) / total : 0, i1 = nu ? ((first + nu) * n_cta - 1) / total : -1;
-  const float *pm = a.part_m + (i0 + pair) * kHeads, *pl = a.part_l + (i0 + pair) * kHeads;
-  const int np = static_cast<int>(i1 - i0 + 1);
-  auto stats = [&](int hd, float &top, float &sum) {  // by one warp
-    top = kNegInf;
-    for (int i = lane; i < np; i += 32) top = fmaxf(top, pm[i * kHeads + hd]);
+  // CTAs that hold the nu units from `at`
+  auto part0 = [&](int64_t at) { return nu ? ((at + 1) * n_cta - 1) / total : 0; };
+  auto parts = [&](int64_t at) { return nu ? static_cast<int>(((at + nu) * n_cta - 1) / total - part0(at)) + 1 : 0; };
+
+  if (static_cast<int>(blockIdx.y) < heads) {
+    const int hd = blockIdx.y, hg = c * kHeads + hd, np = parts(first);
+    const int64_t slot0 = part0(first) + pair;
+    const float *pm = a.part_m + slot0 * kHeads + hd, *pl = a.part_l + slot0 * kHeads + hd;
+    float m0 = kNegInf, l0 = 0.0f;                    // part `tid`
+    if (tid < np) {
+      m0 = pm[tid * kHeads];
+      l0 = pl[tid * kHeads];
+    }
+    float top = m0;
+    for (int i = tid + kJoin; i < np; i += kJoin) top = fmaxf(top, pm[i * kHeads]);
 #pragma unroll
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    sum = 0.0f;
-    for (int i = lane; i < np; i += 32) {
-      const float mi = pm[i * kHeads + hd];
-      sum += pl[i * kHeads + hd] * (mi == kNegInf ? 1.0f : ex2(mi - top));
+    if (lane == 0) s_red[0][warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+
+    const int col = tid % kCols, grp = tid / kCols;
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = 0; p0 < np; p0 += kJoin) {
+      const int i = p0 + tid;
+      float f = 0.0f;
+      if (i < np) {
+        f = part_factor(p0 ? pm[i * kHeads] : m0, top);
+        sum += f * (p0 ? pl[i * kHeads] : l0);
+      }
+      if (p0) __syncthreads();
+      s_f[tid] = f;
+      __syncthreads();
+      const float4 *po = reinterpret_cast<const float4 *>(a.part_o + ((slot0 + p0) * kHeads + hd) * D) + col;
+      const int m = min(kJoin, np - p0);
+#pragma unroll 8
+      for (int y = grp; y < m; y += kGroups) {
+        const float4 v = po[static_cast<int64_t>(y) * (kHeads * kCols)];
+        const float fy = s_f[y];
+        o.x = fmaf(v.x, fy, o.x);
+        o.y = fmaf(v.y, fy, o.y);
+        o.z = fmaf(v.z, fy, o.z);
+        o.w = fmaf(v.w, fy, o.w);
+      }
     }
 #pragma unroll
     for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-  };
-
-  if (blockIdx.y < kHeads) {
-    const int hd = blockIdx.y, hg = c * kHeads + hd;
-    if (hg >= a.G) return;
-    float top, sum;
-    stats(hd, top, sum);
+    if (lane == 0) s_red[1][warp] = sum;
+    s_o[tid] = o;
+    __syncthreads();
+    sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
     const int64_t head = static_cast<int64_t>(b) * a.Hq + h * a.G + hg;
-    const float inv = bad ? nan : (np > 0 ? 1.0f / sum : 0.0f);
-    if (a.lse && threadIdx.x == 0) a.lse[head] = bad ? nan : (np > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
-    const float *po = a.part_o + ((i0 + pair) * kHeads + hd) * D;
-    for (int d = threadIdx.x * 2; d < D; d += kJoin * 2) {
-      float x = 0.0f, y = 0.0f;
-      for (int i = 0; i < np; ++i) {
-        const float mi = pm[i * kHeads + hd];
-        const float f = mi == kNegInf ? 1.0f : ex2(mi - top);
-        const float2 v = *reinterpret_cast<const float2 *>(po + static_cast<int64_t>(i) * kHeads * D + d);
-        x = fmaf(v.x, f, x);
-        y = fmaf(v.y, f, y);
+    if (tid < kCols) {
+#pragma unroll
+      for (int y = 1; y < kGroups; ++y) {
+        const float4 v = s_o[y * kCols + tid];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
       }
-      reinterpret_cast<uint32_t *>(a.out + head * D + d)[0] = bf16x2(x * inv, y * inv);
+      const float inv = bad ? nan : (np > 0 ? 1.0f / sum : 0.0f);
+      reinterpret_cast<uint2 *>(a.out + head * D)[tid] = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
     }
+    if (a.lse && tid == 0) a.lse[head] = bad ? nan : (np > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
     return;
   }
-  // mass: sum over the kv head's query heads; one chunk at a time adds (chunk 0's block does all of them)
-  const int64_t k0 = static_cast<int64_t>(blockIdx.y - kHeads) * kRun;
-  if (c != 0 || bad || k0 >= len) return;
+
+  // mass: the weights of keys [k0, k1), summed over the query heads of all chunks
+  const int64_t k0 = static_cast<int64_t>(blockIdx.y - heads) * kRun;
+  if (bad || k0 >= len) return;
   const int64_t k1 = k0 + kRun < len ? k0 + kRun : len;
   float *mass = a.mass + (static_cast<int64_t>(b) * a.pool.Hkv + h) * cap;
   float acc[kRun / kJoin];
 #pragma unroll
   for (int x = 0; x < kRun / kJoin; ++x) acc[x] = 0.0f;
   for (int cc = 0; cc < a.NC; ++cc) {
-    const int64_t f2 = first + cc * nu;
-    const int64_t j0 = ((f2 + 1) * n_cta - 1) / total, j1 = ((f2 + nu) * n_cta - 1) / total;
-    const float *qm = a.part_m + (j0 + pair + cc) * kHeads, *ql = a.part_l + (j0 + pair + cc) * kHeads;
-    const int nq = static_cast<int>(j1 - j0 + 1);
+    const int64_t at = first + cc * nu, slot0 = part0(at) + pair + cc;
+    const int n = parts(at) * kHeads;
+    const float *qm = a.part_m + slot0 * kHeads, *ql = a.part_l + slot0 * kHeads;
+    // thread t joins every (kJoin / kHeads)-th part of head t % kHeads
+    float top = kNegInf, sum = 0.0f;
+#pragma unroll 4
+    for (int i = tid; i < n; i += kJoin) {
+      const float mi = qm[i], li = ql[i], t = fmaxf(top, mi);
+      sum = sum * part_factor(top, t) + li * part_factor(mi, t);
+      top = t;
+    }
+    s_st[tid] = make_float2(top, sum);
     __syncthreads();
-    for (int hd = warp; hd < kHeads; hd += kJoin / 32) {
-      float top = kNegInf, sum = 0.0f;
-      for (int i = lane; i < nq; i += 32) top = fmaxf(top, qm[i * kHeads + hd]);
-#pragma unroll
-      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      for (int i = lane; i < nq; i += 32) {
-        const float mi = qm[i * kHeads + hd];
-        sum += ql[i * kHeads + hd] * (mi == kNegInf ? 1.0f : ex2(mi - top));
+    if (tid < kHeads) {
+      for (int y = tid + kHeads; y < kJoin; y += kHeads) {
+        const float2 v = s_st[y];
+        const float t = fmaxf(top, v.x);
+        sum = sum * part_factor(top, t) + v.y * part_factor(v.x, t);
+        top = t;
       }
-#pragma unroll
-      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (lane == 0) s_lse2[hd] = top + log2f(sum);
+      s_lse2[tid] = top + log2f(sum);
     }
     __syncthreads();
     const int live = min(kHeads, a.G - cc * kHeads);
-    const float *sc = a.scores + (pair + cc) * cap * kHeads;
+    const float *sc = a.scores + (pair + cc) * cap * a.score_heads;
 #pragma unroll
     for (int x = 0; x < kRun / kJoin; ++x) {
-      const int64_t key = k0 + x * kJoin + threadIdx.x;
-      if (key < k1)
-        for (int hd = 0; hd < live; ++hd) acc[x] += ex2(sc[key * kHeads + hd] - s_lse2[hd]);
+      const int64_t key = k0 + x * kJoin + tid;
+      if (key < k1) {
+        const float2 *sp = reinterpret_cast<const float2 *>(sc + key * a.score_heads);
+#pragma unroll
+        for (int y = 0; y < kHeads / 2; ++y)
+          if (2 * y < live) {
+            const float2 v = sp[y];
+            acc[x] += ex2(v.x - s_lse2[2 * y]);
+            if (2 * y + 1 < live) acc[x] += ex2(v.y - s_lse2[2 * y + 1]);
+          }
+      }
     }
   }
 #pragma unroll
   for (int x = 0; x < kRun / kJoin; ++x) {
-    const int64_t key = k0 + x * kJoin + threadIdx.x;
+    const int64_t key = k0 + x * kJoin + tid;
     if (key < k1) mass[key] += acc[x];
   }
 }
@@ -624,14 +689,14 @@ int grid_of(int64_t most_units) {
 template <int D, int FMT, int NH>
 int launch(DecodeArgs &a, cudaStream_t stream) {
   using S = Shape<D, FMT, NH>;
-  auto kern = k_attn_decode<D, FMT, NH>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (e == cudaSuccess) e = wm::launch_pdl(kern, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
+  cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH>>(S::kSmem);
+  if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
   const unsigned runs = a.mass ? static_cast<unsigned>((cap + kRun - 1) / kRun) : 0u;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC), S::kHeads + runs);
-  e = wm::launch_pdl(k_attn_join<NH>, grid, dim3(kJoin), 0, stream, a, D);
+  const int heads = std::min(S::kHeads, a.G);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC), heads + runs);
+  e = wm::launch_pdl(k_attn_join<D, NH>, grid, dim3(kJoin), 0, stream, a, heads);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   return wm::check_launch("wattn_decode");
 }
@@ -664,7 +729,7 @@ struct Launch {
 };
 
 struct Plan {
-  int NC, heads, n_cta;
+  int NC, heads, score_heads, n_cta;
   int64_t pairs, slots, cap;
   size_t off_m, off_l, off_s, bytes;
 };
@@ -674,6 +739,7 @@ Plan plan_of(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_page
   const int G = Hq / Hkv;
   p.heads = chunk_heads(G);
   p.NC = (G + p.heads - 1) / p.heads;
+  p.score_heads = std::min(p.heads, (G + 1) & ~1);
   p.pairs = static_cast<int64_t>(B) * Hkv * p.NC;
   p.cap = static_cast<int64_t>(max_pages) * page_size;
   p.n_cta = dispatch(D, fmt, G, GridOf{p.pairs * ((p.cap + kUnit - 1) / kUnit)});
@@ -682,7 +748,7 @@ Plan plan_of(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_page
   p.off_m = up(static_cast<size_t>(p.slots) * p.heads * D * 4);
   p.off_l = p.off_m + up(static_cast<size_t>(p.slots) * p.heads * 4);
   p.off_s = p.off_l + up(static_cast<size_t>(p.slots) * p.heads * 4);
-  p.bytes = p.off_s + (with_mass ? static_cast<size_t>(p.pairs) * p.cap * p.heads * 4 : 0);
+  p.bytes = p.off_s + (with_mass ? static_cast<size_t>(p.pairs) * p.cap * p.score_heads * 4 : 0);
   return p;
 }
 
@@ -712,8 +778,8 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
   WM_REQUIRE(scale > 0.0f && scale <= 3.4028234663852886e38f, "decode attention: the scale must be positive and finite");
   if (B == 0) return WM_OK;
   WM_REQUIRE(q && lengths && out, "decode attention: missing input or output");
-  WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && q_stride % 2 == 0 && wm::aligned(q, 4) && wm::aligned(out, 4),
-             "decode attention: query rows must be 4-byte aligned and hold Hq * D values");
+  WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && q_stride % 2 == 0 && wm::aligned(q, 4) && wm::aligned(out, 8),
+             "decode attention: query rows must be 4-byte aligned and hold Hq * D values, the output 8-byte aligned");
   const Plan p = plan_of(B, Hq, Hkv, D, fmt, page_size, max_pages, mass != nullptr);
   WM_REQUIRE(p.pairs <= INT32_MAX && (p.cap + kRun - 1) / kRun <= 65000, "decode attention: batch or capacity too large");
   if (ws_bytes < p.bytes) return wm::fail(WM_ERR_WORKSPACE, "decode attention: workspace too small");
@@ -721,7 +787,7 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   DecodeArgs a{pool, q, q_stride, lengths, B, Hq, Hq / Hkv, p.NC, scale * kLog2e, out, lse, mass,
                reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + p.off_m), reinterpret_cast<float *>(ws + p.off_l),
-               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.n_cta};
+               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.score_heads, p.n_cta};
   return dispatch(D, fmt, a.G, Launch{a, stream});
 }
 

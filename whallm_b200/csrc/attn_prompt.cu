@@ -718,10 +718,9 @@ int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t
   // at most one partial block per sequence beyond the rows' own blocks
   const int64_t most = (static_cast<int64_t>(a.Tq) * a.G / C::kRows + a.B) * a.Hkv;
   const int grid = static_cast<int>(std::min<int64_t>(most, wm::sm_count()));
-  auto kern = k_attn_prompt<D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+  const cudaError_t e = wm::allow_smem<k_attn_prompt<D>>(smem_bytes<D>());
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
-  kern<<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mk, mv);
+  k_attn_prompt<D><<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mk, mv);
   return wm::check_launch("wattn_prompt");
 }
 

@@ -374,7 +374,7 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   const int key_cap = static_cast<int>(std::min<int64_t>(slice, kKeySmem));
   const size_t smem = static_cast<size_t>(key_cap) * 4;
   WM_REQUIRE(heads * C <= INT32_MAX, "evict: too many sequences");
-  cudaError_t e = cudaFuncSetAttribute(k_paged_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeySmem * 4);
+  cudaError_t e = wm::allow_smem<k_paged_evict>(kKeySmem * 4);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wkv_paged_evict: ") + cudaGetErrorString(e));
   const EvictArgs args{pool, lengths, seen, mass, positions, mass_out, positions_out, lengths_out,
                        static_cast<int32_t *>(workspace), n, recent, sinks, wm_paged::row_bytes(fmt, D) / 16,
