@@ -64,6 +64,7 @@ struct PromptArgs {
   int64_t q_stride, v_stride;
   const int32_t *cu_q, *cu_k;
   int B, Tq, Tk, Hq, Hkv, G, causal;
+  int q_tma;                // G divides 128: a tile of packed rows is one box of q
   float scale2;
   wm_bf16 *out;
   float *lse;
@@ -94,7 +95,7 @@ struct Item {
 
 struct Bars {
   uint64_t item_full[2], item_empty[2], odd_ready[2];
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2], q_empty[2], next_full;          // per 128-row tile
   // an edge tile (values that some row does not see) lands on v_edge, not kv_full: the helpers wait for it, and the
   // MMA warp for v_fixed.  Both advance only with edge tiles, so a phase cannot pass unseen
   uint64_t kv_full[8], kv_empty[8], v_edge[8], v_fixed[8];
@@ -102,6 +103,7 @@ struct Bars {
 };
 
 struct Shared {
+  uint4 next;               // answer to the request for another work item
   Bars bar;
   Item item[2];
   uint32_t tmem;
@@ -109,9 +111,10 @@ struct Shared {
   float m[128], l[2][128];  // D = 256: shared reference points, and each warpgroup's sums at the end
 };
 
-// The tiles start at a multiple of 1024 bytes.
+// The tiles need 1024-byte alignment: the kernel has no static shared memory, so
+// its dynamic part begins at such an address (else the call ends with NaN).
 template <int D>
-constexpr int smem_bytes() { return Cfg<D>::kQBytes + Cfg<D>::kSlots * Cfg<D>::kSlot + static_cast<int>(sizeof(Shared)) + 896; }
+constexpr int smem_bytes() { return Cfg<D>::kQBytes + Cfg<D>::kSlots * Cfg<D>::kSlot + static_cast<int>(sizeof(Shared)); }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "shared memory of a CTA");
 
 // Bounded wait of a whole warp: all its lanes return the same answer.  A wait
@@ -211,6 +214,33 @@ __device__ __forceinline__ int pos_k(int j) { return Cfg<D>::kChain ? (j == 0 ? 
 template <int D>
 __device__ __forceinline__ int pos_v(int j, int n) { return Cfg<D>::kChain ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; }
 
+// Work items are the blocks of the grid: a CTA that has started its item asks the
+// hardware for a block that has not been launched yet and takes its number over
+// (cluster launch control), so items are handed out in order to whoever is free,
+// without a counter in memory.
+__device__ __forceinline__ void ask_next(Shared *sh) {
+  mbar_expect_tx(&sh->bar.next_full, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&sh->next)),
+               "r"(smem_u32(&sh->bar.next_full))
+               : "memory");
+}
+// The block number taken over, or -1 if none was left.
+__device__ __forceinline__ int64_t read_next(Shared *sh) {
+  uint32_t got, x = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(&sh->next))
+      : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next answer overwrites this one
+  return got ? static_cast<int64_t>(x) : -1;
+}
+
 // Work item number x by one warp: blocks of all sequences from the last block of
 // the last sequence backwards (within a causal sequence the longest first), heads
 // innermost.
@@ -220,7 +250,7 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int64_t x, Item *
   const int lane = threadIdx.x & 31;
   int64_t blk = x / a.Hkv;
   const int h = static_cast<int>(x - blk * a.Hkv);
-  for (int hi = a.B; hi > 0; hi -= 32) {              // lane l: sequence hi - 1 - l
+  for (int hi = x < 0 ? 0 : a.B; hi > 0; hi -= 32) {  // lane l: sequence hi - 1 - l
     const int b = hi - 1 - lane;
     int q0 = 0, nq = 0, k0 = 0, nk = 0;
     if (b >= 0) seq_bounds(a, b, q0, nq, k0, nk);
@@ -253,15 +283,15 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int64_t x, Item *
     }
     blk -= __shfl_sync(0xffffffffu, s, 31);
   }
-  if (lane == 0) out->valid = 0;
+  if (lane == 0) out->valid = 0;                      // x < 0 or past the last block
 }
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attn_prompt(PromptArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    k_attn_prompt(PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<D>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
   Shared &sh = *reinterpret_cast<Shared *>(smem + C::kQBytes + C::kSlots * C::kSlot);
   const uint32_t q_s = smem_u32(smem), kv_s = q_s + C::kQBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -272,13 +302,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.item_full[i], 1);
       mbar_init(&b.item_empty[i], 8 + 1 + 2);         // softmax, MMA and helper warps
       mbar_init(&b.odd_ready[i], kHelpers);
+      mbar_init(&b.q_full[i], a.q_tma ? 1 : kHelpers);
+      mbar_init(&b.q_empty[i], 1);
       mbar_init(&b.s_full[i], 1);
       mbar_init(&b.p_ready[i], 128);
       mbar_init(&b.o_done[i], 1);
       mbar_init(&b.m_ready[i], 128);
     }
-    mbar_init(&b.q_full, kHelpers);
-    mbar_init(&b.q_empty, 1);
+    mbar_init(&b.next_full, 1);
     mbar_init(&b.o_free, 256);
     mbar_init(&b.both, 256);
     for (int i = 0; i < C::kSlots; ++i) {
@@ -287,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.v_edge[i], 1);
       mbar_init(&b.v_fixed[i], kHelpers);
     }
-    sh.abort = 0;
+    sh.abort = (smem_u32(smem) & 1023u) != 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -300,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sh.tmem;
   Bars &bar = sh.bar;
 
-  if (warp >= 8) {
+  if (sh.abort) {
+  } else if (warp >= 8) {
     // 384 threads at 168 registers are launched: 256 x 208 + 128 x 88 is the same sum
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
@@ -308,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t g = 0;                                  // loads so far
       uint32_t edge_ph = 0u, edge_last = 0u;          // per slot: phase of v_edge, and whether the last load was an edge tile
       int it = 0;
-      for (int64_t x = blockIdx.x;; x += gridDim.x, ++it) {
+      for (int64_t x = blockIdx.x;; ++it) {
         const int sl = it & 1;
         if (!wait(&sh, &bar.item_empty[sl], ((it >> 1) & 1) ^ 1)) break;
         Item *item = &sh.item[sl];
@@ -316,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.item_full[sl]);
         if (!item->valid) break;
+        if (elect_one()) ask_next(&sh);
         const int n = item->tiles, first = item->first;
         bool ok = true;
         for (int p = 0; ok && p < 2 * n; ++p, ++g) {
@@ -345,7 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         }
-        if (!ok) break;
+        if (!ok || !wait(&sh, &bar.next_full, it & 1)) break;
+        x = read_next(&sh);
+        __syncwarp();
       }
       // loads in flight when the others gave up must land before the CTA leaves
       if (*reinterpret_cast<volatile int *>(&sh.abort))
@@ -372,13 +407,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
         if (!valid) break;
         const int steps = n * C::kTiles;
-        ok = wait(&sh, &bar.q_full, it & 1);
-        if (!ok) break;
         auto slot_of = [&](int64_t gg) { return static_cast<int>(gg % C::kSlots); };
         auto phase_of = [&](int64_t gg) { return static_cast<uint32_t>((gg / C::kSlots) & 1); };
         auto issue_s = [&](int s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1;
           const int64_t gg = g0 + pos_k<D>(j);
+          if (j == 0 && !wait(&sh, &bar.q_full[w], it & 1)) return false;
           if (!wait(&sh, &bar.kv_full[slot_of(gg)], phase_of(gg))) return false;
           tc_fence_after();
           if (elect_one()) {
@@ -389,12 +423,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                      wm_tc::bdesc_sw128(kb + (kk >> 2) * C::kPanel + (kk & 3) * 32), id_s, kk != 0);
             tc_commit(&bar.s_full[s & 1]);
             if (C::kChain || w == 1) tc_commit(&bar.kv_empty[slot_of(gg)]);
-            if (s == steps - 1) tc_commit(&bar.q_empty);
+            if (s >= steps - C::kTiles) tc_commit(&bar.q_empty[w]);
           }
           __syncwarp();
           return true;
         };
-        if (steps == 0 && lane == 0) mbar_arrive(&bar.q_empty);       // nothing to read Q for
+        if (steps == 0)                               // nothing to read Q for
+          for (int w = 0; ok && w < C::kTiles; ++w) {
+            ok = wait(&sh, &bar.q_full[w], it & 1);
+            if (ok && lane == 0) mbar_arrive(&bar.q_empty[w]);
+          }
         for (int s = 0; ok && s < 2 && s < steps; ++s) ok = issue_s(s);
         if (ok && it > 0) ok = wait(&sh, &bar.o_free, (it - 1) & 1);  // the last item's O has been read
         for (int s = 0; ok && s < steps; ++s) {
@@ -437,21 +475,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!item->valid) break;
         const int n = item->tiles, first = item->first, nk = item->nk;
         const int64_t rows = static_cast<int64_t>(item->nq) * a.G;
-        ok = wait(&sh, &bar.q_empty, (it & 1) ^ 1);
-        if (!ok) break;
-        const int R0 = item->blk * C::kRows;
-        constexpr int per = D / 8;                    // 16-byte pieces of a row
-        for (int x = ht; x < C::kRows * per; x += kHelpers) {
-          const int r = x / per, c = x % per;
-          const bool in = R0 + r < rows;
-          const int i = in ? (R0 + r) / a.G : 0, hg = in ? (R0 + r) - i * a.G : 0;
-          const wm_bf16 *src = a.q + (static_cast<int64_t>(item->q0) + i) * a.q_stride + static_cast<int64_t>(item->h * a.G + hg) * D + c * 8;
-          const uint32_t dst = q_s + (r >> 7) * (128 * D * 2) + (c >> 3) * 16384 + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+        for (int w = 0; ok && w < C::kTiles; ++w) {
+          ok = wait(&sh, &bar.q_empty[w], (it & 1) ^ 1);
+          if (!ok) break;
+          const int R0 = item->blk * C::kRows + w * 128;
+          const uint32_t qt = q_s + w * (128 * D * 2);
+          if (a.q_tma) {
+            // rows behind the sequence bring other rows' values; they are computed and not stored
+            if (warp == 10 && elect_one()) {
+              mbar_expect_tx(&bar.q_full[w], 128 * D * 2);
+#pragma unroll
+              for (int d = 0; d < D / 64; ++d)
+                tma_load_3d(qt + d * 16384, &map_q, d * 64, item->h * a.G, item->q0 + R0 / a.G, &bar.q_full[w]);
+            }
+            __syncwarp();
+            continue;
+          }
+          constexpr int per = D / 8;                  // 16-byte pieces of a row
+          constexpr int kStep = kHelpers / per;       // rows that the helpers copy at once
+          const int c = ht % per;
+          int r = ht / per, i = (R0 + r) / a.G, hg = R0 + r - i * a.G;
+          const wm_bf16 *base = a.q + static_cast<int64_t>(item->q0) * a.q_stride + static_cast<int64_t>(item->h) * a.G * D + c * 8;
+#pragma unroll 4
+          for (; r < 128; r += kStep) {
+            const bool in = R0 + r < rows;
+            const wm_bf16 *src = base + (in ? i * a.q_stride + static_cast<int64_t>(hg) * D : 0);
+            const uint32_t dst = qt + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+            for (hg += kStep; hg >= a.G; hg -= a.G) ++i;
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&bar.q_full[w]);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&bar.q_full);
         for (int j = first; ok && j < n; ++j) {
           const int64_t gg = g0 + pos_v<D>(j, n);
           const int slot = static_cast<int>(gg % C::kSlots);
@@ -692,13 +748,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // [tokens, heads, D] bf16 with `stride` values between tokens, boxes of 64
-// dimensions x 1 head x `rows` tokens; tokens behind the last read as zeros.
-int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t tokens, int64_t stride, int rows) {
+// dimensions x box_heads heads x box_rows tokens; tokens behind the last read as
+// zeros.
+int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t tokens, int64_t stride, int box_heads, int box_rows) {
   auto fn = wm_tc::encode_fn();
   if (!fn) return wm::fail(WM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(stride) * 2};
-  cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -710,17 +767,19 @@ int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t toke
 template <int D>
 int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t stream) {
   using C = Cfg<D>;
-  CUtensorMap mk, mv;
+  CUtensorMap mq, mk, mv;
+  if (int rc = make_map3(&mq, a.q, D, a.Hq, a.Tq, a.q_stride, a.q_tma ? a.G : 1, a.q_tma ? 128 / a.G : 128)) return rc;
   // without keys no tile is loaded; the maps then describe one row of q
   const bool any = a.Tk > 0;
-  if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, C::kN)) return rc;
-  if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, C::kN)) return rc;
+  if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, 1, C::kN)) return rc;
+  if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, 1, C::kN)) return rc;
   // at most one partial block per sequence beyond the rows' own blocks
   const int64_t most = (static_cast<int64_t>(a.Tq) * a.G / C::kRows + a.B) * a.Hkv;
-  const int grid = static_cast<int>(std::min<int64_t>(most, wm::sm_count()));
+  WM_REQUIRE(most <= INT32_MAX, "prompt attention: too many rows");
+  const int grid = static_cast<int>(std::max<int64_t>(most, 1));
   const cudaError_t e = wm::allow_smem<k_attn_prompt<D>>(smem_bytes<D>());
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
-  k_attn_prompt<D><<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mk, mv);
+  k_attn_prompt<D><<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mq, mk, mv);
   return wm::check_launch("wattn_prompt");
 }
 
@@ -744,7 +803,7 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
              "prompt attention: token rows must be 16-byte aligned and hold their heads");
   WM_REQUIRE(static_cast<int64_t>(Tq) * (Hq / Hkv) <= INT32_MAX - 256, "prompt attention: too many rows per key-value head");
   const PromptArgs a{q, v, q_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, Hq / Hkv, causal,
-                     scale * kLog2e, out, lse};
+                     128 % (Hq / Hkv) == 0, scale * kLog2e, out, lse};
   if (D == 64) return launch<64>(a, k, k_stride, stream);
   if (D == 128) return launch<128>(a, k, k_stride, stream);
   return launch<256>(a, k, k_stride, stream);
