@@ -99,7 +99,7 @@ struct Bars {
   // an edge tile (values that some row does not see) lands on v_edge, not kv_full: the helpers wait for it, and the
   // MMA warp for v_fixed.  Both advance only with edge tiles, so a phase cannot pass unseen
   uint64_t kv_full[8], kv_empty[8], v_edge[8], v_fixed[8];
-  uint64_t s_full[2], p_ready[2], o_done[2], m_ready[2], o_free, both;
+  uint64_t s_full[2], p_half[2], p_ready[2], o_done[2], m_ready[2], o_free, both;
 };
 
 struct Shared {
@@ -117,14 +117,29 @@ template <int D>
 constexpr int smem_bytes() { return Cfg<D>::kQBytes + Cfg<D>::kSlots * Cfg<D>::kSlot + static_cast<int>(sizeof(Shared)); }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "shared memory of a CTA");
 
+// try_wait without a suspend hint: with the hint of the other kernels' waits a
+// warp saw a completed phase 400 to 500 cycles late, which is on the critical
+// path here twice per step.
+__device__ __forceinline__ bool try_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait of a whole warp: all its lanes return the same answer.  A wait
 // that runs out makes every other wait of the CTA end, too.
 __device__ __forceinline__ bool wait(Shared *sh, uint64_t *bar, uint32_t parity) {
-  if (__all_sync(0xffffffffu, wm_tc::mbar_try(bar, parity))) return true;
+  if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
   const unsigned long long t0 = wm_tc::gtimer();
   while (true) {
-    for (int i = 0; i < 8; ++i)
-      if (__all_sync(0xffffffffu, wm_tc::mbar_try(bar, parity))) return true;
+    for (int i = 0; i < 64; ++i)
+      if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
     const bool late = wm_tc::gtimer() - t0 > wm_tc::kWaitNs;
     if (late) *reinterpret_cast<volatile int *>(&sh->abort) = 1;
     if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int *>(&sh->abort) != 0)) return false;
@@ -138,21 +153,34 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
+// Shared memory operands by the low half of their descriptors (start address,
+// panel distance); the high half, 8-row groups 1024 B apart in the 128-byte
+// swizzle, is the same for all.  K-major: rows of 128 B, 16 values further along
+// K are 32 B.  MN-major (V): rows of 64 values along MN, panels of 64 MN values
+// kPanel apart, 16 keys further along K are 2048 B.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr, uint32_t panel) { return ((saddr & 0x3FFFFu) >> 4) | ((panel >> 4) << 16); }
+
 // D[tmem] (+)= A[smem] * B[smem]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
       : "memory");
 }
-
-// MN-major operand in the 128-byte swizzle: rows of 64 MN values (128 B), groups
-// of 8 rows along K 1024 B apart, panels of 64 MN values `panel` bytes apart.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t panel) {
-  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(panel >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
+      : "memory");
 }
 
 // kind::f16 instruction descriptor: bf16 x bf16 -> f32, M = 128; B MN-major for PV
@@ -178,9 +206,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       WM_U8(r, 0), WM_U8(r, 8), WM_U8(r, 16), WM_U8(r, 24)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      WM_U8(r, 0), WM_U8(r, 8)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -305,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.q_full[i], a.q_tma ? 1 : kHelpers);
       mbar_init(&b.q_empty[i], 1);
       mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_half[i], 128);
       mbar_init(&b.p_ready[i], 128);
       mbar_init(&b.o_done[i], 1);
       mbar_init(&b.m_ready[i], 128);
@@ -393,39 +433,57 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 9) {
       // ------------------------------------------------------------- MMAs
+      // One thread issues, but the whole warp keeps the state, and what it reads from shared memory goes
+      // through a warp reduction: the compiler then sees uniform values, and descriptors and addresses stay
+      // in uniform registers.  With state in ordinary registers each MMA took about 130 cycles to issue,
+      // twice its time on the tensor core.
       constexpr uint32_t id_s = idesc_bf16(C::kN, false), id_o = idesc_bf16(D, true);
-      int64_t g0 = 0;                                 // loads before this item
-      uint32_t fixed = 0u, pph = 0u;                  // phase bits: v_fixed per slot, p_ready per buffer
+      struct Ring {
+        int slot;
+        uint32_t ph;
+        __device__ __forceinline__ void next(int d) {
+          slot += d;
+          if (slot >= C::kSlots) {
+            slot -= C::kSlots;
+            ph ^= 1u;
+          }
+        }
+      };
+      Ring base{0, 0u};                               // load position of this item's first key tile
+      uint32_t fixed = 0u, pph = 0u;                  // phase bits: v_fixed per slot, P per buffer
+      const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
       bool ok = true;
       for (int it = 0; ok; ++it) {
         const int sl = it & 1;
         ok = wait(&sh, &bar.item_full[sl], (it >> 1) & 1);
         if (!ok) break;
         const Item *item = &sh.item[sl];
-        const int n = item->tiles, first = item->first, valid = item->valid;
+        const int n = __reduce_max_sync(0xffffffffu, item->tiles), first = __reduce_max_sync(0xffffffffu, item->first);
+        const int valid = __reduce_max_sync(0xffffffffu, item->valid);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
         if (!valid) break;
         const int steps = n * C::kTiles;
-        auto slot_of = [&](int64_t gg) { return static_cast<int>(gg % C::kSlots); };
-        auto phase_of = [&](int64_t gg) { return static_cast<uint32_t>((gg / C::kSlots) & 1); };
+        // key tiles at load positions 0, 2, 4, ... and value tiles at 1, 3, ...; at D = 256 0, 1, 3, 5, ... and
+        // 2, 4, ..., 2 n - 2, 2 n - 1
+        Ring rk = base, rv = base;
+        rv.next(C::kChain && n > 1 ? 2 : 1);
         auto issue_s = [&](int s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1;
-          const int64_t gg = g0 + pos_k<D>(j);
           if (j == 0 && !wait(&sh, &bar.q_full[w], it & 1)) return false;
-          if (!wait(&sh, &bar.kv_full[slot_of(gg)], phase_of(gg))) return false;
+          if (!wait(&sh, &bar.kv_full[rk.slot], rk.ph)) return false;
           tc_fence_after();
+          const uint32_t qa = desc_k(q_s + w * (128 * D * 2)), kb = desc_k(kv_s + rk.slot * C::kSlot), d = tm + (s & 1) * C::kN;
           if (elect_one()) {
-            const uint32_t qa = q_s + w * (128 * D * 2), kb = kv_s + slot_of(gg) * C::kSlot;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss(tmem + (s & 1) * C::kN, wm_tc::bdesc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32),
-                     wm_tc::bdesc_sw128(kb + (kk >> 2) * C::kPanel + (kk & 3) * 32), id_s, kk != 0);
+              mma_ss(d, qa + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * C::kPanel + (kk & 3) * 32) >> 4), id_s, kk != 0);
             tc_commit(&bar.s_full[s & 1]);
-            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[slot_of(gg)]);
+            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[rk.slot]);
             if (s >= steps - C::kTiles) tc_commit(&bar.q_empty[w]);
           }
           __syncwarp();
+          if (C::kChain || w == 1) rk.next(C::kChain && j == 0 ? 1 : 2);
           return true;
         };
         if (steps == 0)                               // nothing to read Q for
@@ -437,29 +495,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && it > 0) ok = wait(&sh, &bar.o_free, (it - 1) & 1);  // the last item's O has been read
         for (int s = 0; ok && s < steps; ++s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1, buf = s & 1;
-          const int64_t gg = g0 + pos_v<D>(j, n);
-          const int slot = slot_of(gg);
-          ok = wait(&sh, &bar.kv_full[slot], phase_of(gg));
+          ok = wait(&sh, &bar.kv_full[rv.slot], rv.ph);
           if (ok && j >= first && w == 0) {
-            ok = wait(&sh, &bar.v_fixed[slot], (fixed >> slot) & 1u);
-            fixed ^= 1u << slot;
+            ok = wait(&sh, &bar.v_fixed[rv.slot], (fixed >> rv.slot) & 1u);
+            fixed ^= 1u << rv.slot;
           }
-          ok = ok && wait(&sh, &bar.p_ready[buf], (pph >> buf) & 1u);
+          // the keys of P's first half are multiplied while the softmax still works on the second
+          constexpr int kHalf = C::kN / 32;
+          const uint32_t vb = desc_mn(kv_s + rv.slot * C::kSlot, C::kPanel), o = tm + C::kOCol + w * D, p = tm + buf * C::kN;
+          ok = ok && wait(&sh, &bar.p_half[buf], (pph >> buf) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kHalf; ++kk) mma_ts(o, p + kk * 8, vb + kk * (2048 >> 4), id_o, (j | kk) != 0);
+          }
+          __syncwarp();
+          ok = wait(&sh, &bar.p_ready[buf], (pph >> buf) & 1u);
           pph ^= 1u << buf;
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t vb = kv_s + slot * C::kSlot, o = tmem + C::kOCol + w * D, p = tmem + buf * C::kN;
 #pragma unroll
-            for (int kk = 0; kk < C::kN / 16; ++kk)
-              wm_tc::tc_mma_ts(o, p + kk * 8, desc_mn(vb + kk * 2048, C::kPanel), id_o, (j | kk) != 0);
+            for (int kk = kHalf; kk < 2 * kHalf; ++kk) mma_ts(o, p + kk * 8, vb + kk * (2048 >> 4), id_o, 1u);
             if (C::kChain || s >= steps - 2) tc_commit(&bar.o_done[buf]);
-            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[slot]);
+            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[rv.slot]);
           }
           __syncwarp();
+          if (s == steps - 1) {                       // the last load of the item
+            base = rv;
+            base.next(1);
+          }
+          if (C::kChain || w == 1) rv.next(C::kChain && j == n - 2 ? 1 : 2);
           if (s + 2 < steps) ok = issue_s(s + 2);
         }
-        g0 += 2 * n;
       }
     } else {
       // --------------------------------- query rows, and values of edge tiles
@@ -591,7 +660,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[0][c]);
 #pragma unroll
-        for (int c = 4; c < C::kN; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c >> 5][c & 31]));
+        for (int c = 4; c + 8 <= C::kN; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            mx[e] = max3(mx[e], __uint_as_float(x[(c + 2 * e) >> 5][(c + 2 * e) & 31]), __uint_as_float(x[(c + 2 * e + 1) >> 5][(c + 2 * e + 1) & 31]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[C::kN / 32 - 1][28 + e]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
         if constexpr (C::kChain) {
           if (s > 0) {                                // the reference point as the other warpgroup left it
@@ -636,18 +710,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 sc = make_float2(a.scale2, a.scale2), nb = make_float2(-base, -base);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-        for (int h = 0; h < C::kN / 64; ++h) {        // 64 keys: 32 registers of P
-          uint32_t p[32];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[C::kN / 4];                      // half of the keys
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int c = h * 64 + 2 * i;
+          for (int i = 0; i < C::kN / 4; ++i) {
+            const int c = h * (C::kN / 2) + 2 * i;
             float2 e = wm_fma2(make_float2(__uint_as_float(x[c >> 5][c & 31]), __uint_as_float(x[(c + 1) >> 5][(c + 1) & 31])), sc, nb);
             e.x = ex2(e.x);
             e.y = ex2(e.y);
             sum[i & 1] = wm_add2(sum[i & 1], e);
             p[i] = bf16x2(e.x, e.y);
           }
-          tmem_st32(s_t + h * 32, p);
+          if constexpr (C::kN == 128) tmem_st32(s_t + h * 32, p);
+          else tmem_st16(s_t + h * 16, p);
+          if (h == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar.p_half[w]);
+          }
         }
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         tmem_wait_st();
