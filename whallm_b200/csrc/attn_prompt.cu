@@ -75,12 +75,15 @@ struct Cfg {
   static constexpr bool kChain = D == 256;            // one tile, the warpgroups share its rows
   static constexpr int kTiles = kChain ? 1 : 2;       // 128-row tiles of a block
   static constexpr int kRows = 128 * kTiles;
-  static constexpr int kN = kChain ? 64 : 128;        // keys of a tile
+  static constexpr int kN = 128;                      // keys of a tile
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kSlot = kN * D * 2;            // one K or V tile
+  // K and V tiles come in pieces of one slot: at D = 256 two, half of the dimensions of K or half of the keys of V
+  static constexpr int kParts = kChain ? 2 : 1;
+  static constexpr int kSlot = kN * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kKDims = D / kParts, kVKeys = kN / kParts;
+  static constexpr int kKPanel = kN * 128, kVPanel = kVKeys * 128;   // 64 dimensions of a piece
   static constexpr int kOCol = 2 * kN;                // TMEM: two S / P buffers, then O
-  static constexpr int kPanel = kN * 128;             // 64 dimensions of a K or V tile
 };
 
 // One block of packed rows of one (sequence, key-value head).
@@ -206,12 +209,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       WM_U8(r, 0), WM_U8(r, 8), WM_U8(r, 16), WM_U8(r, 24)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      WM_U8(r, 0), WM_U8(r, 8)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -246,10 +243,8 @@ __device__ __forceinline__ void seq_bounds(const PromptArgs &a, int b, int &q0, 
   nk = max(min(a.cu_k[b + 1], a.Tk) - k0, 0);
 }
 
-// Load positions of key tile j and value tile j within an item of n tiles: the
-// order in which the MMA warp needs them.
-template <int D>
-__device__ __forceinline__ int pos_k(int j) { return Cfg<D>::kChain ? (j == 0 ? 0 : 2 * j - 1) : 2 * j; }
+// Position of value tile j among the 2 n tiles of an item, which come in the order
+// in which the MMA warp needs them.
 template <int D>
 __device__ __forceinline__ int pos_v(int j, int n) { return Cfg<D>::kChain ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; }
 
@@ -377,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
       // ------------------------------------------------- items and TMA loads
-      int64_t g = 0;                                  // loads so far
+      uint32_t g = 0u;                                // pieces loaded so far
       uint32_t edge_ph = 0u, edge_last = 0u;          // per slot: phase of v_edge, and whether the last load was an edge tile
       int it = 0;
       for (int64_t x = blockIdx.x;; ++it) {
@@ -391,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) ask_next(&sh);
         const int n = item->tiles, first = item->first;
         bool ok = true;
-        for (int p = 0; ok && p < 2 * n; ++p, ++g) {
+        for (int p = 0; ok && p < 2 * n; ++p) {
           bool is_v;
           int j;
           if constexpr (C::kChain) {
@@ -401,22 +396,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             is_v = p & 1;
             j = p >> 1;
           }
-          const int slot = static_cast<int>(g % C::kSlots);
-          ok = wait(&sh, &bar.kv_empty[slot], static_cast<uint32_t>((g / C::kSlots) & 1) ^ 1);
           const bool edge = is_v && j >= first;
-          if (ok && elect_one()) {
-            uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
-            mbar_expect_tx(full, C::kSlot);
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-              tma_load_3d(kv_s + slot * C::kSlot + d * C::kPanel, is_v ? &map_v : &map_k, d * 64, item->h, item->k0 + j * C::kN, full);
-            if (edge) mbar_arrive(&bar.kv_full[slot]);
-          }
-          if (ok) {
+          for (int part = 0; ok && part < C::kParts; ++part, ++g) {
+            const int slot = static_cast<int>(g % C::kSlots);
+            ok = wait(&sh, &bar.kv_empty[slot], ((g / C::kSlots) & 1u) ^ 1u);
+            if (!ok) break;
+            if (elect_one()) {
+              uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
+              const uint32_t dst = kv_s + slot * C::kSlot;
+              const int row = item->k0 + j * C::kN;
+              mbar_expect_tx(full, C::kSlot);
+              if (is_v) {
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * C::kVPanel, &map_v, d * 64, item->h, row + part * C::kVKeys, full);
+              } else {
+#pragma unroll
+                for (int d = 0; d < C::kKDims / 64; ++d)
+                  tma_load_3d(dst + d * C::kKPanel, &map_k, part * C::kKDims + d * 64, item->h, row, full);
+              }
+              if (edge) mbar_arrive(&bar.kv_full[slot]);
+            }
             edge_ph ^= edge ? 1u << slot : 0u;
             edge_last = edge ? edge_last | (1u << slot) : edge_last & ~(1u << slot);
+            __syncwarp();
           }
-          __syncwarp();
         }
         if (!ok || !wait(&sh, &bar.next_full, it & 1)) break;
         x = read_next(&sh);
@@ -424,11 +428,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // loads in flight when the others gave up must land before the CTA leaves
       if (*reinterpret_cast<volatile int *>(&sh.abort))
-        for (int64_t i = g > C::kSlots ? g - C::kSlots : 0; i < g; ++i) {
+        for (uint32_t i = g > C::kSlots ? g - C::kSlots : 0u; i < g; ++i) {
           const int slot = static_cast<int>(i % C::kSlots);
           const bool edge = (edge_last >> slot) & 1u;
           uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
-          const uint32_t ph = edge ? ((edge_ph >> slot) & 1u) ^ 1u : static_cast<uint32_t>((i / C::kSlots) & 1);
+          const uint32_t ph = edge ? ((edge_ph >> slot) & 1u) ^ 1u : (i / C::kSlots) & 1u;
           for (int tries = 0; tries < 1000 && !wm_tc::mbar_try(full, ph); ++tries) {}
         }
     } else if (warp == 9) {
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      Ring base{0, 0u};                               // load position of this item's first key tile
+      Ring base{0, 0u};                               // slot of this item's first piece
       uint32_t fixed = 0u, pph = 0u;                  // phase bits: v_fixed per slot, P per buffer
       const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
       bool ok = true;
@@ -464,26 +468,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
         if (!valid) break;
         const int steps = n * C::kTiles;
-        // key tiles at load positions 0, 2, 4, ... and value tiles at 1, 3, ...; at D = 256 0, 1, 3, 5, ... and
+        // key tiles come at positions 0, 2, 4, ... and value tiles at 1, 3, ...; at D = 256 at 0, 1, 3, 5, ... and
         // 2, 4, ..., 2 n - 2, 2 n - 1
         Ring rk = base, rv = base;
-        rv.next(C::kChain && n > 1 ? 2 : 1);
+        rv.next(C::kChain && n > 1 ? 2 * C::kParts : C::kParts);
         auto issue_s = [&](int s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1;
           if (j == 0 && !wait(&sh, &bar.q_full[w], it & 1)) return false;
-          if (!wait(&sh, &bar.kv_full[rk.slot], rk.ph)) return false;
-          tc_fence_after();
-          const uint32_t qa = desc_k(q_s + w * (128 * D * 2)), kb = desc_k(kv_s + rk.slot * C::kSlot), d = tm + (s & 1) * C::kN;
-          if (elect_one()) {
+          Ring at = rk;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss(d, qa + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * C::kPanel + (kk & 3) * 32) >> 4), id_s, kk != 0);
-            tc_commit(&bar.s_full[s & 1]);
-            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[rk.slot]);
-            if (s >= steps - C::kTiles) tc_commit(&bar.q_empty[w]);
+          for (int part = 0; part < C::kParts; ++part, at.next(1)) {
+            if (!wait(&sh, &bar.kv_full[at.slot], at.ph)) return false;
+            tc_fence_after();
+            const uint32_t qa = desc_k(q_s + w * (128 * D * 2) + part * (C::kKDims / 64) * 16384), kb = desc_k(kv_s + at.slot * C::kSlot);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < C::kKDims / 16; ++kk) {
+                const uint32_t step = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;       // both panels are 16 KB
+                mma_ss(tm + (s & 1) * C::kN, qa + step, kb + step, id_s, (part | kk) != 0);
+              }
+              if (C::kChain || w == 1) tc_commit(&bar.kv_empty[at.slot]);
+              if (part == C::kParts - 1) {
+                tc_commit(&bar.s_full[s & 1]);
+                if (s >= steps - C::kTiles) tc_commit(&bar.q_empty[w]);
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          if (C::kChain || w == 1) rk.next(C::kChain && j == 0 ? 1 : 2);
+          if (C::kChain || w == 1) rk.next(C::kChain && j == 0 ? C::kParts : 2 * C::kParts);
           return true;
         };
         if (steps == 0)                               // nothing to read Q for
@@ -495,46 +507,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && it > 0) ok = wait(&sh, &bar.o_free, (it - 1) & 1);  // the last item's O has been read
         for (int s = 0; ok && s < steps; ++s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1, buf = s & 1;
-          ok = wait(&sh, &bar.kv_full[rv.slot], rv.ph);
-          if (ok && j >= first && w == 0) {
-            ok = wait(&sh, &bar.v_fixed[rv.slot], (fixed >> rv.slot) & 1u);
-            fixed ^= 1u << rv.slot;
-          }
           // the keys of P's first half are multiplied while the softmax still works on the second
-          constexpr int kHalf = C::kN / 32;
-          const uint32_t vb = desc_mn(kv_s + rv.slot * C::kSlot, C::kPanel), o = tm + C::kOCol + w * D, p = tm + buf * C::kN;
-          ok = ok && wait(&sh, &bar.p_half[buf], (pph >> buf) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
+          const uint32_t o = tm + C::kOCol + w * D, p = tm + buf * C::kN;
+          Ring at = rv;
 #pragma unroll
-            for (int kk = 0; kk < kHalf; ++kk) mma_ts(o, p + kk * 8, vb + kk * (2048 >> 4), id_o, (j | kk) != 0);
+          for (int half = 0; half < 2; ++half) {
+            if (half == 0 || C::kParts == 2) {
+              if (half == 1) at.next(1);
+              ok = ok && wait(&sh, &bar.kv_full[at.slot], at.ph);
+              if (ok && j >= first && w == 0) {
+                ok = wait(&sh, &bar.v_fixed[at.slot], (fixed >> at.slot) & 1u);
+                fixed ^= 1u << at.slot;
+              }
+            }
+            ok = ok && wait(&sh, half ? &bar.p_ready[buf] : &bar.p_half[buf], (pph >> buf) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vb = desc_mn(kv_s + at.slot * C::kSlot, C::kVPanel);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < C::kN / 32; ++kk) {
+                const int kp = half * (C::kN / 32) + kk, kv = C::kParts == 2 ? kk : kp;
+                mma_ts(o, p + kp * 8, vb + kv * (2048 >> 4), id_o, (j | kp) != 0);
+              }
+              if (half == 1 && (C::kChain || s >= steps - 2)) tc_commit(&bar.o_done[buf]);
+              if (C::kChain || (half == 1 && w == 1)) tc_commit(&bar.kv_empty[at.slot]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          ok = wait(&sh, &bar.p_ready[buf], (pph >> buf) & 1u);
+          if (!ok) break;
           pph ^= 1u << buf;
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = kHalf; kk < 2 * kHalf; ++kk) mma_ts(o, p + kk * 8, vb + kk * (2048 >> 4), id_o, 1u);
-            if (C::kChain || s >= steps - 2) tc_commit(&bar.o_done[buf]);
-            if (C::kChain || w == 1) tc_commit(&bar.kv_empty[rv.slot]);
-          }
-          __syncwarp();
-          if (s == steps - 1) {                       // the last load of the item
-            base = rv;
+          if (s == steps - 1) {                       // the item's last piece
+            base = at;
             base.next(1);
           }
-          if (C::kChain || w == 1) rv.next(C::kChain && j == n - 2 ? 1 : 2);
+          if (C::kChain || w == 1) rv.next(C::kChain && j == n - 2 ? C::kParts : 2 * C::kParts);
           if (s + 2 < steps) ok = issue_s(s + 2);
         }
       }
     } else {
       // --------------------------------- query rows, and values of edge tiles
       const int ht = tid - 320;
-      int64_t g0 = 0;
-      uint32_t edge_ph = 0u;
+      uint32_t g0 = 0u, edge_ph = 0u;                 // pieces before this item, phases of v_edge
       bool ok = true;
       for (int it = 0; ok; ++it) {
         const int sl = it & 1;
@@ -577,22 +591,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           mbar_arrive(&bar.q_full[w]);
         }
-        for (int j = first; ok && j < n; ++j) {
-          const int64_t gg = g0 + pos_v<D>(j, n);
-          const int slot = static_cast<int>(gg % C::kSlots);
+        for (int y = first * C::kParts; ok && y < n * C::kParts; ++y) {
+          const int j = y / C::kParts, part = y % C::kParts;
+          const int slot = static_cast<int>((g0 + pos_v<D>(j, n) * C::kParts + part) % C::kSlots);
           ok = wait(&sh, &bar.v_edge[slot], (edge_ph >> slot) & 1u);
           if (!ok) break;
           edge_ph ^= 1u << slot;
-          uint8_t *vt = smem + C::kQBytes + slot * C::kSlot;
+          uint4 *vt = reinterpret_cast<uint4 *>(smem + C::kQBytes + slot * C::kSlot);
           const int live = nk - j * C::kN;
           for (int x = ht; x < C::kSlot / 16; x += kHelpers) {
-            const int r = (x >> 3) % C::kN;           // key of this 16-byte piece
-            uint4 *p = reinterpret_cast<uint4 *>(vt) + x;
+            const int r = part * C::kVKeys + (x >> 3) % C::kVKeys;    // key of this 16-byte piece
             if (r >= live) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
+              vt[x] = make_uint4(0u, 0u, 0u, 0u);
               continue;
             }
-            const uint4 v = *p;
+            const uint4 v = vt[x];
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
             bool odd = false;
 #pragma unroll
@@ -602,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               w[e] = (lo ? 0u : w[e] & 0xffffu) | (hi ? 0u : w[e] & 0xffff0000u);
             }
             if (odd) {
-              *p = make_uint4(w[0], w[1], w[2], w[3]);
+              vt[x] = make_uint4(w[0], w[1], w[2], w[3]);
               if (j - first < 4) atomicOr(&item->odd[(j - first) * 4 + (r >> 5)], 1u << (r & 31));
             }
           }
@@ -612,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bar.odd_ready[sl]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
-        g0 += 2 * n;
+        g0 += 2 * n * C::kParts;
       }
     }
   } else {
@@ -721,8 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum[i & 1] = wm_add2(sum[i & 1], e);
             p[i] = bf16x2(e.x, e.y);
           }
-          if constexpr (C::kN == 128) tmem_st32(s_t + h * 32, p);
-          else tmem_st16(s_t + h * 16, p);
+          tmem_st32(s_t + h * 32, p);
           if (h == 0) {
             tmem_wait_st();
             tc_fence_before();
@@ -852,7 +864,7 @@ int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t
   // without keys no tile is loaded; the maps then describe one row of q
   const bool any = a.Tk > 0;
   if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, 1, C::kN)) return rc;
-  if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, 1, C::kN)) return rc;
+  if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, 1, C::kVKeys)) return rc;
   // at most one partial block per sequence beyond the rows' own blocks
   const int64_t most = (static_cast<int64_t>(a.Tq) * a.G / C::kRows + a.B) * a.Hkv;
   WM_REQUIRE(most <= INT32_MAX, "prompt attention: too many rows");
