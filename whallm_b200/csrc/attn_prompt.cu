@@ -212,6 +212,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void store32(wm_bf16 *p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), WM_U8(r, 0) : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -808,16 +811,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
         }
-        uint4 *dst = reinterpret_cast<uint4 *>(a.out + head * D + c);
+        // whole 32-byte sectors: 16-byte stores to 32 rows at a time took twice as long
+        wm_bf16 *dst = a.out + head * D + c;
 #pragma unroll
-        for (int e = 0; live && e < 4; ++e) {
-          uint32_t y[4];
+        for (int e = 0; e < 2; ++e) {
+          uint32_t y[8];
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float lo = __uint_as_float(o[8 * e + 2 * z]), hi = __uint_as_float(o[8 * e + 2 * z + 1]);
+          for (int z = 0; z < 8; ++z) {
+            const float lo = __uint_as_float(o[16 * e + 2 * z]), hi = __uint_as_float(o[16 * e + 2 * z + 1]);
             y[z] = see > 0 ? bf16x2(lo * inv, hi * inv) : 0u;
           }
-          dst[e] = make_uint4(y[0], y[1], y[2], y[3]);
+          if (live) store32(dst + 16 * e, y);
         }
         __syncwarp();                                 // the TMEM loads are whole-warp instructions
       }
@@ -891,8 +895,8 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
   WM_REQUIRE(q && out && cu_seqlens_q && cu_seqlens_k && (Tk == 0 || (k && v)), "prompt attention: missing input or output");
   WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && k_stride >= static_cast<int64_t>(Hkv) * D &&
                  v_stride >= static_cast<int64_t>(Hkv) * D && q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 &&
-                 wm::aligned(q, 16) && wm::aligned(k, 16) && wm::aligned(v, 16) && wm::aligned(out, 16),
-             "prompt attention: token rows must be 16-byte aligned and hold their heads");
+                 wm::aligned(q, 16) && wm::aligned(k, 16) && wm::aligned(v, 16) && wm::aligned(out, 32),
+             "prompt attention: token rows must be 16-byte aligned and hold their heads, the output 32-byte aligned");
   WM_REQUIRE(static_cast<int64_t>(Tq) * (Hq / Hkv) <= INT32_MAX - 256, "prompt attention: too many rows per key-value head");
   const PromptArgs a{q, v, q_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, Hq / Hkv, causal,
                      128 % (Hq / Hkv) == 0, scale * kLog2e, out, lse};
