@@ -83,7 +83,7 @@ def test_evict_refusals():
     expect(f, evict_args(mo=ctypes.c_void_p(1 << 21)), "both in place")
     expect(f, evict_args(bytes=8), "workspace too small", L.WM_ERR_WORKSPACE)
     expect(f, evict_args(B=0), None, L.WM_OK)
-    assert L.lib().wkv_evict_workspace_size(2, 4, 32) == 2 * 4 * 2 * 32 * 12
+    assert L.lib().wkv_evict_workspace_size(2, 4, 32) == 2 * 4 * (2 * 32 * 12 + 4)
     assert L.lib().wkv_evict_workspace_size(0, 4, 32) == 0
 
 

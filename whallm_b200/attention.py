@@ -162,7 +162,7 @@ def paged_evict(k_cache, v_cache, page_table, lengths, mass, positions, seen, bu
     if budget <= 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError("the budget must be positive and hold the recent and the first positions")
     budget = min(budget, 2**31 - 1)
-    ws = mass.new_empty((6 * B * heads * max(1, min(budget, cap)),))
+    ws = mass.new_empty((B * heads * (6 * max(1, min(budget, cap)) + 1),))
     _call("wkv_paged_evict", dev, B, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width,
           _at("lengths", lengths, _INT, (B,), dev), _at("seen", seen, _INT, (B,), dev), _at("mass", mass, _F32, shape, dev),
           _at("positions", positions, _INT, shape, dev), budget, recent, sinks, _at("new mass", new_mass, _F32, shape, dev),

@@ -76,21 +76,28 @@ __global__ void __launch_bounds__(256) k_paged_append(const wm_bf16 *__restrict_
 
 // ------------------------------------------------------------------- evict --
 //
-// One cluster of CTAs per (sequence, head).  Every entry gets a 32-bit key
-// whose unsigned order is (protected, weight); the budget-th largest key is
-// found by a radix select of three digits (11, 11 and 10 bits), its ties go to
-// the lowest entries, and the r-th kept entry behind the budget moves into the
-// r-th hole before it.  Attention does not depend on the order of its keys, so
-// nothing that stays is copied, sources and destinations never overlap, and no
-// move waits for another.  The CTAs of a cluster hold a slice of the keys each
-// in shared memory and add their digit counts over distributed shared memory:
-// weights and positions are read from memory once.
-// Bound by the latency of its eight cluster-wide steps for short caches, by the
-// reads of weights and positions and by the moved rows for long ones.
+// One CTA, or for more than 4096 entries one cluster of CTAs, per (sequence,
+// head).  Every entry gets a 32-bit key whose unsigned order is (protected,
+// weight); the budget-th largest key is found by a radix select of four 8-bit
+// digits, its ties go to the lowest entries, and the r-th kept entry behind the
+// budget moves into the r-th hole before it.  Attention does not depend on the
+// order of its keys, so nothing that stays is copied, sources and destinations
+// never overlap, and no move waits for another.
+//
+// The CTAs of a cluster hold a slice of the keys each in shared memory and add
+// their digit counts over distributed shared memory: weights and positions are
+// read from memory once.  256 bins rather than 2048 (three passes) because every
+// CTA reads the bins of all: 8 x 8 KB took 6000 cycles a pass.  The first digit
+// of positive weights falls into a few bins, so lanes with equal digits add once.
+// A single CTA moves its rows itself; behind a cluster a second kernel does, over
+// the whole GPU.  Bound by the latency of the selection's steps (about 15
+// dependent phases) for short caches and by the moved rows for long ones.
 
 constexpr int kET = 512;           // threads
-constexpr int kBins = 2048;        // bins of a digit
+constexpr int kBins = 256;         // bins of a digit
 constexpr int kKeySmem = 40960;    // keys held per CTA (160 KB); longer slices read them again
+constexpr int kTableSmem = 2048;   // page numbers held per CTA
+constexpr int kMoveCtas = 4;       // CTAs per SM of the move kernel
 
 struct EvictArgs {
   Pool pool;
@@ -101,6 +108,7 @@ struct EvictArgs {
   int32_t *positions_out, *lengths_out;
   int64_t *rows;                   // [B * Hkv][2][budget]: cache rows of the holes, then of the tails
   int32_t *lists;                  // the same for the entries' numbers
+  int32_t *moves;                  // [B * Hkv]
   int budget, recent, sinks, row16_log2, scale_bytes, key_cap;
 };
 
@@ -145,187 +153,20 @@ __device__ __forceinline__ void move_scales(void *base, const int64_t *to, const
   }
 }
 
-__global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
-  extern __shared__ uint32_t sk[];                     // [key_cap] keys of this CTA's slice
-  __shared__ uint32_t hist[2][kBins];
-  __shared__ int warp_sums[kET / 32];
-  __shared__ int counts[4];                            // this CTA's ties, holes, tails
-  __shared__ int pick[2];                              // chosen digit, keys above it
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank()), C = static_cast<int>(cluster.num_blocks());
-  auto sync_all = [&] {
-    if (C > 1) cluster.sync();
-    else __syncthreads();
-  };
-  const int bh = static_cast<int>(blockIdx.x) / C, b = bh / a.pool.Hkv, h = bh - b * a.pool.Hkv;
-  const int tid = threadIdx.x;
-  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
-  const int len = a.lengths[b];
+// Thread ct of CT carries out the moves of one (sequence, head).
+__device__ __forceinline__ void carry_out(const EvictArgs &a, int64_t bh, int moves, int ct, int CT) {
   const int n = a.budget;
-  const int32_t *table = a.pool.table + static_cast<int64_t>(b) * a.pool.max_pages;
-  const float *mass = a.mass + bh * cap;
-  const int32_t *pos = a.positions + bh * cap;
-  float *mass_out = a.mass_out + bh * cap;
-  int32_t *pos_out = a.positions_out + bh * cap;
-
-  // a length or a page out of range leaves the sequence as it is
-  bool bad = len < 0 || len > cap;
-  if (!bad) {
-    const int np = (len + a.pool.page_size - 1) / a.pool.page_size;
-    for (int i = tid; i < np; i += kET) bad |= table[i] < 0 || table[i] >= a.pool.n_pages;
-  }
-  bad = __syncthreads_or(bad);
-  const int live = bad ? (len < 0 ? 0 : static_cast<int>(len < cap ? len : cap)) : len;
-  const bool copy = mass_out != mass;
-  if (bad || len <= n) {
-    if (copy)
-      for (int i = rank * kET + tid; i < live; i += C * kET) {
-        mass_out[i] = mass[i];
-        pos_out[i] = pos[i];
-      }
-    if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = len;
-    return;                                            // every CTA of the cluster returns here together
-  }
-  if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = n;
-
-  // this CTA's slice of the entries
-  const int S = ((len + C - 1) / C + 3) & ~3;
-  const int s0 = min(rank * S, len), s1 = min(s0 + S, len);
-  const int32_t from = a.seen[b] - a.recent;
-  const bool held = S <= a.key_cap;
-  auto key_at = [&](int i) { return held ? sk[i - s0] : evict_key(mass[i], pos[i], from, a.sinks); };
-  for (int i = tid; i < kBins; i += kET) hist[0][i] = 0u;
-  __syncthreads();
-  constexpr int kBatch = 4;                            // loads in flight per thread
-  for (int i0 = s0 + tid; i0 < s1; i0 += kBatch * kET) {
-    float m[kBatch];
-    int32_t p[kBatch];
-#pragma unroll
-    for (int x = 0; x < kBatch; ++x) {
-      const int i = i0 + x * kET;
-      m[x] = i < s1 ? mass[i] : 0.0f;
-      p[x] = i < s1 ? pos[i] : 0;
-    }
-#pragma unroll
-    for (int x = 0; x < kBatch; ++x) {
-      const int i = i0 + x * kET;
-      if (i >= s1) break;
-      const uint32_t key = evict_key(m[x], p[x], from, a.sinks);
-      if (held) sk[i - s0] = key;
-      if (copy && i < n) {                             // a hole's copy is replaced after the last barrier
-        mass_out[i] = m[x];
-        pos_out[i] = p[x];
-      }
-      atomicAdd(&hist[0][key >> 21], 1u);
-    }
-  }
-
-  // radix select of the n-th largest key
-  uint32_t prefix = 0u, mask = 0u;
-  int need = n;
-  const int shifts[3] = {21, 10, 0};
-#pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = shifts[pass];
-    uint32_t *hc = hist[pass & 1];
-    if (pass > 0) {
-      const uint32_t dm = pass == 1 ? 2047u : 1023u;
-      for (int i = s0 + tid; i < s1; i += kET) {
-        const uint32_t key = key_at(i);
-        if ((key & mask) == prefix) atomicAdd(&hc[(key >> shift) & dm], 1u);
-      }
-    }
-    uint32_t *hn = hist[(pass + 1) & 1];               // last read two barriers ago
-    sync_all();
-    if (pass < 2)
-      for (int i = tid; i < kBins; i += kET) hn[i] = 0u;
-    // thread t holds bins 2047 - 4t down to 2044 - 4t
-    const int at = kBins / 4 - 1 - tid;
-    uint4 sum = make_uint4(0u, 0u, 0u, 0u);
-    for (int r = 0; r < C; ++r) {
-      const uint4 x = reinterpret_cast<const uint4 *>(cluster.map_shared_rank(hc, r))[at];
-      sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-    }
-    const int c4[4] = {static_cast<int>(sum.w), static_cast<int>(sum.z), static_cast<int>(sum.y), static_cast<int>(sum.x)};
-    int total, before = block_scan(c4[0] + c4[1] + c4[2] + c4[3], warp_sums, &total);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (before < need && need <= before + c4[j]) {
-        pick[0] = 4 * at + 3 - j;
-        pick[1] = before;
-      }
-      before += c4[j];
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(pick[0]) << shift;
-    mask |= (pass == 2 ? 1023u : 2047u) << shift;
-    need -= pick[1];
-  }
-  // keys above prefix stay, and the first `need` entries whose key is prefix
-
-  // ranks: each thread walks a run of consecutive entries
-  const int E = (s1 - s0 + kET - 1) / kET;
-  const int r0 = min(s0 + tid * E, s1), r1 = min(r0 + E, s1);
-  int ties = 0;
-  for (int i = r0; i < r1; ++i) ties += key_at(i) == prefix;
-  int total_ties, tie0 = block_scan(ties, warp_sums, &total_ties);
-  if (tid == 0) counts[0] = total_ties;
-  sync_all();
-  for (int r = 0; r < rank; ++r) tie0 += *cluster.map_shared_rank(&counts[0], r);
-  int holes = 0, tails = 0, tr = tie0;
-  for (int i = r0; i < r1; ++i) {
-    const uint32_t key = key_at(i);
-    const bool keep = key > prefix || (key == prefix && tr++ < need);
-    holes += i < n && !keep;
-    tails += i >= n && keep;
-  }
-  int total_holes, total_tails;
-  int hole0 = block_scan(holes, warp_sums, &total_holes);
-  int tail0 = block_scan(tails, warp_sums, &total_tails);
-  if (tid == 0) {
-    counts[1] = total_holes;
-    counts[2] = total_tails;
-  }
-  sync_all();
-  int moves = 0;
-  for (int r = 0; r < C; ++r) {
-    const int x = *cluster.map_shared_rank(&counts[1], r);
-    const int y = *cluster.map_shared_rank(&counts[2], r);
-    if (r < rank) {
-      hole0 += x;
-      tail0 += y;
-    }
-    moves += x;
-  }
-  int32_t *hl = a.lists + static_cast<int64_t>(bh) * 2 * n, *tl = hl + n;
-  int64_t *hr = a.rows + static_cast<int64_t>(bh) * 2 * n, *tr_rows = hr + n;
-  auto row_of = [&](int e) {
-    const int pi = e / a.pool.page_size;
-    return (static_cast<int64_t>(table[pi]) * a.pool.Hkv + h) * a.pool.page_size + (e - pi * a.pool.page_size);
-  };
-  tr = tie0;
-  for (int i = r0; i < r1; ++i) {
-    const uint32_t key = key_at(i);
-    const bool keep = key > prefix || (key == prefix && tr++ < need);
-    if (i < n && !keep) {
-      hl[hole0] = i;
-      hr[hole0++] = row_of(i);
-    }
-    if (i >= n && keep) {
-      tl[tail0] = i;
-      tr_rows[tail0++] = row_of(i);
-    }
-  }
-  sync_all();                                          // also: no CTA leaves while its counts are read
-
-  const int ct = rank * kET + tid, CT = C * kET;
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  const int32_t *hl = a.lists + bh * 2 * n, *tl = hl + n;
+  const int64_t *to = a.rows + bh * 2 * n, *from = to + n;
   for (int r = ct; r < moves; r += CT) {
     const int d = hl[r], s = tl[r];
-    mass_out[d] = mass[s];
-    pos_out[d] = pos[s];
+    const float m = a.mass[bh * cap + s];
+    const int32_t p = a.positions[bh * cap + s];
+    a.mass_out[bh * cap + d] = m;
+    a.positions_out[bh * cap + d] = p;
   }
   // 16-byte pieces of the moved rows, the key rows' then the value rows'; several loads in flight per thread
-  // (one at a time, each behind its list entries and page lookups, took 45 of 67 us for 3500 moves a head)
   constexpr int kFly = 8;
   const int lg = a.row16_log2;
   const int64_t items = static_cast<int64_t>(moves) << (lg + 1);
@@ -339,8 +180,8 @@ __global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
       if (j < items) {
         const int r = static_cast<int>(j >> (lg + 1)), c = static_cast<int>(j) & ((2 << lg) - 1);
         uint4 *base = static_cast<uint4 *>(c >> lg ? a.pool.v : a.pool.k) + (c & ((1 << lg) - 1));
-        v[x] = base[tr_rows[r] << lg];
-        dst[x] = base + (hr[r] << lg);
+        v[x] = base[from[r] << lg];
+        dst[x] = base + (to[r] << lg);
       }
     }
 #pragma unroll
@@ -351,11 +192,196 @@ __global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
     for (int x = 0; x < 2; ++x) {
       void *base = x ? a.pool.vs : a.pool.ks;
       const int at = x ? CT - 1 - ct : ct;             // the two arrays begin at different threads
-      if (a.scale_bytes == 2) move_scales<uint16_t>(base, hr, tr_rows, moves, at, CT);
-      else if (a.scale_bytes == 4) move_scales<uint32_t>(base, hr, tr_rows, moves, at, CT);
-      else if (a.scale_bytes == 8) move_scales<uint2>(base, hr, tr_rows, moves, at, CT);
-      else move_scales<uint4>(base, hr, tr_rows, moves, at, CT);
+      if (a.scale_bytes == 2) move_scales<uint16_t>(base, to, from, moves, at, CT);
+      else if (a.scale_bytes == 4) move_scales<uint32_t>(base, to, from, moves, at, CT);
+      else if (a.scale_bytes == 8) move_scales<uint2>(base, to, from, moves, at, CT);
+      else move_scales<uint4>(base, to, from, moves, at, CT);
     }
+}
+
+__global__ void __launch_bounds__(256) k_paged_move(EvictArgs a) {
+  WM_PDL_WAIT();
+  const int moves = a.moves[blockIdx.x];
+  carry_out(a, blockIdx.x, moves, static_cast<int>(blockIdx.y * blockDim.x + threadIdx.x), static_cast<int>(gridDim.y * blockDim.x));
+}
+
+__global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
+  extern __shared__ uint32_t sk[];                     // [key_cap] keys of this CTA's slice
+  __shared__ uint32_t hist[2][kBins];
+  __shared__ int32_t stab[kTableSmem];
+  __shared__ int warp_sums[kET / 32];
+  __shared__ int counts[3];                            // this CTA's ties, holes, tails
+  __shared__ int pick[2];                              // chosen digit, keys above it
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), C = static_cast<int>(cluster.num_blocks());
+  auto sync_all = [&] {
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+  };
+  const int bh = static_cast<int>(blockIdx.x) / C, b = bh / a.pool.Hkv, h = bh - b * a.pool.Hkv;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  WM_PDL_LAUNCH();
+  const int len = a.lengths[b];
+  const int n = a.budget;
+  const int32_t *table = a.pool.table + static_cast<int64_t>(b) * a.pool.max_pages;
+  const float *mass = a.mass + bh * cap;
+  const int32_t *pos = a.positions + bh * cap;
+  float *mass_out = a.mass_out + bh * cap;
+  int32_t *pos_out = a.positions_out + bh * cap;
+
+  // a length or a page out of range leaves the sequence as it is
+  bool bad = len < 0 || len > cap;
+  const int np = bad ? 0 : (len + a.pool.page_size - 1) / a.pool.page_size;
+#pragma unroll 4
+  for (int i = tid; i < np; i += kET) {
+    const int p = table[i];
+    bad |= p < 0 || p >= a.pool.n_pages;
+    if (i < kTableSmem) stab[i] = p;
+  }
+  bad = __syncthreads_or(bad);
+  const int live = bad ? (len < 0 ? 0 : static_cast<int>(len < cap ? len : cap)) : len;
+  const bool copy = mass_out != mass;
+  if (bad || len <= n) {
+    if (copy)
+      for (int i = rank * kET + tid; i < live; i += C * kET) {
+        mass_out[i] = mass[i];
+        pos_out[i] = pos[i];
+      }
+    if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = len;
+    if (rank == 0 && tid == 0) a.moves[bh] = 0;
+    return;                                            // every CTA of the cluster returns here together
+  }
+  if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = n;
+
+  // this CTA's slice of the entries
+  const int S = ((len + C - 1) / C + 3) & ~3;
+  const int s0 = min(rank * S, len), s1 = min(s0 + S, len);
+  const int32_t from = a.seen[b] - a.recent;
+  const bool held = S <= a.key_cap;
+  auto key_at = [&](int i) { return held ? sk[i - s0] : evict_key(mass[i], pos[i], from, a.sinks); };
+  if (tid < kBins) hist[0][tid] = 0u;
+  __syncthreads();
+  constexpr int kBatch = 4;                            // loads in flight per thread
+  for (int i0 = s0; i0 < s1; i0 += kBatch * kET) {
+    float m[kBatch];
+    int32_t p[kBatch];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int i = i0 + x * kET + tid;
+      m[x] = i < s1 ? mass[i] : 0.0f;
+      p[x] = i < s1 ? pos[i] : 0;
+    }
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int i = i0 + x * kET + tid;
+      const uint32_t key = evict_key(m[x], p[x], from, a.sinks);
+      const unsigned in = __ballot_sync(0xffffffffu, i < s1);
+      if (i < s1) {
+        if (held) sk[i - s0] = key;
+        if (copy && i < n) {                           // a hole's copy is replaced after the last barrier
+          mass_out[i] = m[x];
+          pos_out[i] = p[x];
+        }
+        const unsigned same = __match_any_sync(in, key >> 24);
+        if (lane == __ffs(same) - 1) atomicAdd(&hist[0][key >> 24], static_cast<uint32_t>(__popc(same)));
+      }
+    }
+  }
+
+  // radix select of the n-th largest key
+  uint32_t prefix = 0u, mask = 0u;
+  int need = n;
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    uint32_t *hc = hist[pass & 1];
+    if (pass > 0)
+      for (int i = s0 + tid; i < s1; i += kET) {
+        const uint32_t key = key_at(i);
+        if ((key & mask) == prefix) atomicAdd(&hc[(key >> shift) & 255u], 1u);
+      }
+    sync_all();
+    if (pass < 3 && tid < kBins) hist[(pass + 1) & 1][tid] = 0u;     // last read two barriers ago
+    int count = 0;                                     // thread t < 256: bin 255 - t, over the cluster
+    if (tid < kBins) {
+#pragma unroll 8
+      for (int r = 0; r < C; ++r) count += static_cast<int>(cluster.map_shared_rank(hc, r)[kBins - 1 - tid]);
+    }
+    int total;
+    const int before = block_scan(count, warp_sums, &total);
+    if (before < need && need <= before + count) {
+      pick[0] = kBins - 1 - tid;
+      pick[1] = before;
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(pick[0]) << shift;
+    mask |= 255u << shift;
+    need -= pick[1];
+  }
+  // keys above prefix stay, and the first `need` entries whose key is prefix
+
+  // Sums of counts[which] over the CTAs before this one and over all, by every warp.
+  auto across = [&](int which, int &before, int &all) {
+    const int v = lane < C ? *cluster.map_shared_rank(&counts[which], lane) : 0;
+    int x = lane < rank ? v : 0, y = v;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      x += __shfl_xor_sync(0xffffffffu, x, d);
+      y += __shfl_xor_sync(0xffffffffu, y, d);
+    }
+    before = x;
+    all = y;
+  };
+  // ranks: each thread walks a run of consecutive entries
+  const int E = (s1 - s0 + kET - 1) / kET;
+  const int r0 = min(s0 + tid * E, s1), r1 = min(r0 + E, s1);
+  int ties = 0;
+  for (int i = r0; i < r1; ++i) ties += key_at(i) == prefix;
+  int total, before, all, tie0 = block_scan(ties, warp_sums, &total);
+  if (tid == 0) counts[0] = total;
+  sync_all();
+  across(0, before, all);
+  tie0 += before;
+  int holes = 0, tails = 0, tr = tie0;
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t key = key_at(i);
+    const bool keep = key > prefix || (key == prefix && tr++ < need);
+    holes += i < n && !keep;
+    tails += i >= n && keep;
+  }
+  int hole0 = block_scan(holes, warp_sums, &total);
+  if (tid == 0) counts[1] = total;
+  int tail0 = block_scan(tails, warp_sums, &total);
+  if (tid == 0) counts[2] = total;
+  sync_all();
+  int moves;
+  across(1, before, moves);
+  hole0 += before;
+  across(2, before, all);
+  tail0 += before;
+  int32_t *hl = a.lists + static_cast<int64_t>(bh) * 2 * n, *tl = hl + n;
+  int64_t *hole_rows = a.rows + static_cast<int64_t>(bh) * 2 * n, *tail_rows = hole_rows + n;
+  auto row_of = [&](int e) {
+    const int pi = e / a.pool.page_size;
+    return (static_cast<int64_t>(pi < kTableSmem ? stab[pi] : table[pi]) * a.pool.Hkv + h) * a.pool.page_size + (e - pi * a.pool.page_size);
+  };
+  tr = tie0;
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t key = key_at(i);
+    const bool keep = key > prefix || (key == prefix && tr++ < need);
+    if (i < n && !keep) {
+      hl[hole0] = i;
+      hole_rows[hole0++] = row_of(i);
+    }
+    if (i >= n && keep) {
+      tl[tail0] = i;
+      tail_rows[tail0++] = row_of(i);
+    }
+  }
+  if (rank == 0 && tid == 0) a.moves[bh] = moves;
+  sync_all();                                          // also: no CTA leaves while its counts are read
+  if (C == 1) carry_out(a, bh, moves, tid, kET);
 }
 
 }  // namespace
@@ -392,7 +418,7 @@ int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride, int64
 
 size_t wkv_evict_workspace_size(int B, int Hkv, int budget) {
   if (B <= 0 || Hkv <= 0 || budget <= 0) return 0;
-  return static_cast<size_t>(B) * Hkv * 2 * budget * (sizeof(int64_t) + sizeof(int32_t));
+  return static_cast<size_t>(B) * Hkv * (2 * static_cast<size_t>(budget) * (sizeof(int64_t) + sizeof(int32_t)) + sizeof(int32_t));
 }
 
 int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k_scales, void *v_scales, int fmt, int n_pages,
@@ -414,7 +440,7 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   WM_REQUIRE(workspace && wm::aligned(workspace, 8), "evict: the workspace must be 8-byte aligned");
   const int64_t heads = static_cast<int64_t>(B) * Hkv;
   // CTAs per (sequence, head): enough to fill the GPU, at least 2048 entries each, at most a portable cluster; up
-  // to 4096 entries one CTA, whose barriers are cheaper than a cluster's
+  // to 4096 entries one CTA, whose barriers are cheaper than a cluster's and which needs no second launch
   int C = 1;
   while (cap > 4096 && C < 8 && heads * C * 2 <= 2 * wm::sm_count() && cap > 2048 * C) C *= 2;
   const int64_t slice = ((cap + C - 1) / C + 3) & ~int64_t{3};
@@ -427,8 +453,8 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   int lg = 0;
   while ((16 << lg) < wm_paged::row_bytes(fmt, D)) ++lg;
   const EvictArgs args{pool, lengths, seen, mass, positions, mass_out, positions_out, lengths_out, rows,
-                       reinterpret_cast<int32_t *>(rows + heads * 2 * n), n, recent, sinks, lg,
-                       wm_paged::scale_bytes(fmt, D), key_cap};
+                       reinterpret_cast<int32_t *>(rows + heads * 2 * n), reinterpret_cast<int32_t *>(rows + heads * 3 * n), n,
+                       recent, sinks, lg, wm_paged::scale_bytes(fmt, D), key_cap};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(heads * C));
   cfg.blockDim = dim3(kET);
@@ -442,6 +468,10 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, k_paged_evict, args);
+  if (e == cudaSuccess && C > 1) {
+    const int64_t per = std::max<int64_t>(1, std::min<int64_t>(kMoveCtas * wm::sm_count() / heads, (static_cast<int64_t>(n) << (lg + 1)) / 256));
+    e = wm::launch_pdl(k_paged_move, dim3(static_cast<unsigned>(heads), static_cast<unsigned>(per)), dim3(256), 0, stream, args);
+  }
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wkv_paged_evict: ") + cudaGetErrorString(e));
   return wm::check_launch("wkv_paged_evict");
 }
