@@ -95,11 +95,15 @@ def test_decode_refusals():
         expect(f, decode_args(scale=s), "positive and finite")
     expect(f, decode_args(q=None), "missing input or output")
     expect(f, decode_args(qs=1000), "4-byte aligned")
-    expect(f, decode_args(bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, decode_args(width=1024, bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, decode_args(width=1024, ws=ODD), "256-byte aligned")
+    expect(f, decode_args(mass=P, bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
     expect(f, decode_args(B=0), None, L.WM_OK)
     size = L.lib().wattn_decode_workspace_size
     assert size(2, 6, 4, 128, L.WKV_BF16, 16, 4, 0) == 0 and size(2, 8, 4, 100, L.WKV_BF16, 16, 4, 0) == 0
-    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 1) - size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 0) == 2 * 4 * 64 * 2 * 4
+# one cluster per pair joins short caches without a workspace; collecting weights needs the scores
+    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 0) == 0 and size(2, 8, 4, 128, L.WKV_BF16, 16, 4, 1) > 2 * 4 * 64 * 2 * 4
+    assert size(2, 8, 4, 128, L.WKV_BF16, 16, 1024, 1) - size(2, 8, 4, 128, L.WKV_BF16, 16, 1024, 0) == 2 * 4 * 16384 * 2 * 4
 
 
 def test_prompt_refusals():

@@ -159,6 +159,20 @@ def test_decode_long(dev, n):
     run_decode(dev, [n], 8, 1, 128, 64, "fp8_f32_b64", seed=5, mass=True)
 
 
+@pytest.mark.parametrize("B", [1, 2, 9, 20, 40, 80, 160])
+def test_decode_short_caches(dev, B):
+    # clusters of 8, 4, 2 and 1 CTAs per (sequence, head), lengths from nothing to a few units per CTA
+    r = np.random.RandomState(B)
+    run_decode(dev, [int(x) for x in r.randint(0, 1025, B - 1)] + [0 if B == 1 else 1024], 4, 2, 64, 64, FMTS[B % 3], seed=B)
+
+
+@pytest.mark.parametrize("cap", [8192, 8256])
+@pytest.mark.parametrize("fmt,D,G", [("bf16", 128, 4), ("mxfp8", 256, 12)])
+def test_decode_at_the_cluster_limit(dev, cap, fmt, D, G):
+    # the longest capacity that one cluster joins, and the next page
+    run_decode(dev, [5, cap - 3], 2 * G, 2, D, 64, fmt, seed=cap)
+
+
 def test_decode_large_scores(dev):
     # scores of deviation ~60: nearly one-hot weights, running maxima that grow late
     run_decode(dev, [300, 5], 8, 2, 128, 16, "bf16", seed=6, scale=2.0, std=1.5)

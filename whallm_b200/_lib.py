@@ -125,11 +125,16 @@ def call(name: str, *args):
     everything else RuntimeError."""
     rc = getattr(lib(), name)(*args)
     if rc != WM_OK:
-        msg = f"{name}: {last_error()} (status {rc})"
-        if rc == WM_ERR_INVALID:
-            raise ValueError(msg)
-        raise NativeError(msg)
+        fail(name, rc)
     return rc
+
+
+def fail(name: str, rc: int):
+    """Raise for the status of a failed entry point."""
+    msg = f"{name}: {last_error()} (status {rc})"
+    if rc == WM_ERR_INVALID:
+        raise ValueError(msg)
+    raise NativeError(msg)
 
 
 def ptr(t):

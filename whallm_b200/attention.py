@@ -18,6 +18,7 @@ Every function runs on the current stream of its tensors' device.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -35,11 +36,17 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 
 def _call(name, dev, *args):
     """Call an entry point on device number ``dev`` and its current stream."""
-    if dev == torch.cuda.current_device():
-        L.call(name, *args, _raw_stream(dev))
-    else:
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            L.call(name, *args, _raw_stream(dev))
+            return _call(name, dev, *args)
+    rc = getattr(L.lib(), name)(*args, _raw_stream(dev))
+    if rc:
+        L.fail(name, rc)
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_bytes(*shape):
+    return L.lib().wattn_decode_workspace_size(*shape)
 
 
 def _at(name, t, dtype, shape, dev):
@@ -188,16 +195,15 @@ def decode_attention(q, k_cache, v_cache, page_table, lengths, fmt="bf16", k_sca
         raise ValueError("q must be [sequences, a multiple of the cache's heads, D]")
     scale = _scale(scale, d)
     _on(dev, q)
-    device = q.device
     if out is None:
-        out = torch.empty((B, Hq, d), dtype=_BF16, device=device)
-    lse = torch.empty((B, Hq), dtype=_F32, device=device) if return_lse else None
-    nbytes = L.lib().wattn_decode_workspace_size(B, Hq, heads, d, f, size, width, mass is not None)
-    ws = torch.empty((max(nbytes, 256),), dtype=_U8, device=device)
+        out = q.new_empty((B, Hq, d))
+    lse = q.new_empty((B, Hq), dtype=_F32) if return_lse else None
+    nbytes = _decode_bytes(B, Hq, heads, d, f, size, width, mass is not None)
+    ws = q.new_empty((nbytes,), dtype=_U8) if nbytes else None     # short caches need none
     _call("wattn_decode", dev, q.data_ptr(), qs, B, Hq, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width,
           _at("lengths", lengths, _INT, (B,), dev), scale, _at("out", out, _BF16, (B, Hq, d), dev),
-          lse.data_ptr() if return_lse else None, _at("mass", mass, _F32, (B, heads, width * size), dev), ws.data_ptr(),
-          nbytes)
+          lse.data_ptr() if return_lse else None, _at("mass", mass, _F32, (B, heads, width * size), dev),
+          ws.data_ptr() if nbytes else None, nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -223,11 +229,11 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     if B < 0:
         raise ValueError("cu_seqlens must be int32 [sequences + 1]")
     scale = _scale(scale, d)
-    dev, device = q.get_device(), q.device
+    dev = q.get_device()
     _on(dev, k, v)
     if out is None:
-        out = torch.empty((Tq, Hq, d), dtype=_BF16, device=device)
-    lse = torch.empty((Tq, Hq), dtype=_F32, device=device) if return_lse else None
+        out = q.new_empty((Tq, Hq, d))
+    lse = q.new_empty((Tq, Hq), dtype=_F32) if return_lse else None
     _call("wattn_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
           _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev), _at("cu_seqlens_k", cu_seqlens_k, _INT, (B + 1,), dev), B, Tq,
           Tk, Hq, Hkv, d, scale, 1 if causal else 0, _at("out", out, _BF16, (Tq, Hq, d), dev),

@@ -27,11 +27,14 @@
 // e4m3 rows are widened to bf16 exactly.  A key's block scales multiply its
 // partial scores, a value's block scales its weight before the rounding, so no
 // dequantized row is ever rounded.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "wm_paged.cuh"
 #include "wm_tc.cuh"
 
+namespace cg = cooperative_groups;
 using wm_paged::Pool;
 
 namespace {
@@ -39,6 +42,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTile = 16;               // keys of a warp's tile
 constexpr int kUnit = kWarps * kTile;   // keys of a unit of work
+constexpr int kMaxCluster = 8;
+constexpr int kClusterKeys = 1024;      // capacity per CTA up to which a cluster joins a pair
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -57,6 +62,7 @@ struct DecodeArgs {
   float *scores;                        // [pairs][capacity][score_heads], with mass only
   int score_heads;                      // a chunk's query heads, rounded up to 2
   int n_cta;                            // CTAs the line is split over
+  int cluster;                          // CTAs per pair, or 0 for the line
 };
 
 __device__ __forceinline__ int64_t units_of(const DecodeArgs &a, int b) {
@@ -143,59 +149,31 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
   return a ^ ((a >> 3) & 0x70u);
 }
 
-template <int D, int FMT, int NH>
+// Factor of a part with maximum m under the pair's maximum: a part without a
+// finite score keeps its sum (zero, or NaN).
+__device__ __forceinline__ float part_factor(float m, float top) { return m == kNegInf ? 1.0f : ex2(m - top); }
+
+// CL: a cluster of CTAs per pair instead of a share of the line (see launch()).
+template <int D, int FMT, int NH, bool CL>
 __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   using S = Shape<D, FMT, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
+  __shared__ float2 sm_part[S::kHeads];               // the CTA's maximum and sum
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i2 = (lane & 3) * 2;
   uint8_t *ring = smem + warp * (S::kStages * S::kStage);
   const uint32_t ring_u = wm_tc::smem_u32(ring);
   WM_PDL_WAIT();
   WM_PDL_LAUNCH();                                    // the join may be placed; it waits for this kernel's end
 
-  // this CTA's share [u, u_end) of the line of units
   const int PH = a.pool.Hkv * a.NC;
-  const int64_t total = warp_units(a, a.B) * PH;
-  const int64_t n_cta = parts_of(a, total);
-  if (blockIdx.x >= n_cta) return;
-  int64_t u = total * blockIdx.x / n_cta;
-  const int64_t u_end = total * (blockIdx.x + 1) / n_cta;
-  int b = 0;
-  int64_t base = 0;                                   // line position of sequence b
-  for (int b0 = 0;; b0 += 32) {                       // the sequence that holds unit u
-    const int64_t mine = b0 + lane < a.B ? units_of(a, b0 + lane) * PH : 0;
-    int64_t s = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += o;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + s > u);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      b = b0 + l;
-      base += __shfl_sync(0xffffffffu, s - mine, l);
-      break;
-    }
-    base += __shfl_sync(0xffffffffu, s, 31);
-  }
-
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
-  while (u < u_end) {
-    const int64_t nu = units_of(a, b);
-    if (nu == 0 || u >= base + nu * PH) {             // next sequence
-      base += nu * PH;
-      ++b;
-      continue;
-    }
-    const int hc = static_cast<int>((u - base) / nu);               // kv head and chunk of its query heads
-    const int64_t unit0 = (u - base) - hc * nu;
-    const int64_t unit1 = unit0 + (u_end - u) < nu ? unit0 + (u_end - u) : nu;
-    u += unit1 - unit0;
+
+  // units [unit0, unit1) of the pair (sequence b, hc = kv head and chunk of its query heads)
+  auto segment = [&](const int b, const int hc, const int64_t unit0, const int64_t unit1) {
     const int h = hc / a.NC, c = hc - h * a.NC;
     const int64_t pair = static_cast<int64_t>(b) * PH + hc;
-    const int len = static_cast<int>(a.lengths[b] < cap ? a.lengths[b] : cap);
+    const int len = static_cast<int>(a.lengths[b] < cap ? max(a.lengths[b], 0) : cap);
     const int32_t *table = a.pool.table + static_cast<int64_t>(b) * a.pool.max_pages;
 
     // tiles of this warp: 16 keys at (unit * 4 + warp) * 16
@@ -483,8 +461,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
         }
       }
     __syncthreads();
-    const int64_t slot = blockIdx.x + pair;
-    for (int x = threadIdx.x; x < S::kHeads * D / 4; x += kWarps * 32) {
+    auto merged = [&](int x) {                        // four values of the CTA's output
       const float4 *p = reinterpret_cast<const float4 *>(mg) + x;
       float4 r = p[0];
 #pragma unroll
@@ -492,18 +469,117 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
         const float4 y = p[w * (S::kHeads * D / 4)];
         r.x += y.x; r.y += y.y; r.z += y.z; r.w += y.w;
       }
-      reinterpret_cast<float4 *>(a.part_o + slot * (S::kHeads * D))[x] = r;
-    }
-    if (threadIdx.x < S::kHeads) {
-      const int hd = threadIdx.x;
-      const float top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
-      float sum = 0.0f;
+      return r;
+    };
+    auto stats = [&](int hd, float &top, float &sum) {
+      top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
+      sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) sum += sm_m[w][hd] == kNegInf ? sm_l[w][hd] : sm_l[w][hd] * ex2(sm_m[w][hd] - top);
-      a.part_m[slot * S::kHeads + hd] = top;
-      a.part_l[slot * S::kHeads + hd] = sum;
+    };
+    if constexpr (!CL) {
+      const int64_t slot = blockIdx.x + pair;
+      for (int x = threadIdx.x; x < S::kHeads * D / 4; x += kWarps * 32)
+        reinterpret_cast<float4 *>(a.part_o + slot * (S::kHeads * D))[x] = merged(x);
+      if (threadIdx.x < S::kHeads) {
+        float top, sum;
+        stats(threadIdx.x, top, sum);
+        a.part_m[slot * S::kHeads + threadIdx.x] = top;
+        a.part_l[slot * S::kHeads + threadIdx.x] = sum;
+      }
+      __syncthreads();
+    } else {
+      // join over distributed shared memory: the CTA's output replaces its warp 0's, every CTA of the cluster
+      // then adds up a share of the columns
+      cg::cluster_group cluster = cg::this_cluster();
+      const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+      for (int x = threadIdx.x; x < S::kHeads * D / 4; x += kWarps * 32) reinterpret_cast<float4 *>(mg)[x] = merged(x);
+      if (threadIdx.x < S::kHeads) {
+        float top, sum;
+        stats(threadIdx.x, top, sum);
+        sm_part[threadIdx.x] = make_float2(top, sum);
+      }
+      cluster.sync();
+      const int live = min(S::kHeads, a.G - c * S::kHeads);
+      const bool bad_len = a.lengths[b] < 0 || a.lengths[b] > cap;
+      const float nan = __uint_as_float(0x7fc00000u);
+      for (int x = rank * (kWarps * 32) + threadIdx.x; x < live * (D / 4); x += C * (kWarps * 32)) {
+        const int hd = x / (D / 4);
+        float top = kNegInf, sum = 0.0f;
+        float2 st[kMaxCluster];
+        float4 v[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < C) {
+            st[r] = cluster.map_shared_rank(sm_part, r)[hd];
+            v[r] = reinterpret_cast<const float4 *>(cluster.map_shared_rank(mg, r))[x];
+            top = fmaxf(top, st[r].x);
+          }
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < C) {
+            const float f = part_factor(st[r].x, top);
+            sum = fmaf(st[r].y, f, sum);
+            o.x = fmaf(v[r].x, f, o.x);
+            o.y = fmaf(v[r].y, f, o.y);
+            o.z = fmaf(v[r].z, f, o.z);
+            o.w = fmaf(v[r].w, f, o.w);
+          }
+        const int64_t head = static_cast<int64_t>(b) * a.Hq + h * a.G + c * S::kHeads + hd;
+        const float inv = bad_len ? nan : (len > 0 ? 1.0f / sum : 0.0f);
+        reinterpret_cast<uint2 *>(a.out + head * D)[x % (D / 4)] = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
+        if (a.lse && x % (D / 4) == 0) a.lse[head] = bad_len ? nan : (len > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
+      }
+      cluster.sync();                                 // no CTA leaves while its shared memory is read
     }
-    __syncthreads();
+  };
+
+  if constexpr (CL) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int64_t C = cluster.num_blocks(), rank = cluster.block_rank(), pair = blockIdx.x / C;
+    const int b = static_cast<int>(pair / PH);
+    const int64_t nu = units_of(a, b);
+    segment(b, static_cast<int>(pair - static_cast<int64_t>(b) * PH), nu * rank / C, nu * (rank + 1) / C);
+  } else {
+    // this CTA's share [u, u_end) of the line of units
+    const int64_t total = warp_units(a, a.B) * PH;
+    const int64_t n_cta = parts_of(a, total);
+    if (blockIdx.x >= n_cta) return;
+    int64_t u = total * blockIdx.x / n_cta;
+    const int64_t u_end = total * (blockIdx.x + 1) / n_cta;
+    int b = 0;
+    int64_t base = 0;                                 // line position of sequence b
+    for (int b0 = 0;; b0 += 32) {                     // the sequence that holds unit u
+      const int64_t mine = b0 + lane < a.B ? units_of(a, b0 + lane) * PH : 0;
+      int64_t s = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d) s += o;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, base + s > u);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = b0 + l;
+        base += __shfl_sync(0xffffffffu, s - mine, l);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, s, 31);
+    }
+    while (u < u_end) {
+      const int64_t nu = units_of(a, b);
+      if (nu == 0 || u >= base + nu * PH) {           // next sequence
+        base += nu * PH;
+        ++b;
+        continue;
+      }
+      const int hc = static_cast<int>((u - base) / nu);
+      const int64_t unit0 = (u - base) - hc * nu;
+      const int64_t unit1 = unit0 + (u_end - u) < nu ? unit0 + (u_end - u) : nu;
+      u += unit1 - unit0;
+      segment(b, hc, unit0, unit1);
+    }
   }
 }
 
@@ -514,10 +590,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
 // the parts one by one took 9.8 us for 37 parts of 128 values).
 constexpr int kJoin = 128;             // threads
 constexpr int kRun = 512;              // keys of a mass block
-
-// Factor of a part with maximum m under the pair's maximum: a part without a
-// finite score keeps its sum (zero, or NaN).
-__device__ __forceinline__ float part_factor(float m, float top) { return m == kNegInf ? 1.0f : ex2(m - top); }
 
 template <int D, int NH>
 __global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
@@ -689,9 +761,27 @@ int grid_of(int64_t most_units) {
 template <int D, int FMT, int NH>
 int launch(DecodeArgs &a, cudaStream_t stream) {
   using S = Shape<D, FMT, NH>;
-  cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH>>(S::kSmem);
-  if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
-  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
+  if (a.cluster) {
+    cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH, true>>(S::kSmem);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.n_cta));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(a.cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, k_attn_decode<D, FMT, NH, true>, a);
+    if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
+    return wm::check_launch("wattn_decode");
+  }
+  cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH, false>>(S::kSmem);
+  if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH, false>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
   const unsigned runs = a.mass ? static_cast<unsigned>((cap + kRun - 1) / kRun) : 0u;
   const int heads = std::min(S::kHeads, a.G);
@@ -729,7 +819,7 @@ struct Launch {
 };
 
 struct Plan {
-  int NC, heads, score_heads, n_cta;
+  int NC, heads, score_heads, n_cta, cluster;
   int64_t pairs, slots, cap;
   size_t off_m, off_l, off_s, bytes;
 };
@@ -742,6 +832,15 @@ Plan plan_of(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_page
   p.score_heads = std::min(p.heads, (G + 1) & ~1);
   p.pairs = static_cast<int64_t>(B) * Hkv * p.NC;
   p.cap = static_cast<int64_t>(max_pages) * page_size;
+  // Short caches: a cluster of CTAs per pair that joins over shared memory, in one launch and without a workspace.
+  // Its split is by pairs, not by the line, so it is taken while a CTA has at most kClusterKeys keys.
+  p.cluster = kMaxCluster;
+  while (p.cluster > 1 && p.pairs * p.cluster > 2 * wm::sm_count()) p.cluster /= 2;
+  if (with_mass || p.cap > static_cast<int64_t>(kClusterKeys) * p.cluster || p.pairs * p.cluster > INT32_MAX) p.cluster = 0;
+  if (p.cluster) {
+    p.n_cta = static_cast<int>(p.pairs * p.cluster);
+    return p;
+  }
   p.n_cta = dispatch(D, fmt, G, GridOf{p.pairs * ((p.cap + kUnit - 1) / kUnit)});
   p.slots = p.n_cta + p.pairs;
   auto up = [](size_t x) { return (x + 255) & ~size_t{255}; };
@@ -783,11 +882,11 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
   const Plan p = plan_of(B, Hq, Hkv, D, fmt, page_size, max_pages, mass != nullptr);
   WM_REQUIRE(p.pairs <= INT32_MAX && (p.cap + kRun - 1) / kRun <= 65000, "decode attention: batch or capacity too large");
   if (ws_bytes < p.bytes) return wm::fail(WM_ERR_WORKSPACE, "decode attention: workspace too small");
-  WM_REQUIRE(workspace && wm::aligned(workspace, 256), "decode attention: the workspace must be 256-byte aligned");
+  WM_REQUIRE(p.bytes == 0 || (workspace && wm::aligned(workspace, 256)), "decode attention: the workspace must be 256-byte aligned");
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   DecodeArgs a{pool, q, q_stride, lengths, B, Hq, Hq / Hkv, p.NC, scale * kLog2e, out, lse, mass,
                reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + p.off_m), reinterpret_cast<float *>(ws + p.off_l),
-               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.score_heads, p.n_cta};
+               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.score_heads, p.n_cta, p.cluster};
   return dispatch(D, fmt, a.G, Launch{a, stream});
 }
 
