@@ -24,14 +24,22 @@
 // 32-bit; P is rounded to bf16 once, the type of V, an error of at most 2^-8 of
 // each weight that the sum over keys averages out.
 //
-// e4m3 rows are widened to bf16 exactly.  A key's block scales multiply its
-// partial scores, a value's block scales its weight before the rounding, so no
-// dequantized row is ever rounded.
+// e4m3 rows are widened to f16, which holds every e4m3 value, in one instruction
+// per pair, and multiplied there (widening to bf16 takes four; at D = 256 that
+// arithmetic, not the memory, set the time).  The query goes to f16 with a power
+// of two per head that puts its largest magnitude into [2^14, 2^15): exact for
+// values within 2^-28 of it, off by less than 2^-39 of it below.  A key's block
+// scales multiply its partial scores.  A value's block scales multiply its weight
+// before the rounding, in units of the largest power of two seen among the warp's
+// scales (O is rescaled when that grows, as for the maximum) and times 2^15: the
+// weights are f16 values of at most 2^15, rounded to 11 bits down to 2^-29 of the
+// largest, and no dequantized row is ever rounded.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
 #include "wm_paged.cuh"
+#include "wm_stream.cuh"
 #include "wm_tc.cuh"
 
 namespace cg = cooperative_groups;
@@ -117,12 +125,37 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// two e4m3 codes (low half of w) -> two bf16, exact (4 significant bits, exponents -9 to 8)
-__device__ __forceinline__ uint32_t e4m3x2_bf16x2(uint32_t w) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(w)));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-  return bf16x2(f.x, f.y);
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Scales of one row as floats.
+template <int FMT, int N>
+__device__ __forceinline__ void load_scales(const uint8_t *p, float (&f)[N]) {
+  if constexpr (FMT == WKV_FP8_F32_B64) {
+    if constexpr (N == 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(p);
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else if constexpr (N == 2) {
+      const float2 v = *reinterpret_cast<const float2 *>(p);
+      f[0] = v.x; f[1] = v.y;
+    } else {
+      f[0] = *reinterpret_cast<const float *>(p);
+    }
+  } else if constexpr (FMT == WKV_MXFP8_B32) {
+    uint32_t w[(N + 3) / 4];
+    if constexpr (N == 8) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else if constexpr (N == 4) {
+      w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t *>(p);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = wm_e8m0((w[i >> 2] >> (8 * (i & 3))) & 255u);
+  }
 }
 
 template <int D, int FMT, int NH>
@@ -199,8 +232,33 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       }
     }
 
+    // scores in units of log2: factor of this thread's two heads
+    float sc2[NH][2];
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) {
+      sc2[nh][0] = sc2[nh][1] = a.scale2;
+      if constexpr (FMT != WKV_BF16) {
+        uint32_t top = 0u;                            // largest magnitude of head g, as bf16 bits
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) top = __vmaxu2(top, __vmaxu2(qf[nh][ks][0] & 0x7fff7fffu, qf[nh][ks][1] & 0x7fff7fffu));
+        top = max(top & 0xffffu, top >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(static_cast<int>(top >> 7) - 141, -100);
+        const float down = wm_stream::pow2f(-e), up = wm_stream::pow2f(e) * a.scale2;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qf[nh][ks][x] = wm_stream::f32x2_to_f16x2(wm_bf16lo(qf[nh][ks][x]) * down, wm_bf16hi(qf[nh][ks][x]) * down);
+        sc2[nh][0] = __shfl_sync(0xffffffffu, up, i2 * 4);
+        sc2[nh][1] = __shfl_sync(0xffffffffu, up, i2 * 4 + 4);
+      }
+    }
+
     float o[D / 16][NH][4];
     float m[NH][2], l[NH][2];
+    float unit = 0.0f, per_unit = 0.0f;               // e4m3: O is in units of `unit`; 2^15 / unit
 #pragma unroll
     for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -258,11 +316,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       __syncwarp();
       const uint32_t kt = ring_u + (i % S::kStages) * S::kStage, vt = kt + kTile * S::kRow;
       const uint8_t *sc = ring + (i % S::kStages) * S::kStage + 2 * kTile * S::kRow;
-      auto scale_of = [&](int which, int r, int blk) {
-        const uint8_t *p = sc + which * (kTile * S::kScale) + r * S::kScale;
-        if constexpr (FMT == WKV_FP8_F32_B64) return reinterpret_cast<const float *>(p)[blk];
-        else return wm_e8m0(p[blk]);
-      };
+      float ka[S::kBlocks], kb[S::kBlocks], va[S::kBlocks], vb[S::kBlocks];     // scales of keys and values g and g + 8
+      if constexpr (FMT != WKV_BF16) {
+        load_scales<FMT>(sc + g * S::kScale, ka);
+        load_scales<FMT>(sc + (g + 8) * S::kScale, kb);
+        load_scales<FMT>(sc + (kTile + g) * S::kScale, va);
+        load_scales<FMT>(sc + (kTile + g + 8) * S::kScale, vb);
+      }
 
       // scores: rows are keys (g, g + 8), columns heads (i2, i2 + 1)
       float s[NH][4];
@@ -297,19 +357,20 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
             // f[0], f[1]: rows g, g + 8 of piece ks; f[2], f[3]: of piece ks + 1
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const uint32_t w0 = f[2 * y], w1 = f[2 * y + 1];
-              const uint32_t fa[4] = {e4m3x2_bf16x2(w0), e4m3x2_bf16x2(w1), e4m3x2_bf16x2(w0 >> 16), e4m3x2_bf16x2(w1 >> 16)};
+              uint32_t h0[2], h1[2];
+              wm_stream::e4m3x4_to_f16x2(f[2 * y], h0);
+              wm_stream::e4m3x4_to_f16x2(f[2 * y + 1], h1);
+              const uint32_t fa[4] = {h0[0], h1[0], h0[1], h1[1]};
 #pragma unroll
-              for (int nh = 0; nh < NH; ++nh) mma(t[nh], fa, qf[nh][ks + y][0], qf[nh][ks + y][1]);
+              for (int nh = 0; nh < NH; ++nh) mma_f16(t[nh], fa, qf[nh][ks + y][0], qf[nh][ks + y][1]);
             }
           }
-          const float s0 = scale_of(0, g, blk), s1 = scale_of(0, g + 8, blk);
 #pragma unroll
           for (int nh = 0; nh < NH; ++nh) {
-            s[nh][0] = fmaf(t[nh][0], s0, s[nh][0]);
-            s[nh][1] = fmaf(t[nh][1], s0, s[nh][1]);
-            s[nh][2] = fmaf(t[nh][2], s1, s[nh][2]);
-            s[nh][3] = fmaf(t[nh][3], s1, s[nh][3]);
+            s[nh][0] = fmaf(t[nh][0], ka[blk], s[nh][0]);
+            s[nh][1] = fmaf(t[nh][1], ka[blk], s[nh][1]);
+            s[nh][2] = fmaf(t[nh][2], kb[blk], s[nh][2]);
+            s[nh][3] = fmaf(t[nh][3], kb[blk], s[nh][3]);
           }
         }
       }
@@ -317,10 +378,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       const int rows = min(kTile, len - key);
 #pragma unroll
       for (int nh = 0; nh < NH; ++nh) {
-        s[nh][0] = g < rows ? s[nh][0] * a.scale2 : kNegInf;
-        s[nh][1] = g < rows ? s[nh][1] * a.scale2 : kNegInf;
-        s[nh][2] = g + 8 < rows ? s[nh][2] * a.scale2 : kNegInf;
-        s[nh][3] = g + 8 < rows ? s[nh][3] * a.scale2 : kNegInf;
+        s[nh][0] = g < rows ? s[nh][0] * sc2[nh][0] : kNegInf;
+        s[nh][1] = g < rows ? s[nh][1] * sc2[nh][1] : kNegInf;
+        s[nh][2] = g + 8 < rows ? s[nh][2] * sc2[nh][0] : kNegInf;
+        s[nh][3] = g + 8 < rows ? s[nh][3] * sc2[nh][1] : kNegInf;
       }
       if (a.scores) {
         const int sh = a.score_heads;
@@ -389,16 +450,36 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
           for (int nh = 0; nh < NH; ++nh) mma(o[mt][nh], f, p[nh][0], p[nh][1]);
         }
       } else {
+        // the unit follows the largest scale of the warp's values
+        float big = 0.0f;
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk) big = fmaxf(big, fmaxf(va[blk], vb[blk]));
+        if (__any_sync(0xffffffffu, big > unit)) {
+          big = fmaxf(big, unit);
+#pragma unroll
+          for (int x = 16; x; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+          // the next power of two, within what has a reciprocal
+          const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 126, -100), 127);
+          const float u = wm_stream::pow2f(e), f = unit / u;
+          unit = u;
+          per_unit = 32768.0f / u;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[mt][nh][x] *= f;
+        }
         constexpr int per = D / 16 / S::kBlocks;
         const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
 #pragma unroll
         for (int blk = 0; blk < S::kBlocks; ++blk) {
-          const float s0 = scale_of(1, g, blk), s1 = scale_of(1, g + 8, blk);
+          const float s0 = va[blk] * per_unit, s1 = vb[blk] * per_unit;
           uint32_t p[NH][2];
 #pragma unroll
           for (int nh = 0; nh < NH; ++nh) {
-            p[nh][0] = transpose8(bf16x2(s[nh][0] * s0, s[nh][1] * s0));
-            p[nh][1] = transpose8(bf16x2(s[nh][2] * s1, s[nh][3] * s1));
+            p[nh][0] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][0] * s0, s[nh][1] * s0));
+            p[nh][1] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][2] * s1, s[nh][3] * s1));
           }
 #pragma unroll
           for (int x = 0; x < per; x += 2) {
@@ -409,10 +490,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
             // dimensions 2g, 2g + 1 of two keys: row g of the tile is dimension 2g, row g + 8 is 2g + 1
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const uint32_t w0 = __byte_perm(f[y], 0u, 0x3120), w1 = __byte_perm(f[y + 2], 0u, 0x3120);
-              const uint32_t fa[4] = {e4m3x2_bf16x2(w0), e4m3x2_bf16x2(w0 >> 16), e4m3x2_bf16x2(w1), e4m3x2_bf16x2(w1 >> 16)};
+              uint32_t h0[2], h1[2];
+              wm_stream::e4m3x4_to_f16x2(__byte_perm(f[y], 0u, 0x3120), h0);
+              wm_stream::e4m3x4_to_f16x2(__byte_perm(f[y + 2], 0u, 0x3120), h1);
+              const uint32_t fa[4] = {h0[0], h0[1], h1[0], h1[1]};
 #pragma unroll
-              for (int nh = 0; nh < NH; ++nh) mma(o[mt + y][nh], fa, p[nh][0], p[nh][1]);
+              for (int nh = 0; nh < NH; ++nh) mma_f16(o[mt + y][nh], fa, p[nh][0], p[nh][1]);
             }
           }
         }
@@ -451,7 +534,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       for (int j = 0; j < 2; ++j) {
         const int hd = nh * 8 + i2 + j;
         const float top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
-        const float f = m[nh][j] == kNegInf ? (n > 0 ? 1.0f : 0.0f) : ex2(m[nh][j] - top);
+        float f = m[nh][j] == kNegInf ? (n > 0 ? 1.0f : 0.0f) : ex2(m[nh][j] - top);
+        if constexpr (FMT != WKV_BF16) f *= unit * 0x1p-15f;
         float *row = mg + (warp * S::kHeads + hd) * D;
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) {
