@@ -73,6 +73,13 @@ struct DecodeArgs {
   int cluster;                          // CTAs per pair, or 0 for the line
 };
 
+// x / y for x >= 0, y > 0: 64-bit divisions are subroutines of about 0.4 us on the
+// critical path, and nearly every position on the line fits 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
+
 __device__ __forceinline__ int64_t units_of(const DecodeArgs &a, int b) {
   const int64_t len = a.lengths[b], cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
   return len <= 0 ? 0 : ((len < cap ? len : cap) + kUnit - 1) / kUnit;
@@ -95,6 +102,10 @@ __device__ __forceinline__ int64_t parts_of(const DecodeArgs &a, int64_t total) 
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -165,8 +176,12 @@ struct Shape {
   static constexpr int kScale = wm_paged::scale_bytes(FMT, D);    // bytes of a row's scales
   static constexpr int kBlocks = FMT == WKV_BF16 ? 1 : (FMT == WKV_FP8_F32_B64 ? D / 64 : D / 32);
   static constexpr int kStage = 2 * kTile * (kRow + kScale);      // keys, values and their scales
-  // at least 64 KB in flight per SM with two CTAs (one for 256 x bf16)
-  static constexpr int kStages = D == 64 && FMT != WKV_BF16 ? 4 : 3;
+#ifndef XST
+#define XST 3
+#define XCT 2
+#endif
+  static constexpr int kStages = D == 256 && FMT != WKV_BF16 ? XST : (D == 64 && FMT != WKV_BF16 ? 4 : 3);
+  static constexpr int kCtas = D == 256 && FMT != WKV_BF16 && NH==1 ? XCT : 1;   // per SM, for the register limit
   static constexpr int kHeads = 8 * NH;
   static constexpr int kMerge = kWarps * kHeads * D * 4;          // the warps' outputs when a part ends
   static constexpr int kRing = kWarps * kStages * kStage;
@@ -188,7 +203,7 @@ __device__ __forceinline__ float part_factor(float m, float top) { return m == k
 
 // CL: a cluster of CTAs per pair instead of a share of the line (see launch()).
 template <int D, int FMT, int NH, bool CL>
-__global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, (Shape<D, FMT, NH>::kCtas)) k_attn_decode(DecodeArgs a) {
   using S = Shape<D, FMT, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
@@ -271,29 +286,45 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       l[nh][0] = l[nh][1] = 0.0f;
     }
 
-    int pages = 0;                                    // lane i: page of tile (32 * block + i)
+    const uint32_t lane_swz = swz<S::kRow>(lane / S::kChunks, lane % S::kChunks);
+    int pages = 0, slots = 0;                         // lane i: page and slot of the first key of tile 32 * block + i
     auto issue = [&](int i) {
       if (i < n) {
         if ((i & 31) == 0) {
-          const int64_t key = (static_cast<int64_t>(t0) + static_cast<int64_t>(i + lane) * kWarps) * kTile;
-          pages = i + lane < n ? table[key / a.pool.page_size] : 0;
+          if (i + lane < n) {
+            const int first = (t0 + (i + lane) * kWarps) * kTile, pi = first / a.pool.page_size;
+            pages = table[pi];
+            slots = first - pi * a.pool.page_size;
+          }
         }
-        int page = __shfl_sync(0xffffffffu, pages, i & 31);
+        const int page = __shfl_sync(0xffffffffu, pages, i & 31), slot = __shfl_sync(0xffffffffu, slots, i & 31);
         const int key = (t0 + i * kWarps) * kTile;
         const int rows = min(kTile, len - key);
         const bool ok = page >= 0 && page < a.pool.n_pages;
         bad |= !ok;
-        const int64_t row = ok ? (static_cast<int64_t>(page) * a.pool.Hkv + h) * a.pool.page_size + key % a.pool.page_size : 0;
+        const int64_t row = ok ? (static_cast<int64_t>(page) * a.pool.Hkv + h) * a.pool.page_size + slot : 0;
         const uint32_t st = ring_u + (i % S::kStages) * S::kStage;
         const uint8_t *kp = static_cast<const uint8_t *>(a.pool.k) + row * S::kRow;
         const uint8_t *vp = static_cast<const uint8_t *>(a.pool.v) + row * S::kRow;
+        // a tile is one run of bytes; step x of the warp copies 512 of them, whose swizzle differs from step 0's by
+        // a constant
+        if (ok && rows == kTile) {
 #pragma unroll
-        for (int x = 0; x < kTile * S::kChunks / 32; ++x) {
-          const int r = (x * 32 + lane) / S::kChunks, cc = (x * 32 + lane) % S::kChunks;
-          const int take = ok && r < rows ? 16 : 0;
-          const int64_t off = take ? (r * S::kChunks + cc) * 16 : 0;
-          cp16(st + swz<S::kRow>(r, cc), kp + off, take);
-          cp16(st + kTile * S::kRow + swz<S::kRow>(r, cc), vp + off, take);
+          for (int x = 0; x < kTile * S::kChunks / 32; ++x) {
+            constexpr int kStep = S::kRow >= 128 ? 512 / S::kRow : 4;     // swizzle units of 512 bytes
+            const uint32_t dst = st + x * 512 + (lane_swz ^ (((x * kStep) & 7) << 4));
+            cp16(dst, kp + lane * 16 + x * 512);
+            cp16(dst + kTile * S::kRow, vp + lane * 16 + x * 512);
+          }
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < kTile * S::kChunks / 32; ++x) {
+            const int r = (x * 32 + lane) / S::kChunks, cc = (x * 32 + lane) % S::kChunks;
+            const int take = ok && r < rows ? 16 : 0;
+            const int64_t off = take ? (x * 32 + lane) * 16 : 0;
+            cp16(st + swz<S::kRow>(r, cc), kp + off, take);
+            cp16(st + kTile * S::kRow + swz<S::kRow>(r, cc), vp + off, take);
+          }
         }
         if constexpr (S::kScale > 0) {
           constexpr int per = kTile * S::kScale / 16; // 16-byte pieces of a tile's scales
@@ -621,17 +652,17 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
 
   if constexpr (CL) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int64_t C = cluster.num_blocks(), rank = cluster.block_rank(), pair = blockIdx.x / C;
-    const int b = static_cast<int>(pair / PH);
+    const int64_t C = cluster.num_blocks(), rank = cluster.block_rank(), pair = blockIdx.x / static_cast<unsigned>(C);
+    const int b = static_cast<int>(quotient(pair, PH));
     const int64_t nu = units_of(a, b);
-    segment(b, static_cast<int>(pair - static_cast<int64_t>(b) * PH), nu * rank / C, nu * (rank + 1) / C);
+    segment(b, static_cast<int>(pair - static_cast<int64_t>(b) * PH), quotient(nu * rank, C), quotient(nu * (rank + 1), C));
   } else {
     // this CTA's share [u, u_end) of the line of units
     const int64_t total = warp_units(a, a.B) * PH;
     const int64_t n_cta = parts_of(a, total);
     if (blockIdx.x >= n_cta) return;
-    int64_t u = total * blockIdx.x / n_cta;
-    const int64_t u_end = total * (blockIdx.x + 1) / n_cta;
+    int64_t u = quotient(total * blockIdx.x, n_cta);
+    const int64_t u_end = quotient(total * (blockIdx.x + 1), n_cta);
     int b = 0;
     int64_t base = 0;                                 // line position of sequence b
     for (int b0 = 0;; b0 += 32) {                     // the sequence that holds unit u
@@ -658,7 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
         ++b;
         continue;
       }
-      const int hc = static_cast<int>((u - base) / nu);
+      const int hc = static_cast<int>(quotient(u - base, nu));
       const int64_t unit0 = (u - base) - hc * nu;
       const int64_t unit1 = unit0 + (u_end - u) < nu ? unit0 + (u_end - u) : nu;
       u += unit1 - unit0;
@@ -667,28 +698,34 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   }
 }
 
-// Joins the parts of a pair.  Blocks (pair, head) give the output; with a mass
-// array blocks (pair, heads + x) add the weights of a run of keys.  A pair has up
-// to one part per CTA: their factors go to shared memory first, so that the loads
-// of the parts' outputs are independent of one another (a first form that walked
-// the parts one by one took 9.8 us for 37 parts of 128 values).
-constexpr int kJoin = 128;             // threads
-constexpr int kRun = 512;              // keys of a mass block
+// Joins the parts of a pair.  Blocks (pair, group of heads) give the output; with
+// a mass array blocks (pair, groups + x) add the weights of a run of keys.  A pair
+// has up to one part per CTA: their factors go to shared memory first, so that the
+// loads of the parts' outputs are independent of one another (a first form that
+// walked the parts one by one took 9.8 us for 37 parts of 128 values).  Two forms:
+// for few parts per pair 128 threads take kHpb heads, four values each; for many
+// 512 threads take one head and share the parts (74 parts of 8 x 256 values took
+// 8 us on 128 threads).
+constexpr int kManyParts = 8;          // parts per pair from which a block takes a single head
+constexpr int kKeysPerThread = 4;      // of a mass block
 
-template <int D, int NH>
-__global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
-  constexpr int kHeads = 8 * NH;
-  constexpr int kCols = D / 4, kGroups = kJoin / kCols;        // a thread sums 4 values over every kGroups-th part
-  __shared__ float s_f[kJoin], s_red[2][kJoin / 32];
-  __shared__ float4 s_o[kJoin];
-  __shared__ float2 s_st[kJoin];
+template <int D, int NH, int TJ, int HPB>
+__global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
+  constexpr int kHeads = 8 * NH, kJW = TJ / 32;
+  constexpr int kCols = HPB * D / 4, kGroups = TJ / kCols;     // a thread sums 4 values over every kGroups-th part
+  constexpr int kPer = TJ / HPB;                               // parts whose factors are held at once
+  static_assert(kGroups >= 1 && 32 % HPB == 0, "join shape");
+  __shared__ float s_f[TJ], s_top[kJW][HPB], s_sum[kJW][HPB];
+  __shared__ float4 s_o[TJ];
+  __shared__ float2 s_st[kJW][kHeads];
   __shared__ float s_lse2[kHeads];
   const int PH = a.pool.Hkv * a.NC;
   const int64_t pair = blockIdx.x;
-  const int b = static_cast<int>(pair / PH), hc = static_cast<int>(pair - static_cast<int64_t>(b) * PH);
+  const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(PH)), hc = static_cast<int>(pair - static_cast<int64_t>(b) * PH);
   const int h = hc / a.NC, c = hc - h * a.NC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (static_cast<int>(blockIdx.y) < heads ? c * kHeads + static_cast<int>(blockIdx.y) >= a.G : c != 0) return;
+  const bool output = static_cast<int>(blockIdx.y) < groups;
+  if (output ? c * kHeads + static_cast<int>(blockIdx.y) * HPB >= a.G : c != 0) return;
   WM_PDL_WAIT();
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
   int64_t total = 0, first = 0;                       // units of all sequences, and of those before b
@@ -710,31 +747,34 @@ __global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
   const float nan = __uint_as_float(0x7fc00000u);
   const int64_t n_cta = parts_of(a, total);
   // CTAs that hold the nu units from `at`
-  auto part0 = [&](int64_t at) { return nu ? ((at + 1) * n_cta - 1) / total : 0; };
-  auto parts = [&](int64_t at) { return nu ? static_cast<int>(((at + nu) * n_cta - 1) / total - part0(at)) + 1 : 0; };
+  auto part0 = [&](int64_t at) { return nu ? quotient((at + 1) * n_cta - 1, total) : 0; };
+  auto parts = [&](int64_t at, int64_t p0) { return nu ? static_cast<int>(quotient((at + nu) * n_cta - 1, total) - p0) + 1 : 0; };
 
-  if (static_cast<int>(blockIdx.y) < heads) {
-    const int hd = blockIdx.y, hg = c * kHeads + hd, np = parts(first);
-    const int64_t slot0 = part0(first) + pair;
-    const float *pm = a.part_m + slot0 * kHeads + hd, *pl = a.part_l + slot0 * kHeads + hd;
-    float m0 = kNegInf, l0 = 0.0f;                    // part `tid`
-    if (tid < np) {
-      m0 = pm[tid * kHeads];
-      l0 = pl[tid * kHeads];
+  if (output) {
+    const int64_t p00 = part0(first), slot0 = p00 + pair;
+    const int hd0 = blockIdx.y * HPB, np = parts(first, p00);
+    // thread t: head hd0 + t % HPB, part t / HPB
+    const int th = tid % HPB, tp = tid / HPB;
+    const float *pm = a.part_m + slot0 * kHeads + hd0 + th, *pl = a.part_l + slot0 * kHeads + hd0 + th;
+    float m0 = kNegInf, l0 = 0.0f;
+    if (tp < np) {
+      m0 = pm[tp * kHeads];
+      l0 = pl[tp * kHeads];
     }
     float top = m0;
-    for (int i = tid + kJoin; i < np; i += kJoin) top = fmaxf(top, pm[i * kHeads]);
+    for (int i = tp + kPer; i < np; i += kPer) top = fmaxf(top, pm[i * kHeads]);
 #pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    if (lane == 0) s_red[0][warp] = top;
+    for (int x = 16; x >= HPB; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if (lane < HPB) s_top[warp][lane] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+#pragma unroll
+    for (int w = 0; w < kJW; ++w) top = fmaxf(top, s_top[w][th]);
 
-    const int col = tid % kCols, grp = tid / kCols;
+    const int col = tid % kCols, grp = tid / kCols, ch = col / (D / 4);       // column: head ch, values 4 (col % (D / 4))
     float sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p0 = 0; p0 < np; p0 += kJoin) {
-      const int i = p0 + tid;
+    for (int p0 = 0; p0 < np; p0 += kPer) {
+      const int i = p0 + tp;
       float f = 0.0f;
       if (i < np) {
         f = part_factor(p0 ? pm[i * kHeads] : m0, top);
@@ -743,12 +783,12 @@ __global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
       if (p0) __syncthreads();
       s_f[tid] = f;
       __syncthreads();
-      const float4 *po = reinterpret_cast<const float4 *>(a.part_o + ((slot0 + p0) * kHeads + hd) * D) + col;
-      const int m = min(kJoin, np - p0);
+      const float4 *po = reinterpret_cast<const float4 *>(a.part_o + ((slot0 + p0) * kHeads + hd0) * D) + col;
+      const int m = min(kPer, np - p0);
 #pragma unroll 8
       for (int y = grp; y < m; y += kGroups) {
-        const float4 v = po[static_cast<int64_t>(y) * (kHeads * kCols)];
-        const float fy = s_f[y];
+        const float4 v = po[static_cast<int64_t>(y) * (kHeads * D / 4)];
+        const float fy = s_f[y * HPB + ch];
         o.x = fmaf(v.x, fy, o.x);
         o.y = fmaf(v.y, fy, o.y);
         o.z = fmaf(v.z, fy, o.z);
@@ -756,62 +796,75 @@ __global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
       }
     }
 #pragma unroll
-    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) s_red[1][warp] = sum;
-    s_o[tid] = o;
+    for (int x = 16; x >= HPB; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane < HPB) s_sum[warp][lane] = sum;
+    if constexpr (kGroups > 1) s_o[tid] = o;
     __syncthreads();
-    sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-    const int64_t head = static_cast<int64_t>(b) * a.Hq + h * a.G + hg;
-    if (tid < kCols) {
+    if (tid < kCols && c * kHeads + hd0 + ch < a.G) {
+      sum = 0.0f;
+      top = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kJW; ++w) {
+        sum += s_sum[w][ch];
+        top = fmaxf(top, s_top[w][ch]);
+      }
 #pragma unroll
       for (int y = 1; y < kGroups; ++y) {
         const float4 v = s_o[y * kCols + tid];
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
       }
+      const int64_t head = static_cast<int64_t>(b) * a.Hq + h * a.G + c * kHeads + hd0 + ch;
+      const int x = col % (D / 4);
       const float inv = bad ? nan : (np > 0 ? 1.0f / sum : 0.0f);
-      reinterpret_cast<uint2 *>(a.out + head * D)[tid] = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
+      reinterpret_cast<uint2 *>(a.out + head * D)[x] = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
+      if (a.lse && x == 0) a.lse[head] = bad ? nan : (np > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
     }
-    if (a.lse && tid == 0) a.lse[head] = bad ? nan : (np > 0 ? (top + log2f(sum)) * kLn2 : kNegInf);
     return;
   }
 
   // mass: the weights of keys [k0, k1), summed over the query heads of all chunks
-  const int64_t k0 = static_cast<int64_t>(blockIdx.y - heads) * kRun;
+  constexpr int kRun = TJ * kKeysPerThread;
+  const int64_t k0 = static_cast<int64_t>(blockIdx.y - groups) * kRun;
   if (bad || k0 >= len) return;
   const int64_t k1 = k0 + kRun < len ? k0 + kRun : len;
   float *mass = a.mass + (static_cast<int64_t>(b) * a.pool.Hkv + h) * cap;
-  float acc[kRun / kJoin];
+  float acc[kKeysPerThread];
 #pragma unroll
-  for (int x = 0; x < kRun / kJoin; ++x) acc[x] = 0.0f;
+  for (int x = 0; x < kKeysPerThread; ++x) acc[x] = 0.0f;
   for (int cc = 0; cc < a.NC; ++cc) {
-    const int64_t at = first + cc * nu, slot0 = part0(at) + pair + cc;
-    const int n = parts(at) * kHeads;
+    const int64_t at = first + cc * nu, p00 = part0(at), slot0 = p00 + pair + cc;
+    const int n = parts(at, p00) * kHeads;
     const float *qm = a.part_m + slot0 * kHeads, *ql = a.part_l + slot0 * kHeads;
-    // thread t joins every (kJoin / kHeads)-th part of head t % kHeads
+    // thread t joins every (TJ / kHeads)-th part of head t % kHeads
     float top = kNegInf, sum = 0.0f;
 #pragma unroll 4
-    for (int i = tid; i < n; i += kJoin) {
+    for (int i = tid; i < n; i += TJ) {
       const float mi = qm[i], li = ql[i], t = fmaxf(top, mi);
       sum = sum * part_factor(top, t) + li * part_factor(mi, t);
       top = t;
     }
-    s_st[tid] = make_float2(top, sum);
+#pragma unroll
+    for (int x = 16; x >= kHeads; x >>= 1) {
+      const float mi = __shfl_xor_sync(0xffffffffu, top, x), li = __shfl_xor_sync(0xffffffffu, sum, x), t = fmaxf(top, mi);
+      sum = sum * part_factor(top, t) + li * part_factor(mi, t);
+      top = t;
+    }
+    if (lane < kHeads) s_st[warp][lane] = make_float2(top, sum);
     __syncthreads();
     if (tid < kHeads) {
-      for (int y = tid + kHeads; y < kJoin; y += kHeads) {
-        const float2 v = s_st[y];
-        const float t = fmaxf(top, v.x);
-        sum = sum * part_factor(top, t) + v.y * part_factor(v.x, t);
-        top = t;
-      }
+#pragma unroll
+      for (int w = 0; w < kJW; ++w) top = fmaxf(top, s_st[w][tid].x);
+      sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kJW; ++w) sum += s_st[w][tid].y * part_factor(s_st[w][tid].x, top);
       s_lse2[tid] = top + log2f(sum);
     }
     __syncthreads();
     const int live = min(kHeads, a.G - cc * kHeads);
     const float *sc = a.scores + (pair + cc) * cap * a.score_heads;
 #pragma unroll
-    for (int x = 0; x < kRun / kJoin; ++x) {
-      const int64_t key = k0 + x * kJoin + tid;
+    for (int x = 0; x < kKeysPerThread; ++x) {
+      const int64_t key = k0 + x * TJ + tid;
       if (key < k1) {
         const float2 *sp = reinterpret_cast<const float2 *>(sc + key * a.score_heads);
 #pragma unroll
@@ -825,10 +878,19 @@ __global__ void __launch_bounds__(kJoin) k_attn_join(DecodeArgs a, int heads) {
     }
   }
 #pragma unroll
-  for (int x = 0; x < kRun / kJoin; ++x) {
-    const int64_t key = k0 + x * kJoin + tid;
+  for (int x = 0; x < kKeysPerThread; ++x) {
+    const int64_t key = k0 + x * TJ + tid;
     if (key < k1) mass[key] += acc[x];
   }
+}
+
+template <int D, int NH, int TJ, int HPB>
+cudaError_t launch_join(const DecodeArgs &a, cudaStream_t stream) {
+  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  const int groups = (std::min(8 * NH, a.G) + HPB - 1) / HPB;
+  const unsigned runs = a.mass ? static_cast<unsigned>((cap + TJ * kKeysPerThread - 1) / (TJ * kKeysPerThread)) : 0u;
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC), groups + runs);
+  return wm::launch_pdl(k_attn_join<D, NH, TJ, HPB>, grid, dim3(TJ), 0, stream, a, groups);
 }
 
 int chunk_heads(int G) { return G <= 8 ? 8 : 16; }
@@ -866,11 +928,9 @@ int launch(DecodeArgs &a, cudaStream_t stream) {
   }
   cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH, false>>(S::kSmem);
   if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH, false>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
-  const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
-  const unsigned runs = a.mass ? static_cast<unsigned>((cap + kRun - 1) / kRun) : 0u;
-  const int heads = std::min(S::kHeads, a.G);
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC), heads + runs);
-  e = wm::launch_pdl(k_attn_join<D, NH>, grid, dim3(kJoin), 0, stream, a, heads);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC;
+  e = a.n_cta >= kManyParts * pairs ? launch_join<D, NH, 512, 1>(a, stream) : launch_join<D, NH, 128, 512 / D>(a, stream);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   return wm::check_launch("wattn_decode");
 }
@@ -964,7 +1024,8 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
   WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && q_stride % 2 == 0 && wm::aligned(q, 4) && wm::aligned(out, 8),
              "decode attention: query rows must be 4-byte aligned and hold Hq * D values, the output 8-byte aligned");
   const Plan p = plan_of(B, Hq, Hkv, D, fmt, page_size, max_pages, mass != nullptr);
-  WM_REQUIRE(p.pairs <= INT32_MAX && (p.cap + kRun - 1) / kRun <= 65000, "decode attention: batch or capacity too large");
+  // the join's grid has a row per 512 entries of the capacity
+  WM_REQUIRE(p.pairs <= INT32_MAX && (mass == nullptr || p.cap <= 512ll * 65000), "decode attention: batch or capacity too large");
   if (ws_bytes < p.bytes) return wm::fail(WM_ERR_WORKSPACE, "decode attention: workspace too small");
   WM_REQUIRE(p.bytes == 0 || (workspace && wm::aligned(workspace, 256)), "decode attention: the workspace must be 256-byte aligned");
   uint8_t *ws = static_cast<uint8_t *>(workspace);
