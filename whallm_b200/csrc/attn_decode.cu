@@ -104,8 +104,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// cached rows pass through L2 once: evict-first, so that the scores and parts that the join reads stay there
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -176,12 +177,7 @@ struct Shape {
   static constexpr int kScale = wm_paged::scale_bytes(FMT, D);    // bytes of a row's scales
   static constexpr int kBlocks = FMT == WKV_BF16 ? 1 : (FMT == WKV_FP8_F32_B64 ? D / 64 : D / 32);
   static constexpr int kStage = 2 * kTile * (kRow + kScale);      // keys, values and their scales
-#ifndef XST
-#define XST 3
-#define XCT 2
-#endif
-  static constexpr int kStages = D == 256 && FMT != WKV_BF16 ? XST : (D == 64 && FMT != WKV_BF16 ? 4 : 3);
-  static constexpr int kCtas = D == 256 && FMT != WKV_BF16 && NH==1 ? XCT : 1;   // per SM, for the register limit
+  static constexpr int kStages = D == 64 && FMT != WKV_BF16 ? 4 : 3;
   static constexpr int kHeads = 8 * NH;
   static constexpr int kMerge = kWarps * kHeads * D * 4;          // the warps' outputs when a part ends
   static constexpr int kRing = kWarps * kStages * kStage;
@@ -203,7 +199,7 @@ __device__ __forceinline__ float part_factor(float m, float top) { return m == k
 
 // CL: a cluster of CTAs per pair instead of a share of the line (see launch()).
 template <int D, int FMT, int NH, bool CL>
-__global__ void __launch_bounds__(kWarps * 32, (Shape<D, FMT, NH>::kCtas)) k_attn_decode(DecodeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   using S = Shape<D, FMT, NH>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
@@ -211,6 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<D, FMT, NH>::kCtas)) k_att
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i2 = (lane & 3) * 2;
   uint8_t *ring = smem + warp * (S::kStages * S::kStage);
   const uint32_t ring_u = wm_tc::smem_u32(ring);
+  const uint64_t policy = wm_tc::l2_evict_first_policy();
   WM_PDL_WAIT();
   WM_PDL_LAUNCH();                                    // the join may be placed; it waits for this kernel's end
 
@@ -313,8 +310,8 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<D, FMT, NH>::kCtas)) k_att
           for (int x = 0; x < kTile * S::kChunks / 32; ++x) {
             constexpr int kStep = S::kRow >= 128 ? 512 / S::kRow : 4;     // swizzle units of 512 bytes
             const uint32_t dst = st + x * 512 + (lane_swz ^ (((x * kStep) & 7) << 4));
-            cp16(dst, kp + lane * 16 + x * 512);
-            cp16(dst + kTile * S::kRow, vp + lane * 16 + x * 512);
+            cp16(dst, kp + lane * 16 + x * 512, policy);
+            cp16(dst + kTile * S::kRow, vp + lane * 16 + x * 512, policy);
           }
         } else {
 #pragma unroll 1
@@ -753,6 +750,17 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
   if (output) {
     const int64_t p00 = part0(first), slot0 = p00 + pair;
     const int hd0 = blockIdx.y * HPB, np = parts(first, p00);
+    const int col = tid % kCols, grp = tid / kCols, ch = col / (D / 4);       // column: head ch, values 4 (col % (D / 4))
+    const float4 *po = reinterpret_cast<const float4 *>(a.part_o + (slot0 * kHeads + hd0) * D) + col;
+    constexpr int64_t kNext = kHeads * D / 4;                                  // from part to part
+    // the first parts' outputs load while their factors are found
+    constexpr int kAhead = 8;
+    float4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int y = grp + k * kGroups;
+      v[k] = y < np ? po[y * kNext] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     // thread t: head hd0 + t % HPB, part t / HPB
     const int th = tid % HPB, tp = tid / HPB;
     const float *pm = a.part_m + slot0 * kHeads + hd0 + th, *pl = a.part_l + slot0 * kHeads + hd0 + th;
@@ -770,11 +778,16 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
 #pragma unroll
     for (int w = 0; w < kJW; ++w) top = fmaxf(top, s_top[w][th]);
 
-    const int col = tid % kCols, grp = tid / kCols, ch = col / (D / 4);       // column: head ch, values 4 (col % (D / 4))
     float sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4 &x, float f) {
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    };
     for (int p0 = 0; p0 < np; p0 += kPer) {
-      const int i = p0 + tp;
+      const int i = p0 + tp, m = min(kPer, np - p0);
       float f = 0.0f;
       if (i < np) {
         f = part_factor(p0 ? pm[i * kHeads] : m0, top);
@@ -783,17 +796,14 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
       if (p0) __syncthreads();
       s_f[tid] = f;
       __syncthreads();
-      const float4 *po = reinterpret_cast<const float4 *>(a.part_o + ((slot0 + p0) * kHeads + hd0) * D) + col;
-      const int m = min(kPer, np - p0);
-#pragma unroll 8
-      for (int y = grp; y < m; y += kGroups) {
-        const float4 v = po[static_cast<int64_t>(y) * (kHeads * D / 4)];
-        const float fy = s_f[y * HPB + ch];
-        o.x = fmaf(v.x, fy, o.x);
-        o.y = fmaf(v.y, fy, o.y);
-        o.z = fmaf(v.z, fy, o.z);
-        o.w = fmaf(v.w, fy, o.w);
+      int y = grp;
+      if (p0 == 0) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k, y += kGroups)
+          if (y < m) add(v[k], s_f[y * HPB + ch]);
       }
+#pragma unroll 4
+      for (; y < m; y += kGroups) add(po[(p0 + y) * kNext], s_f[y * HPB + ch]);
     }
 #pragma unroll
     for (int x = 16; x >= HPB; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -830,11 +840,25 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
   float *mass = a.mass + (static_cast<int64_t>(b) * a.pool.Hkv + h) * cap;
   float acc[kKeysPerThread];
 #pragma unroll
-  for (int x = 0; x < kKeysPerThread; ++x) acc[x] = 0.0f;
+  for (int x = 0; x < kKeysPerThread; ++x) {
+    const int64_t key = k0 + x * TJ + tid;
+    acc[x] = key < k1 ? mass[key] : 0.0f;
+  }
   for (int cc = 0; cc < a.NC; ++cc) {
     const int64_t at = first + cc * nu, p00 = part0(at), slot0 = p00 + pair + cc;
     const int n = parts(at, p00) * kHeads;
     const float *qm = a.part_m + slot0 * kHeads, *ql = a.part_l + slot0 * kHeads;
+    // the scores load while the heads' normalisers are found
+    const int live = min(kHeads, a.G - cc * kHeads);
+    const float *sc = a.scores + (pair + cc) * cap * a.score_heads;
+    float2 v[kKeysPerThread][kHeads / 2];
+#pragma unroll
+    for (int x = 0; x < kKeysPerThread; ++x) {
+      const int64_t key = k0 + x * TJ + tid;
+      const float2 *sp = reinterpret_cast<const float2 *>(sc + key * a.score_heads);
+#pragma unroll
+      for (int y = 0; y < kHeads / 2; ++y) v[x][y] = key < k1 && 2 * y < live ? sp[y] : make_float2(0.0f, 0.0f);
+    }
     // thread t joins every (TJ / kHeads)-th part of head t % kHeads
     float top = kNegInf, sum = 0.0f;
 #pragma unroll 4
@@ -860,27 +884,22 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
       s_lse2[tid] = top + log2f(sum);
     }
     __syncthreads();
-    const int live = min(kHeads, a.G - cc * kHeads);
-    const float *sc = a.scores + (pair + cc) * cap * a.score_heads;
 #pragma unroll
     for (int x = 0; x < kKeysPerThread; ++x) {
-      const int64_t key = k0 + x * TJ + tid;
-      if (key < k1) {
-        const float2 *sp = reinterpret_cast<const float2 *>(sc + key * a.score_heads);
+      float w = 0.0f;
 #pragma unroll
-        for (int y = 0; y < kHeads / 2; ++y)
-          if (2 * y < live) {
-            const float2 v = sp[y];
-            acc[x] += ex2(v.x - s_lse2[2 * y]);
-            if (2 * y + 1 < live) acc[x] += ex2(v.y - s_lse2[2 * y + 1]);
-          }
+      for (int y = 0; y < kHeads / 2; ++y) {
+        if (2 * y < live) w += ex2(v[x][y].x - s_lse2[2 * y]);
+        if (2 * y + 1 < live) w += ex2(v[x][y].y - s_lse2[2 * y + 1]);
       }
+      acc[x] += w;
     }
+    __syncthreads();
   }
 #pragma unroll
   for (int x = 0; x < kKeysPerThread; ++x) {
     const int64_t key = k0 + x * TJ + tid;
-    if (key < k1) mass[key] += acc[x];
+    if (key < k1) mass[key] = acc[x];
   }
 }
 
@@ -930,7 +949,10 @@ int launch(DecodeArgs &a, cudaStream_t stream) {
   if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH, false>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   const int64_t pairs = static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC;
-  e = a.n_cta >= kManyParts * pairs ? launch_join<D, NH, 512, 1>(a, stream) : launch_join<D, NH, 128, 512 / D>(a, stream);
+  const bool many = a.n_cta >= kManyParts * pairs;
+  if (!many) e = launch_join<D, NH, 128, 512 / D>(a, stream);
+  else if (!a.mass) e = launch_join<D, NH, 512, 1>(a, stream);
+  else e = launch_join<D, NH, 128, 1>(a, stream);     // the mass blocks' registers: four 128-thread blocks per SM, one of 512
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   return wm::check_launch("wattn_decode");
 }
