@@ -412,6 +412,23 @@ def test_append_rows_are_the_formats_rows(dev, fmt, D):
             assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_append_a_long_prompt(dev, fmt):
+    # several pieces per thread, the last ones partly past the end
+    Hkv, D, page, n = 5, 128, 64, 4001
+    c = Cache(dev, [n], Hkv, D, page, fmt, seed=35)
+    k, v = (rnd(gen(36 + i, dev), n, Hkv, D, dev=dev) for i in range(2))
+    W.paged_append(k, v, torch.tensor([0, n], dtype=torch.int32, device=dev), c.k, c.v, c.table, c.lengths, fmt, c.ks, c.vs)
+    e = torch.arange(n, device=dev)
+    pg, sl = c.table[0][e // page].long(), e % page
+    for x, cache, scales in ((k, c.k, c.ks), (v, c.v, c.vs)):
+        if fmt == "bf16":
+            assert torch.equal(cache[pg, :, sl], x)
+        else:
+            p, s = W.kv_quantize(x, fmt)
+            assert torch.equal(cache[pg, :, sl], p) and torch.equal(scales[pg, :, sl], s)
+
+
 def test_append_skips_what_is_out_of_range(dev):
     c = Cache(dev, [20, 20, 20], 2, 64, 16, "bf16", seed=33)
     k = rnd(gen(34, dev), 3, 2, 64, dev=dev)

@@ -15,17 +15,22 @@ namespace {
 
 // ------------------------------------------------------------------ append --
 //
-// One thread moves 16 values (two 16-byte loads) of a token's key or value row
-// to its slot; a quantized row's scale blocks are 2 or 4 adjacent lanes, as in
-// k_kv_fp8_quantize.  A token finds its sequence by binary search in
-// cu_seqlens: a step of at most ~10 cached loads that hides under the row's own
-// loads.  HBM bound: 2 B read and 2 B (1 B + scale) written per value.
+// A warp takes kFly x 32 neighbouring pieces of 16 values (two 16-byte loads per
+// lane and piece, all issued first).  Its lanes then find, one token each, where
+// the tokens it touches go: binary search in cu_seqlens (held in shared memory),
+// length, page.  The pieces get their token's row by shuffle; a quantized row's
+// scale blocks are 2 or 4 adjacent lanes, as in k_kv_fp8_quantize.  Bound by HBM
+// for bf16 rows (2 B read, 2 B written per value) and by the quantizer's
+// arithmetic for e4m3 rows: with a search per piece it took 475 instructions per
+// 16 values, 59 % of the issue slots.
 
-template <int FMT>
-__global__ void __launch_bounds__(256) k_paged_append(const wm_bf16 *__restrict__ k, const wm_bf16 *__restrict__ v,
-                                                      int64_t k_stride, int64_t v_stride, int64_t n16, int per_tok,
-                                                      int per_row, const int32_t *__restrict__ cu, int B,
-                                                      const int32_t *__restrict__ lengths, Pool pool,
+constexpr int kSeqSmem = 512;          // sequences searched in shared memory
+
+template <int FMT, int kFly>
+__global__ void __launch_bounds__(256, 5) k_paged_append(const wm_bf16 *__restrict__ k, const wm_bf16 *__restrict__ v,
+                                                      int64_t k_stride, int64_t v_stride, unsigned n16, unsigned per_tok,
+                                                      unsigned tok_magic, int row_log2, const int32_t *__restrict__ cu, int T,
+                                                      int B, const int32_t *__restrict__ lengths, Pool pool,
                                                       float *__restrict__ mass, int32_t *__restrict__ positions,
                                                       const int32_t *__restrict__ seen) {
   const bool is_v = blockIdx.y != 0;
@@ -36,40 +41,73 @@ __global__ void __launch_bounds__(256) k_paged_append(const wm_bf16 *__restrict_
   const int lane = threadIdx.x & 31;
   constexpr int G = FMT == WKV_BF16 ? 1 : wm_kv::Fp8Fmt<FMT == WKV_BF16 ? WKV_MXFP8_B32 : FMT>::kG / 2;
   const unsigned gmask = ((1u << G) - 1u) << (lane & ~(G - 1));
-  // the G lanes of a scale block hold one row: they take every branch together
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n16; i += (int64_t)gridDim.x * blockDim.x) {
-    const int t = static_cast<int>(i / per_tok);
-    const int c = static_cast<int>(i - static_cast<int64_t>(t) * per_tok);
-    const int h = c / per_row, cr = c - h * per_row;
-    const uint4 *p = reinterpret_cast<const uint4 *>(src + t * stride) + 2 * c;
-    const uint4 u[2] = {__ldcs(p), __ldcs(p + 1)};
-    // the last b with cu[b] <= t
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
+  const int64_t cap = static_cast<int64_t>(pool.max_pages) * pool.page_size;
+  __shared__ int32_t s_cu[kSeqSmem + 1], s_len[kSeqSmem];
+  const bool held = B <= kSeqSmem;
+  if (held) {
+    for (int i = threadIdx.x; i <= B; i += 256) {
+      s_cu[i] = __ldg(cu + i);
+      if (i < B) s_len[i] = __ldg(lengths + i);
     }
-    const int b = lo, end = __ldg(cu + b + 1);
-    if (t < __ldg(cu + b) || t >= end) continue;       // behind the last sequence: not a token
-    const int64_t e = static_cast<int64_t>(__ldg(lengths + b)) - (end - t);
-    const int64_t cap = static_cast<int64_t>(pool.max_pages) * pool.page_size;
-    if (e < 0 || e >= cap) continue;
-    const int pi = static_cast<int>(e / pool.page_size), slot = static_cast<int>(e - static_cast<int64_t>(pi) * pool.page_size);
-    const int page = __ldg(pool.table + static_cast<int64_t>(b) * pool.max_pages + pi);
-    if (page < 0 || page >= pool.n_pages) continue;
-    const int64_t row = (static_cast<int64_t>(page) * pool.Hkv + h) * pool.page_size + slot;
-    const int64_t chunk = row * per_row + cr;
-    if constexpr (FMT == WKV_BF16) {
-      uint4 *d = reinterpret_cast<uint4 *>(cache) + 2 * chunk;
-      d[0] = u[0];
-      d[1] = u[1];
-    } else {
-      wm_kv::kv_fp8_quant<FMT, 16>(u, chunk, gmask, lane, cache, scales);
+    __syncthreads();
+  }
+  auto cu_at = [&](int i) { return held ? s_cu[i] : __ldg(cu + i); };
+  constexpr unsigned kSpan = 32u * kFly;
+  const unsigned warps = gridDim.x * 8u;
+  for (unsigned base = (blockIdx.x * 8u + (threadIdx.x >> 5)) * kSpan; base < n16; base += warps * kSpan) {
+    const unsigned t0 = base / per_tok, off = base - t0 * per_tok;
+    uint4 u[kFly][2];
+#pragma unroll
+    for (int x = 0; x < kFly; ++x) {
+      const unsigned y = off + x * 32u + lane, t = __umulhi(y, tok_magic), c = y - t * per_tok;
+      if (base + x * 32u + lane < n16) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(src + (t0 + t) * stride) + 2 * c;
+        u[x][0] = __ldcs(p);
+        u[x][1] = __ldcs(p + 1);
+      }
     }
-    if (!is_v && cr == 0) {
-      const int64_t at = (static_cast<int64_t>(b) * pool.Hkv + h) * cap + e;
-      if (mass) mass[at] = 0.0f;
-      if (positions) positions[at] = __ldg(seen + b) - (end - t);
+    // lane l: token t0 + l; its row for head 0, or -1
+    int64_t row0 = -1;
+    const int tok = static_cast<int>(t0) + lane;
+    if (tok < T && __umulhi(off + kSpan - 1u, tok_magic) >= static_cast<unsigned>(lane)) {
+      int lo = 0, hi = B;                              // the last b with cu[b] <= tok
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu_at(mid) <= tok) lo = mid; else hi = mid;
+      }
+      const int b = lo, end = cu_at(b + 1);
+      const int64_t e = static_cast<int64_t>(held ? s_len[b] : __ldg(lengths + b)) - (end - tok);
+      if (tok >= cu_at(b) && tok < end && e >= 0 && e < cap) {     // else behind the last sequence: not a token
+        const int pi = static_cast<int>(e) / pool.page_size, slot = static_cast<int>(e) - pi * pool.page_size;
+        const int page = __ldg(pool.table + static_cast<int64_t>(b) * pool.max_pages + pi);
+        if (page >= 0 && page < pool.n_pages) {
+          row0 = static_cast<int64_t>(page) * pool.Hkv * pool.page_size + slot;
+          // by the key warp that has the token's first piece
+          if (!is_v && (lane > 0 || off == 0) && (mass || positions)) {
+            const int position = positions ? __ldg(seen + b) - (end - tok) : 0;
+            for (int h = 0; h < pool.Hkv; ++h) {
+              const int64_t at = (static_cast<int64_t>(b) * pool.Hkv + h) * cap + e;
+              if (mass) mass[at] = 0.0f;
+              if (positions) positions[at] = position;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kFly; ++x) {
+      const unsigned y = off + x * 32u + lane, t = __umulhi(y, tok_magic), c = y - t * per_tok;
+      const int64_t row = __shfl_sync(0xffffffffu, row0, t);
+      if (base + x * 32u + lane >= n16 || row < 0) continue;       // the lanes of a scale block together
+      const unsigned h = c >> row_log2, cr = c - (h << row_log2);
+      const int64_t chunk = ((row + static_cast<int64_t>(h) * pool.page_size) << row_log2) + cr;
+      if constexpr (FMT == WKV_BF16) {
+        uint4 *d = reinterpret_cast<uint4 *>(cache) + 2 * chunk;
+        d[0] = u[x][0];
+        d[1] = u[x][1];
+      } else {
+        wm_kv::kv_fp8_quant<FMT, 16>(u[x], chunk, gmask, lane, cache, scales);
+      }
     }
   }
 }
@@ -402,13 +440,27 @@ int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride, int64
                  v_stride % 8 == 0 && wm::aligned(k, 16) && wm::aligned(v, 16),
              "paged append: token rows must be 16-byte aligned and hold Hkv * D values");
   WM_REQUIRE(!positions || seen, "paged append: positions need the sequences' token counts");
-  const int per_row = D / 16, per_tok = Hkv * per_row;
-  const int64_t n16 = static_cast<int64_t>(T) * per_tok;
-  const int64_t want = (n16 + 255) / 256;
+  const int row_log2 = D == 64 ? 2 : (D == 128 ? 3 : 4);           // pieces of a row
+  WM_REQUIRE(Hkv <= 4096, "paged append: at most 4096 heads");
+  const unsigned per_tok = static_cast<unsigned>(Hkv) << row_log2;
+  // x / per_tok = umulhi(x, magic) for x * per_tok < 2^32; the kernel divides numbers below per_tok + 128
+  const unsigned magic = static_cast<unsigned>((1ull << 32) / per_tok + 1);
+  const int64_t pieces = static_cast<int64_t>(T) * per_tok;
+  WM_REQUIRE(pieces <= INT32_MAX, "paged append: too many values in one call");
+  const unsigned n16 = static_cast<unsigned>(pieces);
+  // several pieces per lane once that leaves every SM with work; a small call spreads over the SMs instead
+  const bool many = pieces >= 2ll * 256 * wm::sm_count();
+  const int64_t want = (pieces + (many ? 511 : 255)) / (many ? 512 : 256);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, static_cast<int64_t>(wm::sm_count()) * 16)), 2);
-#define WM_APPEND(F)                                                                                                  \
-  k_paged_append<F><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, per_row, cu_seqlens, B, lengths, \
-                                              pool, mass, positions, seen)
+#define WM_APPEND(F)                                                                                                     \
+  do {                                                                                                                   \
+    if (many)                                                                                                            \
+      k_paged_append<F, 2><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, magic, row_log2, cu_seqlens, \
+                                                     T, B, lengths, pool, mass, positions, seen);                        \
+    else                                                                                                                 \
+      k_paged_append<F, 1><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, magic, row_log2, cu_seqlens, \
+                                                     T, B, lengths, pool, mass, positions, seen);                        \
+  } while (0)
   if (fmt == WKV_BF16) WM_APPEND(WKV_BF16);
   else if (fmt == WKV_FP8_F32_B64) WM_APPEND(WKV_FP8_F32_B64);
   else WM_APPEND(WKV_MXFP8_B32);
