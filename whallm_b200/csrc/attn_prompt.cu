@@ -359,6 +359,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     sh.abort = (smem_u32(smem) & 1023u) != 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 8 && lane == 0) {
+    for (const CUtensorMap *m : {&map_q, &map_k, &map_v})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+  }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -368,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   Bars &bar = sh.bar;
+  WM_PDL_WAIT();                                      // the set-up above overlaps the end of the kernel before
 
   if (sh.abort) {
   } else if (warp >= 8) {
@@ -875,7 +880,8 @@ int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t
   const int grid = static_cast<int>(std::max<int64_t>(most, 1));
   const cudaError_t e = wm::allow_smem<k_attn_prompt<D>>(smem_bytes<D>());
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
-  k_attn_prompt<D><<<grid, kThreads, smem_bytes<D>(), stream>>>(a, mq, mk, mv);
+  const cudaError_t l = wm::launch_pdl(k_attn_prompt<D>, dim3(grid), dim3(kThreads), smem_bytes<D>(), stream, a, mq, mk, mv);
+  if (l != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(l));
   return wm::check_launch("wattn_prompt");
 }
 

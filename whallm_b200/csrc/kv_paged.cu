@@ -44,6 +44,8 @@ __global__ void __launch_bounds__(256, 5) k_paged_append(const wm_bf16 *__restri
   const int64_t cap = static_cast<int64_t>(pool.max_pages) * pool.page_size;
   __shared__ int32_t s_cu[kSeqSmem + 1], s_len[kSeqSmem];
   const bool held = B <= kSeqSmem;
+  WM_PDL_WAIT();
+  WM_PDL_LAUNCH();
   if (held) {
     for (int i = threadIdx.x; i <= B; i += 256) {
       s_cu[i] = __ldg(cu + i);
@@ -259,6 +261,7 @@ __global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
   const int bh = static_cast<int>(blockIdx.x) / C, b = bh / a.pool.Hkv, h = bh - b * a.pool.Hkv;
   const int tid = threadIdx.x, lane = tid & 31;
   const int64_t cap = static_cast<int64_t>(a.pool.max_pages) * a.pool.page_size;
+  WM_PDL_WAIT();
   WM_PDL_LAUNCH();
   const int len = a.lengths[b];
   const int n = a.budget;
@@ -452,19 +455,15 @@ int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride, int64
   const bool many = pieces >= 2ll * 256 * wm::sm_count();
   const int64_t want = (pieces + (many ? 511 : 255)) / (many ? 512 : 256);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(want, static_cast<int64_t>(wm::sm_count()) * 16)), 2);
-#define WM_APPEND(F)                                                                                                     \
-  do {                                                                                                                   \
-    if (many)                                                                                                            \
-      k_paged_append<F, 2><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, magic, row_log2, cu_seqlens, \
-                                                     T, B, lengths, pool, mass, positions, seen);                        \
-    else                                                                                                                 \
-      k_paged_append<F, 1><<<grid, 256, 0, stream>>>(k, v, k_stride, v_stride, n16, per_tok, magic, row_log2, cu_seqlens, \
-                                                     T, B, lengths, pool, mass, positions, seen);                        \
-  } while (0)
+  cudaError_t err = cudaSuccess;
+#define WM_APPEND(F)                                                                                                    \
+  err = wm::launch_pdl(many ? k_paged_append<F, 2> : k_paged_append<F, 1>, grid, dim3(256), 0, stream, k, v, k_stride,  \
+                       v_stride, n16, per_tok, magic, row_log2, cu_seqlens, T, B, lengths, pool, mass, positions, seen)
   if (fmt == WKV_BF16) WM_APPEND(WKV_BF16);
   else if (fmt == WKV_FP8_F32_B64) WM_APPEND(WKV_FP8_F32_B64);
   else WM_APPEND(WKV_MXFP8_B32);
 #undef WM_APPEND
+  if (err != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wkv_paged_append: ") + cudaGetErrorString(err));
   return wm::check_launch("wkv_paged_append");
 }
 
@@ -512,13 +511,15 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   cfg.blockDim = dim3(kET);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(C);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(C);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = C > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, k_paged_evict, args);
   if (e == cudaSuccess && C > 1) {
     const int64_t per = std::max<int64_t>(1, std::min<int64_t>(kMoveCtas * wm::sm_count() / heads, (static_cast<int64_t>(n) << (lg + 1)) / 256));
