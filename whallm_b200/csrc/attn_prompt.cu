@@ -262,7 +262,7 @@ __device__ __forceinline__ void ask_next(Shared *sh) {
                : "memory");
 }
 // The block number taken over, or -1 if none was left.
-__device__ __forceinline__ int64_t read_next(Shared *sh) {
+__device__ __forceinline__ int read_next(Shared *sh) {
   uint32_t got, x = 0u;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
@@ -275,27 +275,26 @@ __device__ __forceinline__ int64_t read_next(Shared *sh) {
       : "r"(smem_u32(&sh->next))
       : "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next answer overwrites this one
-  return got ? static_cast<int64_t>(x) : -1;
+  return got ? static_cast<int>(x) : -1;
 }
 
 // Work item number x by one warp: blocks of all sequences from the last block of
 // the last sequence backwards (within a causal sequence the longest first), heads
 // innermost.
 template <int D>
-__device__ __forceinline__ void find_item(const PromptArgs &a, int64_t x, Item *out) {
+__device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out) {
   using C = Cfg<D>;
   const int lane = threadIdx.x & 31;
-  int64_t blk = x / a.Hkv;
-  const int h = static_cast<int>(x - blk * a.Hkv);
+  unsigned blk = static_cast<unsigned>(x) / static_cast<unsigned>(a.Hkv);
+  const int h = static_cast<int>(static_cast<unsigned>(x) - blk * static_cast<unsigned>(a.Hkv));
   for (int hi = x < 0 ? 0 : a.B; hi > 0; hi -= 32) {  // lane l: sequence hi - 1 - l
     const int b = hi - 1 - lane;
     int q0 = 0, nq = 0, k0 = 0, nk = 0;
     if (b >= 0) seq_bounds(a, b, q0, nq, k0, nk);
-    const int64_t mine = (static_cast<int64_t>(nq) * a.G + C::kRows - 1) / C::kRows;
-    int64_t s = mine;
+    unsigned s = (static_cast<unsigned>(nq) * static_cast<unsigned>(a.G) + (C::kRows - 1)) / C::kRows;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+      const unsigned o = __shfl_up_sync(0xffffffffu, s, d);
       if (lane >= d) s += o;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, s > blk);
@@ -303,7 +302,7 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int64_t x, Item *
       if (lane == __ffs(hit) - 1) {
         const int k = static_cast<int>(s - 1 - blk);  // block within the sequence, last first
         const int R0 = k * C::kRows;
-        const int R1 = static_cast<int>(min(static_cast<int64_t>(R0) + C::kRows, static_cast<int64_t>(nq) * a.G)) - 1;
+        const int R1 = min(R0 + C::kRows, nq * a.G) - 1;
         const int n0 = visible(a, nq, nk, R0), n1 = visible(a, nq, nk, R1);
         out->valid = 1;
         out->q0 = q0;
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t g = 0u;                                // pieces loaded so far
       uint32_t edge_ph = 0u, edge_last = 0u;          // per slot: phase of v_edge, and whether the last load was an edge tile
       int it = 0;
-      for (int64_t x = blockIdx.x;; ++it) {
+      for (int x = static_cast<int>(blockIdx.x);; ++it) {
         const int sl = it & 1;
         if (!wait(&sh, &bar.item_empty[sl], ((it >> 1) & 1) ^ 1)) break;
         Item *item = &sh.item[sl];
