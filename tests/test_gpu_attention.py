@@ -106,8 +106,8 @@ class Cache:
         return (self.k, self.v, self.table, self.lengths, self.fmt, self.ks, self.vs)
 
 
-def run_decode(dev, lens, Hq, Hkv, D, page, fmt, seed=0, mass=False, scale=None, std=1.0):
-    c = Cache(dev, lens, Hkv, D, page, fmt, seed, std=std)
+def run_decode(dev, lens, Hq, Hkv, D, page, fmt, seed=0, mass=False, scale=None, std=1.0, max_pages=None):
+    c = Cache(dev, lens, Hkv, D, page, fmt, seed, std=std, max_pages=max_pages)
     q = rnd(gen(seed + 1, dev), len(lens), Hq, D, std=2.0, dev=dev)
     m = torch.rand((len(lens), Hkv, c.width * page), generator=gen(seed + 2, dev), device=dev) if mass else None
     before = m.clone() if mass else None
@@ -130,6 +130,21 @@ RAGGED = [1, 0, 15, 16, 17, 63, 64, 65, 130, 997]
 @pytest.mark.parametrize("Hq,Hkv", [(8, 8), (32, 4), (16, 1)])
 def test_decode_vs_64_bits(dev, fmt, D, Hq, Hkv):
     run_decode(dev, RAGGED, Hq, Hkv, D, 64, fmt, seed=D + Hq)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv", [(6, 2), (16, 1)])
+def test_decode_long_capacity(dev, fmt, D, Hq, Hkv):
+    # a capacity that is split over the GPU whatever the lengths: few and many parts per pair
+    run_decode(dev, [9000, 0, 3, 64, 65, 2000], Hq, Hkv, D, 64, fmt, seed=D + Hq + 1)
+    run_decode(dev, [4100], Hq, Hkv, D, 128, fmt, seed=D + Hq + 2, max_pages=100)
+
+
+def test_decode_long_capacity_batch(dev):
+    r = np.random.RandomState(5)
+    run_decode(dev, [int(x) for x in r.randint(0, 900, 90)], 8, 4, 64, 64, "mxfp8", seed=6, max_pages=200)
+    run_decode(dev, [0, 0, 0], 8, 4, 64, 64, "bf16", seed=7, max_pages=200)
 
 
 @pytest.mark.parametrize("G", [1, 3, 5, 7, 9, 12, 17, 40])
@@ -219,9 +234,10 @@ def test_decode_bad_lengths_and_pages(dev):
     assert torch.equal(out[4], good[4]) and torch.isfinite(mass[4]).all()
 
 
-def test_decode_captured_follows_lengths(dev):
+@pytest.mark.parametrize("max_pages", [None, 300])
+def test_decode_captured_follows_lengths(dev, max_pages):
     """Two graphs, one pool: each follows the lengths and tables as they are at its replay."""
-    c = Cache(dev, [500, 60, 0], 2, 128, 32, "bf16", seed=15)
+    c = Cache(dev, [500, 60, 0], 2, 128, 32, "bf16", seed=15, max_pages=max_pages)
     q = rnd(gen(16, dev), 3, 8, 128, dev=dev)
     W.decode_attention(q, *c.args)
     graphs = []
@@ -240,16 +256,23 @@ def test_decode_captured_follows_lengths(dev):
             assert torch.equal(out, want)
 
 
-def test_decode_on_a_side_stream(dev):
-    c = Cache(dev, [300], 2, 64, 16, "bf16", seed=17)
-    q = rnd(gen(18, dev), 1, 4, 64, dev=dev)
-    want = W.decode_attention(q, *c.args)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        outs = [W.decode_attention(q, *c.args) for _ in range(20)]
-    torch.cuda.current_stream().wait_stream(side)
-    assert all(torch.equal(o, want) for o in outs)
+@pytest.mark.parametrize("max_pages", [None, 600])
+def test_decode_on_two_streams(dev, max_pages):
+    """Calls on two streams at once: each has its own workspace."""
+    cs = [Cache(dev, [300 + 50 * i, 17], 2, 64, 16, "bf16", seed=17 + i, max_pages=max_pages) for i in range(2)]
+    qs = [rnd(gen(18 + i, dev), 2, 4, 64, dev=dev) for i in range(2)]
+    want = [W.decode_attention(q, *c.args) for q, c in zip(qs, cs)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(30):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                outs[i].append(W.decode_attention(qs[i], *cs[i].args))
+    for s in sides:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
 
 
 # ------------------------------------------------------------------ prompts --
@@ -306,6 +329,43 @@ def test_prompt_full(dev, D):
 @pytest.mark.parametrize("D,n", [(64, 1500), (128, 1111), (256, 900)])
 def test_prompt_long(dev, D, n):
     run_prompt(dev, [n], [n], 2, 1, D, seed=24)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_many_sequences(dev, D):
+    # more sequences than a warp has lanes and more blocks than SMs, with and without keys
+    r = np.random.RandomState(D)
+    nq = [int(x) for x in r.randint(0, 40, 75)]
+    nk = [max(0, n + int(d)) for n, d in zip(nq, r.randint(-20, 60, 75))]
+    run_prompt(dev, nq, nk, 8, 4, D, seed=29)
+
+
+@pytest.mark.parametrize("D,Hkv", [(64, 8), (128, 8), (256, 4)])
+def test_prompt_blocks_handed_on(dev, D, Hkv):
+    # several blocks per SM, long and short ones in turn: the same rows as when each sequence is alone
+    n = [700, 3, 400, 1, 129, 900]
+    g = gen(30, dev)
+    q, k, v = (rnd(g, sum(n), h, D, dev=dev) for h in (2 * Hkv, Hkv, Hkv))
+    cu = torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=dev)
+    out = W.prompt_attention(q, k, v, cu)
+    at = 0
+    for x in n:
+        one = torch.tensor([0, x], dtype=torch.int32, device=dev)
+        assert torch.equal(W.prompt_attention(q[at:at + x], k[at:at + x], v[at:at + x], one), out[at:at + x])
+        at += x
+
+
+def test_prompt_malformed_sequence_bounds(dev):
+    """Bounds outside the tensors are cut to them; bounds that run backwards are empty sequences."""
+    g = gen(31, dev)
+    q, k, v = (rnd(g, 100, h, 64, dev=dev) for h in (4, 2, 2))
+    good = torch.tensor([0, 40, 100], dtype=torch.int32, device=dev)
+    want = W.prompt_attention(q, k, v, good)
+    cut = torch.tensor([-5, 40, 5000], dtype=torch.int32, device=dev)
+    assert torch.equal(W.prompt_attention(q, k, v, cut), want)
+    out = torch.full_like(q, 7.0)
+    W.prompt_attention(q, k, v, torch.tensor([0, 40, 20, 20], dtype=torch.int32, device=dev), out=out)
+    assert torch.equal(out[:40], want[:40]) and (out[40:] == 7.0).all()
 
 
 def test_prompt_large_scores(dev):

@@ -90,6 +90,8 @@ def _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt):
     if len(shape) != 4 or k_cache.dtype != dt or v_cache.dtype != dt or v_cache.shape != shape:
         raise ValueError(f"caches must be {dt} [n_pages, heads, page_size, D] of one shape")
     pages, heads, size, d = shape
+    if not heads:
+        raise ValueError("a paged cache needs heads")
     if page_table.dim() != 2 or page_table.dtype != _INT:
         raise ValueError("page_table must be int32 [sequences, max_pages]")
     tshape = page_table.shape

@@ -1040,7 +1040,7 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
             const_cast<void *>(v_scales), page_table, n_pages, page_size, max_pages, Hkv};
   if (int rc = wm_paged::check_pool(pool, B, D, fmt)) return rc;
   WM_REQUIRE(Hq > 0 && Hq % Hkv == 0, "decode attention: the query heads must be a multiple of the key-value heads");
-  WM_REQUIRE(scale > 0.0f && scale <= 3.4028234663852886e38f, "decode attention: the scale must be positive and finite");
+  WM_REQUIRE(scale > 0.0f && scale * kLog2e <= 3.4028234663852886e38f, "decode attention: the scale must be positive and finite");
   if (B == 0) return WM_OK;
   WM_REQUIRE(q && lengths && out, "decode attention: missing input or output");
   WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && q_stride % 2 == 0 && wm::aligned(q, 4) && wm::aligned(out, 8),

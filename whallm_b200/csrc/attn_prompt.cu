@@ -895,7 +895,7 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
   WM_REQUIRE(B >= 0 && Tq >= 0 && Tk >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0,
              "prompt attention: the query heads must be a multiple of the key-value heads");
   WM_REQUIRE(D == 64 || D == 128 || D == 256, "prompt attention: head dimension 64, 128 or 256");
-  WM_REQUIRE(scale > 0.0f && scale <= 3.4028234663852886e38f, "prompt attention: the scale must be positive and finite");
+  WM_REQUIRE(scale > 0.0f && scale * kLog2e <= 3.4028234663852886e38f, "prompt attention: the scale must be positive and finite");
   if (B == 0 || Tq == 0) return WM_OK;
   WM_REQUIRE(q && out && cu_seqlens_q && cu_seqlens_k && (Tk == 0 || (k && v)), "prompt attention: missing input or output");
   WM_REQUIRE(q_stride >= static_cast<int64_t>(Hq) * D && k_stride >= static_cast<int64_t>(Hkv) * D &&
