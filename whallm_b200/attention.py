@@ -30,16 +30,17 @@ _BF16, _F32, _INT, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 _NO_CPU = "whallm_b200 ops take CUDA tensors (no CPU fallback)"
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
-# The checks below run on every call of a decode step, where the host's time is what counts for small
-# batches: they read each tensor attribute once, and addresses go to the library as plain integers.
+# The checks below run on every call of a decode step, where for small batches the host's time is what counts:
+# each function tests everything that a good call meets in one expression and looks for the reason only when it
+# fails, and addresses go to the library as plain integers.
 
 
 def _call(name, dev, *args):
     """Call an entry point on device number ``dev`` and its current stream."""
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _call(name, dev, *args)
-    rc = getattr(L.lib(), name)(*args, _raw_stream(dev))
+    rc = getattr(L._lib or L.lib(), name)(*args, _raw_stream(dev))
     if rc:
         L.fail(name, rc)
 
@@ -53,49 +54,54 @@ def _at(name, t, dtype, shape, dev):
     """Address of a contiguous tensor of a given type, shape and device (None: 0)."""
     if t is None:
         return None
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {list(shape)}")
-    if t.get_device() != dev or not t.is_contiguous():
-        if not t.is_cuda:
-            raise ValueError(_NO_CPU)
-        if not t.is_contiguous():
-            raise ValueError("whallm_b200 ops take contiguous tensors")
-        raise ValueError("all tensors of a call must be on one device")
-    return t.data_ptr()
-
-
-def _tokens(name, t, heads=None):
-    """bf16 [T, heads, D] whose heads are dense -> (T, heads, D, values between tokens)."""
-    if t.dtype != _BF16 or t.dim() != 3:
-        raise ValueError(f"{name} must be bf16 [tokens, heads, D]")
-    n, h, d = t.shape
-    s0, s1, s2 = t.stride()
-    if heads is not None and h != heads:
-        raise ValueError(f"{name} has {h} heads, expected {heads}")
     if not t.is_cuda:
         raise ValueError(_NO_CPU)
-    if (s2 != 1 and d > 1) or (s1 != d and h > 1):
-        raise ValueError(f"the heads of a token of {name} must be contiguous")
-    return n, h, d, (s0 if n > 1 else h * d)
+    if not t.is_contiguous():
+        raise ValueError("whallm_b200 ops take contiguous tensors")
+    raise ValueError("all tensors of a call must be on one device")
+
+
+def _tokens(name, t, heads, d, dev):
+    """bf16 [T, heads, D] whose heads are dense (heads, d, dev: what it must match, or None) -> (T, heads, D,
+    values between tokens)."""
+    shape = t.shape
+    if len(shape) == 3 and t.dtype is _BF16:
+        n, h, e = shape
+        s0, s1, s2 = t.stride()
+        at = t.get_device()
+        if ((heads is None or h == heads) and (d is None or e == d) and (at == dev or dev is None) and at >= 0
+                and (s2 == 1 or e == 1) and (s1 == e or h == 1)):
+            return n, h, e, (s0 if n > 1 else h * e)
+    if t.dtype != _BF16 or t.dim() != 3:
+        raise ValueError(f"{name} must be bf16 [tokens, heads, D]")
+    if heads is not None and shape[1] != heads:
+        raise ValueError(f"{name} has {shape[1]} heads, expected {heads}")
+    if d is not None and shape[2] != d:
+        raise ValueError(f"{name} has head dimension {shape[2]}, expected {d}")
+    if not t.is_cuda:
+        raise ValueError(_NO_CPU)
+    if dev is not None and t.get_device() != dev:
+        raise ValueError("all tensors of a call must be on one device")
+    raise ValueError(f"the heads of a token of {name} must be contiguous")
 
 
 def _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt):
-    """Check a paged cache's tensors -> (format id, n_pages, Hkv, page_size, D, B, max_pages, device, the
+    """Check a paged cache's tensors -> (format id, n_pages, Hkv, page_size, D, B, max_pages, device, and the
     addresses of caches, scales and table)."""
     f = PAGED_FORMATS.get(fmt)
     if f is None:
         raise ValueError(f"paged cache format must be one of {sorted(PAGED_FORMATS)}, got {fmt!r}")
-    shape = k_cache.shape
+    shape, tshape, dev = k_cache.shape, page_table.shape, k_cache.get_device()
     dt = _BF16 if f == L.WKV_BF16 else _U8
-    if len(shape) != 4 or k_cache.dtype != dt or v_cache.dtype != dt or v_cache.shape != shape:
-        raise ValueError(f"caches must be {dt} [n_pages, heads, page_size, D] of one shape")
-    pages, heads, size, d = shape
-    if not heads:
-        raise ValueError("a paged cache needs heads")
-    if page_table.dim() != 2 or page_table.dtype != _INT:
+    if not (len(shape) == 4 and len(tshape) == 2 and k_cache.dtype is dt and page_table.dtype is _INT):
+        if len(shape) != 4 or k_cache.dtype != dt:
+            raise ValueError(f"caches must be {dt} [n_pages, heads, page_size, D] of one shape")
         raise ValueError("page_table must be int32 [sequences, max_pages]")
-    tshape = page_table.shape
-    dev = k_cache.get_device()
+    pages, heads, size, d = shape
     if f == L.WKV_BF16:
         if k_scales is not None or v_scales is not None:
             raise ValueError("bf16 caches take no scales")
@@ -106,17 +112,13 @@ def _pool(k_cache, v_cache, k_scales, v_scales, page_table, fmt):
         if k_scales is None or v_scales is None:
             raise ValueError(f"{fmt} caches need {sdt} scales [n_pages, heads, page_size, D/{blk}]")
         ks, vs = _at("k_scales", k_scales, sdt, sshape, dev), _at("v_scales", v_scales, sdt, sshape, dev)
-    at = (_at("k_cache", k_cache, dt, shape, dev), _at("v_cache", v_cache, dt, shape, dev), ks, vs,
-          _at("page_table", page_table, _INT, tshape, dev))
-    if dev < 0:
-        raise ValueError(_NO_CPU)
-    return f, pages, heads, size, d, tshape[0], tshape[1], dev, at
-
-
-def _on(dev, *tensors):
-    for t in tensors:
-        if t.get_device() != dev:
-            raise ValueError("all tensors of a call must be on one device")
+    v = _at("v_cache", v_cache, dt, shape, dev)
+    t = _at("page_table", page_table, _INT, tshape, dev)
+    if dev < 0 or not heads or not k_cache.is_contiguous():
+        if not heads:
+            raise ValueError("a paged cache needs heads")
+        raise ValueError(_NO_CPU if dev < 0 else "whallm_b200 ops take contiguous tensors")
+    return f, pages, heads, size, d, tshape[0], tshape[1], dev, k_cache.data_ptr(), v, ks, vs, t
 
 
 def _scale(scale, d):
@@ -136,15 +138,14 @@ def paged_append(k, v, cu_seqlens, k_cache, v_cache, page_table, lengths, fmt="b
     already.  Their ``mass`` (float32 [B, Hkv, capacity]) becomes 0 and their
     ``positions`` (int32, same shape) the token's position, ``seen`` int32 [B]
     counting every token of the sequence up to and including these."""
-    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
-                                                                               page_table, fmt)
-    T, _, dk, ks = _tokens("k", k, heads)
-    Tv, _, dv, vs = _tokens("v", v, heads)
-    if dk != d or dv != d or Tv != T:
-        raise ValueError("k and v must have one shape and the cache's head dimension")
+    f, pages, heads, size, d, B, width, dev, kc, vc, ksc, vsc, table = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                             page_table, fmt)
+    T, _, _, ks = _tokens("k", k, heads, d, dev)
+    Tv, _, _, vs = _tokens("v", v, heads, d, dev)
+    if Tv != T:
+        raise ValueError("k and v must have as many tokens")
     if positions is not None and seen is None:
         raise ValueError("positions need the sequences' token counts (seen)")
-    _on(dev, k, v)
     shape = (B, heads, width * size)
     _call("wkv_paged_append", dev, k.data_ptr(), v.data_ptr(), ks, vs, _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev),
           T, B, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width, _at("lengths", lengths, _INT, (B,), dev),
@@ -162,8 +163,8 @@ def paged_evict(k_cache, v_cache, page_table, lengths, mass, positions, seen, bu
     Without ``out``, mass and positions are updated in place; else ``out`` is
     ``(mass, positions, lengths)`` to write, which may share the input's mass and
     positions but not its lengths.  Returns (mass, positions, lengths)."""
-    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
-                                                                               page_table, fmt)
+    f, pages, heads, size, d, B, width, dev, kc, vc, ksc, vsc, table = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                             page_table, fmt)
     cap = width * size
     shape = (B, heads, cap)
     new_mass, new_pos, new_len = out if out is not None else (mass, positions, torch.empty_like(lengths))
@@ -190,13 +191,12 @@ def decode_attention(q, k_cache, v_cache, page_table, lengths, fmt="bf16", k_sca
     over the query heads of its key-value head.  ``scale`` defaults to D^-1/2.  A
     sequence without entries gets zeros (lse -inf); one whose length or pages are
     out of range gets NaN."""
-    f, pages, heads, size, d, B, width, dev, (kc, vc, ksc, vsc, table) = _pool(k_cache, v_cache, k_scales, v_scales,
-                                                                               page_table, fmt)
-    Bq, Hq, dq, qs = _tokens("q", q)
-    if Bq != B or dq != d or Hq % heads:
+    f, pages, heads, size, d, B, width, dev, kc, vc, ksc, vsc, table = _pool(k_cache, v_cache, k_scales, v_scales,
+                                                                             page_table, fmt)
+    Bq, Hq, _, qs = _tokens("q", q, None, d, dev)
+    if Bq != B or Hq % heads:
         raise ValueError("q must be [sequences, a multiple of the cache's heads, D]")
     scale = _scale(scale, d)
-    _on(dev, q)
     if out is None:
         out = q.new_empty((B, Hq, d))
     lse = q.new_empty((B, Hq), dtype=_F32) if return_lse else None
@@ -218,11 +218,12 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     keys up to i + nk - nq (a prompt that continues a history).  Tokens may be
     strided (slices of one projection).  A row that sees no key gets zeros (lse
     -inf); rows outside every sequence are not written."""
-    Tq, Hq, d, qs = _tokens("q", q)
-    Tk, Hkv, dk, ks = _tokens("k", k)
-    Tv, _, dv, vs = _tokens("v", v, Hkv)
-    if dk != d or dv != d or Tv != Tk or Hkv == 0 or Hq % Hkv:
-        raise ValueError("k and v must have one shape, q's head dimension and a divisor of q's heads")
+    dev = q.get_device()
+    Tq, Hq, d, qs = _tokens("q", q, None, None, None)
+    Tk, Hkv, _, ks = _tokens("k", k, None, d, dev)
+    Tv, _, _, vs = _tokens("v", v, Hkv, d, dev)
+    if Tv != Tk or Hkv == 0 or Hq % Hkv:
+        raise ValueError("k and v must have one shape and a divisor of q's heads")
     if cu_seqlens_k is None:
         if Tk != Tq:
             raise ValueError("keys of another count than the rows need cu_seqlens_k")
@@ -231,8 +232,6 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     if B < 0:
         raise ValueError("cu_seqlens must be int32 [sequences + 1]")
     scale = _scale(scale, d)
-    dev = q.get_device()
-    _on(dev, k, v)
     if out is None:
         out = q.new_empty((Tq, Hq, d))
     lse = q.new_empty((Tq, Hq), dtype=_F32) if return_lse else None
