@@ -21,7 +21,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
           "--expt-relaxed-constexpr"]
-EXACT = {"formats.cu", "router.cu", "moe_mx.cu"}
+EXACT = {"formats.cu", "kv_paged.cu", "router.cu", "moe_mx.cu"}
 
 
 def sources():

@@ -34,6 +34,11 @@
 // scales (O is rescaled when that grows, as for the maximum) and times 2^15: the
 // weights are f16 values of at most 2^15, rounded to 11 bits down to 2^-29 of the
 // largest, and no dequantized row is ever rounded.
+//
+// Measured (CUDA graphs, three input sets in turn): 64 sequences of 90 to 8190
+// entries, 32/8 heads of 128, bf16: 178 us, 6.2 TB/s (94 % of a plain copy); two of
+// 130,000 entries, 16/2 heads of 256, e4m3: 53 to 56 us, the rows at 5.7 TB/s; one of
+// 4095 entries, 32/8 heads of 128: 9.4 us, a chain of latencies.
 #include <cooperative_groups.h>
 
 #include <algorithm>

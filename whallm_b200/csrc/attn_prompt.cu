@@ -37,6 +37,15 @@
 // behind the sequence's end (another sequence's values) and every value that is
 // not finite; such values (there are none in a healthy model) are added to the
 // rows that do see them at the end.  The check hides under the step's softmax.
+//
+// Measured (events, back to back): 8192 tokens without a mask, 32/8 heads, D = 64
+// 730 us (750 TF/s), D = 128 845 us (1300 TF/s), 16/2 heads, D = 256 795 us (1380
+// TF/s; cuBLAS sustains 1406 on the same GPU); causal 16384 tokens 1450, 1715 and
+// 1635 us.  D = 128 and 256 are bound by the tensor pipe and the power limit, D = 64
+// by the exp2 unit (16 per cycle and SM: 2048 of the 3200 cycles of two steps) and
+// the issue of its short MMAs; many short sequences by the 4 us between a block's
+// last product and the next block's (1 PV, 1.5 output, the rest the first S and
+// its softmax).
 #include <algorithm>
 
 #include "wm_tc.cuh"

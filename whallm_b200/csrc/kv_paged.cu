@@ -22,7 +22,8 @@ namespace {
 // scale blocks are 2 or 4 adjacent lanes, as in k_kv_fp8_quantize.  Bound by HBM
 // for bf16 rows (2 B read, 2 B written per value) and by the quantizer's
 // arithmetic for e4m3 rows: with a search per piece it took 475 instructions per
-// 16 values, 59 % of the issue slots.
+// 16 values, 59 % of the issue slots.  13,200 tokens of 2 x 256 values to e4m3: 15.6
+// us (22.5 with one piece per lane and a search each); 64 tokens of 8 x 128: 2.5 us.
 
 constexpr int kSeqSmem = 512;          // sequences searched in shared memory
 
@@ -131,7 +132,9 @@ __global__ void __launch_bounds__(256, 5) k_paged_append(const wm_bf16 *__restri
 // of positive weights falls into a few bins, so lanes with equal digits add once.
 // A single CTA moves its rows itself; behind a cluster a second kernel does, over
 // the whole GPU.  Bound by the latency of the selection's steps (about 15
-// dependent phases) for short caches and by the moved rows for long ones.
+// dependent phases) for short caches and by the moved rows for long ones: 64 heads
+// of 2049 entries 10.5 us, 8 heads of 20,000 to 32,768 entries down to 4096 31 us
+// (67 us when the clusters' own CTAs moved the rows one load at a time).
 
 constexpr int kET = 512;           // threads
 constexpr int kBins = 256;         // bins of a digit

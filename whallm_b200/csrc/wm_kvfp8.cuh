@@ -1,6 +1,7 @@
-// The e4m3 KV row quantizer, shared by the row kernels (formats.cu) and the
-// paged cache's append (kv_paged.cu).  Both are compiled with -fmad=false: the
-// bytes and scales are the same wherever a row is quantized.
+// The e4m3 KV row quantizer, shared by the row kernels (formats.cu, where its
+// arithmetic is explained) and the paged cache's append (kv_paged.cu).  Both are
+// compiled with -fmad=false: the bytes and scales are the same wherever a row is
+// quantized.
 #pragma once
 
 #include "wm_common.cuh"
