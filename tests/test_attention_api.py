@@ -69,6 +69,8 @@ def test_append_refusals():
     expect(f, append_args(vs=504), "16-byte aligned and hold")
     expect(f, append_args(v=ODD), "16-byte aligned and hold")
     expect(f, append_args(pos=P), "token counts")
+    expect(f, append_args(Hkv=5000, ks=5000 * 128, vs=5000 * 128), "at most 4096 heads")
+    expect(f, append_args(Hkv=4096, ks=4096 * 128, vs=4096 * 128, T=1 << 20), "too many values")
     expect(f, append_args(T=0), None, L.WM_OK)
     expect(f, append_args(B=0), None, L.WM_OK)
 
@@ -98,6 +100,8 @@ def test_decode_refusals():
     expect(f, decode_args(width=1024, bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
     expect(f, decode_args(width=1024, ws=ODD), "256-byte aligned")
     expect(f, decode_args(mass=P, bytes=16), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, decode_args(mass=P, page=1 << 20, width=100, bytes=1 << 60), "batch or capacity too large")
+    expect(f, decode_args(out=ctypes.c_void_p((1 << 20) + 4)), "8-byte aligned")
     expect(f, decode_args(B=0), None, L.WM_OK)
     size = L.lib().wattn_decode_workspace_size
     assert size(2, 6, 4, 128, L.WKV_BF16, 16, 4, 0) == 0 and size(2, 8, 4, 100, L.WKV_BF16, 16, 4, 0) == 0
@@ -117,6 +121,8 @@ def test_prompt_refusals():
     expect(f, prompt_args(ks=500), "16-byte aligned and hold")
     expect(f, prompt_args(qs=1028), "16-byte aligned and hold")
     expect(f, prompt_args(k=ODD), "16-byte aligned and hold")
+    expect(f, prompt_args(out=ctypes.c_void_p((1 << 20) + 16)), "32-byte aligned")
+    expect(f, prompt_args(Tq=1 << 30, Hq=16, qs=2048), "too many rows")
     expect(f, prompt_args(Tq=0), None, L.WM_OK)
 
 

@@ -188,6 +188,12 @@ def test_decode_at_the_cluster_limit(dev, cap, fmt, D, G):
     run_decode(dev, [5, cap - 3], 2 * G, 2, D, 64, fmt, seed=cap)
 
 
+@pytest.mark.parametrize("mass", [False, True])
+def test_decode_more_parts_than_join_threads(dev, mass):
+    # one pair over every CTA: 592 parts, more than the join holds factors for at once
+    run_decode(dev, [90001], 1, 1, 64, 64, "mxfp8", seed=11, mass=mass)
+
+
 def test_decode_large_scores(dev):
     # scores of deviation ~60: nearly one-hot weights, running maxima that grow late
     run_decode(dev, [300, 5], 8, 2, 128, 16, "bf16", seed=6, scale=2.0, std=1.5)
@@ -273,6 +279,68 @@ def test_decode_on_two_streams(dev, max_pages):
     for s in sides:
         torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
+
+
+@pytest.mark.parametrize("fmt,max_pages", [("bf16", 8), ("mxfp8", 300)])
+def test_captured_step(dev, fmt, max_pages):
+    """A whole decode step in a graph -- lengths, append, attention with weights -- replayed over new inputs, gives
+    the eager steps' results; the eviction after it likewise."""
+    B, Hkv, Hq, D, page = 3, 2, 8, 128, 16
+    g = gen(61, dev)
+
+    def cache():
+        c = W.PagedKVCache(B, Hkv, D, n_pages=30, page_size=page, max_pages=max_pages, fmt=fmt, track=True)
+        c.reserve([100, 40, 9])
+        return c
+
+    a, b = cache(), cache()
+    b.page_table.copy_(a.page_table)
+    start = [rnd(gen(62 + i, dev), 90, Hkv, D, dev=dev) for i in range(2)]
+    for c in (a, b):
+        c.append(*start, [60, 30, 0])
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    qkv = torch.zeros((B, Hq + 2 * Hkv, D), dtype=torch.bfloat16, device=dev)
+
+    def step(c):
+        q, k, v = qkv.split([Hq, Hkv, Hkv], dim=1)
+        c.lengths.add_(1)
+        c.seen.add_(1)
+        W.paged_append(k, v, cu, c.keys, c.values, c.page_table, c.lengths, c.fmt, c.key_scales, c.value_scales, c.mass,
+                       c.positions, c.seen)
+        return W.decode_attention(q, c.keys, c.values, c.page_table, c.lengths, c.fmt, c.key_scales, c.value_scales,
+                                  mass=c.mass)
+
+    warm = cache()
+    step(warm)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step(b)
+    for _ in range(9):
+        qkv.copy_(rnd(g, B, Hq + 2 * Hkv, D, dev=dev))
+        want = step(a)
+        gr.replay()
+        assert torch.equal(out, want)
+    live = [69, 39, 9]
+    assert a.lengths.tolist() == live == b.lengths.tolist()
+    outs = []
+    for c in (a, b):
+        new = torch.zeros_like(c.lengths)
+        args = (c.keys, c.values, c.page_table, c.lengths, c.mass, c.positions, c.seen, 32, 8, 2, c.fmt, c.key_scales,
+                c.value_scales, (c.mass, c.positions, new))
+        if c is b:
+            ev = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(ev):
+                W.paged_evict(*args)
+            ev.replay()
+        else:
+            W.paged_evict(*args)
+        c.lengths.copy_(new)
+        outs.append(W.decode_attention(qkv[:, :Hq], c.keys, c.values, c.page_table, c.lengths, c.fmt, c.key_scales,
+                                       c.value_scales))
+    assert a.lengths.tolist() == [32, 32, 9] == b.lengths.tolist()
+    assert torch.equal(outs[0], outs[1])
+    for x, n in enumerate([32, 32, 9]):
+        assert torch.equal(a.mass[x, :, :n], b.mass[x, :, :n]) and torch.equal(a.positions[x, :, :n], b.positions[x, :, :n])
 
 
 # ------------------------------------------------------------------ prompts --

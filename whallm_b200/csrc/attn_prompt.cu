@@ -18,8 +18,8 @@
 // writes P = exp2(S scale log2e - m) as bf16 over S; O += P V with P from TMEM.
 // Up to D = 128 the block has two tiles of 128 rows and step s works on tile
 // s & 1 (two softmax warpgroups in turn, each with its own O); at D = 256 TMEM
-// holds one O of 256 columns, the block has one tile, step s takes the s-th
-// 64-key tile and the two warpgroups hand the running maximum to each other.
+// holds one O of 256 columns, the block has one tile, step s takes the s-th key
+// tile and the two warpgroups hand the running maximum to each other.
 // The MMA warp issues PV(s), S(s + 2), PV(s + 1), ...: instructions of one thread
 // execute in order, so S(s + 2) may overwrite the buffer that PV(s) read.
 //
