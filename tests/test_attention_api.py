@@ -188,3 +188,4 @@ def test_paged_cache_refusals():
     with pytest.raises(ValueError, match="CUDA tensors"):
         c.append(x, x)
     assert c.offsets == [0, 0]                   # the refused call added no entry
+    assert c.lengths.tolist() == [0, 0] and c.seen.tolist() == [0, 0]

@@ -459,6 +459,7 @@ class PagedKVCache:
         self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.seen = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._steps = torch.arange(batch + 1, dtype=torch.int32, device=device)
         cap = (batch, heads, self.max_pages * page_size)
         self.mass = torch.zeros(cap, dtype=torch.float32, device=device) if track else None
         self.positions = torch.zeros(cap, dtype=torch.int32, device=device) if track else None
@@ -513,17 +514,23 @@ class PagedKVCache:
         if keys.shape != values.shape or tuple(keys.shape) != (sum(counts), self.heads, self.dimension):
             raise ValueError("keys and values must be [sum of counts, heads, D] of the cache")
         self.reserve(counts)
-        dev = self.lengths.device
-        cu = [0]
-        for c in counts:
-            cu.append(cu[-1] + c)
-        cu = torch.tensor(cu, dtype=torch.int32).to(dev)
-        new = cu[1:] - cu[:-1]
-        lengths, seen = self.lengths + new, self.seen + new
-        _A.paged_append(keys, values, cu, self.keys, self.values, self.page_table, lengths, self.fmt, self.key_scales,
-                        self.value_scales, self.mass, self.positions, seen)
-        self.lengths.copy_(lengths)
-        self.seen.copy_(seen)
+        if min(counts) == max(counts) == 1:              # a decode step: nothing comes from the host
+            cu, new = self._steps, 1
+        else:
+            cu = [0]
+            for c in counts:
+                cu.append(cu[-1] + c)
+            cu = torch.tensor(cu, dtype=torch.int32).to(self.lengths.device)
+            new = cu[1:] - cu[:-1]
+        self.lengths.add_(new)
+        self.seen.add_(new)
+        try:
+            _A.paged_append(keys, values, cu, self.keys, self.values, self.page_table, self.lengths, self.fmt,
+                            self.key_scales, self.value_scales, self.mass, self.positions, self.seen)
+        except Exception:
+            self.lengths.sub_(new)
+            self.seen.sub_(new)
+            raise
         self._len = [n + c for n, c in zip(self._len, counts)]
         self._seen = [n + c for n, c in zip(self._seen, counts)]
 
