@@ -188,6 +188,27 @@ def test_decode_at_the_cluster_limit(dev, cap, fmt, D, G):
     run_decode(dev, [5, cap - 3], 2 * G, 2, D, 64, fmt, seed=cap)
 
 
+@pytest.mark.parametrize("fmt,D,Hq,Hkv,mass", [("bf16", 128, 8, 2, False), ("mxfp8", 64, 4, 1, True), ("fp8_f32_b64", 256, 8, 4, False)])
+def test_decode_in_rounds(dev, fmt, D, Hq, Hkv, mass):
+    # enough units for three rounds of CTAs: their borders fall inside pairs, and some pairs inside one CTA
+    r = np.random.RandomState(8)
+    want = 64 * 592 * 64 // Hkv                                  # keys for the largest number of CTAs in a round
+    lens = [int(x) for x in r.randint(1, 2 * want // 40, 44)] + [0, 1, 70, 0]
+    c = Cache(dev, lens, Hkv, D, 64, fmt, seed=12)
+    q = rnd(gen(13, dev), len(lens), Hq, D, std=2.0, dev=dev)
+    m = torch.zeros((len(lens), Hkv, c.width * 64), device=dev) if mass else None
+    out, lse = W.decode_attention(q, *c.args, mass=m, return_lse=True)
+    for b in (0, 7, 20, 33, 43, 44, 45, 46, 47):
+        ref = A.attend(f64(q[b:b + 1]), *c.rows[b], D ** -0.5)
+        check_out(out[b:b + 1], ref, D)
+        check_lse(lse[b:b + 1], ref, D)
+        if mass:
+            check_mass(f64(m[b, :, :lens[b]]), ref, D)
+    for b in range(len(lens)):                                   # and every sequence as when it is alone
+        one = W.decode_attention(q[b:b + 1], c.k, c.v, c.table[b:b + 1], c.lengths[b:b + 1], fmt, c.ks, c.vs)
+        assert (one.float() - out[b:b + 1].float()).abs().max() <= 2.0 ** -6 * out[b].float().abs().max() + 1e-6
+
+
 @pytest.mark.parametrize("mass", [False, True])
 def test_decode_more_parts_than_join_threads(dev, mass):
     # one pair over every CTA: 592 parts, more than the join holds factors for at once

@@ -7,7 +7,7 @@
 // against 4 D G operations.
 //
 // Work split.  The entries of all (sequence, head) pairs form one line of units
-// of 64 keys; every CTA takes an equal share of the line, found from the
+// of 64 keys; every CTA takes a share of the line (struct Line), found from the
 // lengths on the device (no host copy, so a captured call follows the lengths).
 // A CTA that meets the end of a pair writes its part (running maximum, sum and
 // unnormalised output) and goes on with the next pair; a second kernel joins
@@ -36,7 +36,7 @@
 // largest, and no dequantized row is ever rounded.
 //
 // Measured (CUDA graphs, three input sets in turn): 64 sequences of 90 to 8190
-// entries, 32/8 heads of 128, bf16: 178 us, 6.2 TB/s (94 % of a plain copy); two of
+// entries, 32/8 heads of 128, bf16: 166 us, 6.7 TB/s (a plain copy: 6.5); two of
 // 130,000 entries, 16/2 heads of 256, e4m3: 53 to 56 us, the rows at 5.7 TB/s; one of
 // 4095 entries, 32/8 heads of 128: 9.4 us, a chain of latencies.
 #include <cooperative_groups.h>
@@ -74,7 +74,7 @@ struct DecodeArgs {
   float *part_o, *part_m, *part_l;      // parts: [slots][heads of a chunk][D] and [slots][heads of a chunk]
   float *scores;                        // [pairs][capacity][score_heads], with mass only
   int score_heads;                      // a chunk's query heads, rounded up to 2
-  int n_cta;                            // CTAs the line is split over
+  int n_cta, rounds;                    // CTAs of a round over the line; rounds that a full cache would have
   int cluster;                          // CTAs per pair, or 0 for the line
 };
 
@@ -99,11 +99,63 @@ __device__ __forceinline__ int64_t warp_units(const DecodeArgs &a, int upto) {
   return s;
 }
 
-// CTAs that take part: each has at least one unit, so every part between a
-// pair's first and last is written.
-__device__ __forceinline__ int64_t parts_of(const DecodeArgs &a, int64_t total) {
-  return total < a.n_cta ? total : a.n_cta;
-}
+// The line of units cut among the CTAs.  Equal shares end at different times, as
+// SMs do not get equal bandwidth (130 to 180 us for 114 units a CTA), so a long line
+// has three rounds of up to a.n_cta CTAs, as many as fit on the GPU at once: the
+// first round gets 12 / 16 of it, the later ones, whose CTAs start wherever one has
+// ended, 3 / 16 and 1 / 16 in shares of at least kLeastUnits.  64 sequences of 90 to
+// 8190 entries, 32/8 heads of 128: 182 -> 165 us.  At 27 units a CTA the later CTAs'
+// starts cost more than they even out (two of 130,000 entries, e4m3 of 256 values:
+// 53 -> 61 us), so shorter lines have one round.  Every CTA that takes part has at
+// least one unit and their numbers follow one another along the line, so every part
+// between a pair's first and last is written.
+constexpr int kTiers = 3;
+__device__ constexpr int kShare[kTiers] = {12, 3, 1};
+constexpr int kTierUnits = 64;          // units per CTA from which there are several rounds
+constexpr int kLeastUnits = 16;
+
+struct Line {
+  int64_t from[kTiers + 1];             // the rounds' ends on the line
+  int n;                                // CTAs of a round
+  __device__ __forceinline__ Line(const DecodeArgs &a, int64_t total) : n(a.n_cta) {
+    const bool several = total >= static_cast<int64_t>(kTierUnits) * a.n_cta;
+    from[0] = 0;
+    int done = 0;
+#pragma unroll
+    for (int k = 0; k < kTiers; ++k) {
+      done += kShare[k];
+      from[k + 1] = several ? total * done / 16 : total;
+    }
+  }
+  // CTAs of round k that have units, and the units of CTA i: [start(i), start(i + 1))
+  __device__ __forceinline__ int64_t count(int k) const {
+    const int64_t l = from[k + 1] - from[k];
+    return min(k ? (l + kLeastUnits - 1) / kLeastUnits : l, static_cast<int64_t>(n));
+  }
+  __device__ __forceinline__ int64_t start(int i) const {
+    int64_t x = from[kTiers];
+#pragma unroll
+    for (int k = kTiers - 1; k >= 0; --k) {
+      const int64_t r = i - base(k), c = count(k);
+      if (r >= 0 && r < c) x = from[k] + quotient((from[k + 1] - from[k]) * r, c);
+    }
+    return x;
+  }
+  __device__ __forceinline__ int64_t base(int k) const {           // CTAs of the rounds before
+    int64_t b = 0;
+#pragma unroll
+    for (int y = 0; y < kTiers; ++y) b += y < k ? count(y) : 0;
+    return b;
+  }
+  // the CTA that holds unit x
+  __device__ __forceinline__ int64_t cta(int64_t x) const {
+    int64_t i = 0;
+#pragma unroll
+    for (int k = 0; k < kTiers; ++k)
+      if (x >= from[k] && x < from[k + 1]) i = base(k) + quotient((x - from[k] + 1) * count(k) - 1, from[k + 1] - from[k]);
+    return i;
+  }
+};
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -661,10 +713,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   } else {
     // this CTA's share [u, u_end) of the line of units
     const int64_t total = warp_units(a, a.B) * PH;
-    const int64_t n_cta = parts_of(a, total);
-    if (blockIdx.x >= n_cta) return;
-    int64_t u = quotient(total * blockIdx.x, n_cta);
-    const int64_t u_end = quotient(total * (blockIdx.x + 1), n_cta);
+    const Line line(a, total);
+    int64_t u = line.start(blockIdx.x);
+    const int64_t u_end = line.start(blockIdx.x + 1);
+    if (u >= u_end) return;
     int b = 0;
     int64_t base = 0;                                 // line position of sequence b
     for (int b0 = 0;; b0 += 32) {                     // the sequence that holds unit u
@@ -747,10 +799,10 @@ __global__ void __launch_bounds__(TJ) k_attn_join(DecodeArgs a, int groups) {
   const int len = a.lengths[b];
   const bool bad = len < 0 || len > cap;
   const float nan = __uint_as_float(0x7fc00000u);
-  const int64_t n_cta = parts_of(a, total);
+  const Line line(a, total);
   // CTAs that hold the nu units from `at`
-  auto part0 = [&](int64_t at) { return nu ? quotient((at + 1) * n_cta - 1, total) : 0; };
-  auto parts = [&](int64_t at, int64_t p0) { return nu ? static_cast<int>(quotient((at + nu) * n_cta - 1, total) - p0) + 1 : 0; };
+  auto part0 = [&](int64_t at) { return nu ? line.cta(at) : 0; };
+  auto parts = [&](int64_t at, int64_t p0) { return nu ? static_cast<int>(line.cta(at + nu - 1) - p0) + 1 : 0; };
 
   if (output) {
     const int64_t p00 = part0(first), slot0 = p00 + pair;
@@ -951,7 +1003,7 @@ int launch(DecodeArgs &a, cudaStream_t stream) {
     return wm::check_launch("wattn_decode");
   }
   cudaError_t e = wm::allow_smem<k_attn_decode<D, FMT, NH, false>>(S::kSmem);
-  if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH, false>, dim3(a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
+  if (e == cudaSuccess) e = wm::launch_pdl(k_attn_decode<D, FMT, NH, false>, dim3(a.rounds * a.n_cta), dim3(kWarps * 32), S::kSmem, stream, a);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_decode: ") + cudaGetErrorString(e));
   const int64_t pairs = static_cast<int64_t>(a.B) * a.pool.Hkv * a.NC;
   const bool many = a.n_cta >= kManyParts * pairs;
@@ -990,7 +1042,7 @@ struct Launch {
 };
 
 struct Plan {
-  int NC, heads, score_heads, n_cta, cluster;
+  int NC, heads, score_heads, n_cta, rounds, cluster;
   int64_t pairs, slots, cap;
   size_t off_m, off_l, off_s, bytes;
 };
@@ -1012,8 +1064,10 @@ Plan plan_of(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_page
     p.n_cta = static_cast<int>(p.pairs * p.cluster);
     return p;
   }
-  p.n_cta = dispatch(D, fmt, G, GridOf{p.pairs * ((p.cap + kUnit - 1) / kUnit)});
-  p.slots = p.n_cta + p.pairs;
+  const int64_t most = p.pairs * ((p.cap + kUnit - 1) / kUnit);
+  p.n_cta = dispatch(D, fmt, G, GridOf{most});
+  p.rounds = most >= static_cast<int64_t>(kTierUnits) * p.n_cta ? kTiers : 1;
+  p.slots = static_cast<int64_t>(p.rounds) * p.n_cta + p.pairs;
   auto up = [](size_t x) { return (x + 255) & ~size_t{255}; };
   p.off_m = up(static_cast<size_t>(p.slots) * p.heads * D * 4);
   p.off_l = p.off_m + up(static_cast<size_t>(p.slots) * p.heads * 4);
@@ -1058,7 +1112,7 @@ int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   DecodeArgs a{pool, q, q_stride, lengths, B, Hq, Hq / Hkv, p.NC, scale * kLog2e, out, lse, mass,
                reinterpret_cast<float *>(ws), reinterpret_cast<float *>(ws + p.off_m), reinterpret_cast<float *>(ws + p.off_l),
-               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.score_heads, p.n_cta, p.cluster};
+               mass ? reinterpret_cast<float *>(ws + p.off_s) : nullptr, p.score_heads, p.n_cta, p.rounds, p.cluster};
   return dispatch(D, fmt, a.G, Launch{a, stream});
 }
 
