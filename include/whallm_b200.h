@@ -313,11 +313,14 @@ WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int H
  * tokens, a continuation also its history; else all nk keys.  out bf16
  * [Tq, Hq, D]; lse float32 [Tq, Hq] or NULL (natural logarithm).  A row that sees
  * no key gets zeros and lse -inf; rows outside every sequence are not written.
- * D is 64, 128 or 256.  Uses no workspace.  */
+ * D is 64, 128 or 256.  Workspace: wattn_prompt_workspace_size (0 unless few rows
+ * meet many keys, which are then split over the GPU); calls that share one must
+ * not overlap.  */
+WM_API size_t wattn_prompt_workspace_size(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 WM_API int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q_stride, int64_t k_stride,
                         int64_t v_stride, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int B, int Tq,
                         int Tk, int Hq, int Hkv, int D, float scale, int causal, wm_bf16 *out, float *lse,
-                        wm_stream_t stream);
+                        void *workspace, size_t ws_bytes, wm_stream_t stream);
 
 /* --------------------------------------------------------------- router --- */
 

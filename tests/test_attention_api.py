@@ -39,7 +39,7 @@ def decode_args(**c):
 
 def prompt_args(**c):
     d = dict(q=P, k=P, v=P, qs=1024, ks=512, vs=512, cq=P, ck=P, B=2, Tq=8, Tk=8, Hq=8, Hkv=4, D=128, scale=0.1, causal=1, out=P,
-             lse=None, stream=None)
+             lse=None, ws=None, ws_bytes=0, stream=None)
     return tuple({**d, **c}.values())
 
 
@@ -124,6 +124,15 @@ def test_prompt_refusals():
     expect(f, prompt_args(out=ctypes.c_void_p((1 << 20) + 16)), "32-byte aligned")
     expect(f, prompt_args(Tq=1 << 30, Hq=16, qs=2048), "too many rows")
     expect(f, prompt_args(Tq=0), None, L.WM_OK)
+    # few rows on many keys are split over the GPU, which takes a workspace: at most one slot of 256 rows per SM
+    size = L.lib().wattn_prompt_workspace_size
+    some = size(2, 8, 8192, 8, 4, 128)
+    assert some > 0 and some % (256 * 130 * 4) == 0 and size(2, 8, 8192, 8, 4, 256) % (128 * 258 * 4) == 0
+    assert size(2, 8, 100, 8, 4, 128) == 0 and size(2, 32768, 32768, 8, 4, 128) == 0 and size(0, 8, 8192, 8, 4, 128) == 0
+    assert size(2, 8, 8192, 6, 4, 128) == 0 and size(2, 8, 8192, 8, 4, 96) == 0
+    expect(f, prompt_args(Tk=8192, ws=P, ws_bytes=some - 1), "workspace too small", L.WM_ERR_WORKSPACE)
+    expect(f, prompt_args(Tk=8192, ws_bytes=some), "256-byte aligned")
+    expect(f, prompt_args(Tk=8192, ws=ctypes.c_void_p((1 << 20) + 64), ws_bytes=some), "256-byte aligned")
 
 
 def test_python_refusals():

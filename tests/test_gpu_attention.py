@@ -522,6 +522,84 @@ def test_prompt_repeats_and_captures(dev):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("nq,nk,Hq,Hkv", [
+    ([64], [9000], 8, 2), ([1], [30011], 4, 1),                          # one block a head, many parts
+    ([1, 40, 0, 130, 5, 3], [5000, 41, 30, 130, 9001, 0], 6, 2),         # ragged; q not by TMA; sequences without rows or keys
+    ([300, 70], [4200, 60], 4, 4),                                       # rows without keys beside split ones
+    ([1000], [5000], 16, 1), ([4500], [4500], 2, 2),                     # blocks of very different lengths
+])
+def test_prompt_few_rows_on_many_keys(dev, D, nq, nk, Hq, Hkv):
+    run_prompt(dev, nq, nk, Hq, Hkv, D, seed=40 + D)
+
+
+def test_prompt_split_full_and_many_sequences(dev):
+    run_prompt(dev, [5, 129], [6000, 4097], 4, 1, 128, causal=False, seed=41)
+    nq = [3] * 40                                                        # more sequences than a warp's lanes
+    run_prompt(dev, nq, [10 + 60 * i for i in range(40)], 4, 2, 64, seed=42)
+    run_prompt(dev, [70], [8192], 4, 2, 128, seed=43, scale=1.0)         # scores far apart
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_split_values_that_are_not_finite(dev, D):
+    g = gen(44, dev)
+    nk = 9000
+    q, k, v = rnd(g, 40, 4, D, dev=dev), rnd(g, nk, 2, D, dev=dev), rnd(g, nk, 2, D, dev=dev)
+    cq, ck = (torch.tensor([0, n], dtype=torch.int32, device=dev) for n in (40, nk))
+    want, lse = W.prompt_attention(q, k, v, cq, ck, return_lse=True)
+    for bad in (float("nan"), float("inf")):
+        k2, v2 = k.clone(), v.clone()
+        v2[nk - 11, 1, D - 1] = bad                                      # rows from 29 on see it
+        v2[100, 0, 2] = bad                                              # every row sees it
+        got = W.prompt_attention(q, k, v2, cq, ck)
+        assert torch.equal(got[:29, 2:], want[:29, 2:]) and torch.equal(got[:, 2:, :D - 1], want[:, 2:, :D - 1])
+        late, all_ = got[29:, 2:, D - 1], got[:, :2, 2]
+        assert (torch.isnan(late) if bad != bad else late == bad).all() and not torch.isfinite(all_).any()
+        assert torch.equal(got[:, :2, 3:], want[:, :2, 3:])
+        k2[nk - 21, 0, 5] = float("nan")
+        got, l2 = W.prompt_attention(q, k2, v, cq, ck, return_lse=True)
+        assert torch.equal(got[:19], want[:19]) and torch.equal(got[:, 2:], want[:, 2:]) and torch.equal(l2[:19], lse[:19])
+        assert torch.isnan(got[19:, :2]).all() and torch.isnan(l2[19:, :2]).all()
+
+
+def test_prompt_split_captured_streams_and_bounds(dev):
+    """A captured call follows the device's bounds; two captured calls keep their own sums; rows outside stay."""
+    g = gen(45, dev)
+    q, k, v = rnd(g, 200, 8, 128, dev=dev), rnd(g, 12000, 2, 128, dev=dev), rnd(g, 12000, 2, 128, dev=dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)      # noqa: E731
+    cq, ck, k2 = i32(0, 64, 200), i32(0, 12000, 12000), k.flip(0).contiguous()
+    graphs, outs = [], []
+    for kk in (k, k2):
+        W.prompt_attention(q, kk, v, cq, ck)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(W.prompt_attention(q, kk, v, cq, ck))
+        graphs.append(gr)
+    for a, b in (((0, 64, 200), (0, 12000, 12000)), ((0, 1, 150), (0, 3, 11900)), ((10, 60, 200), (50, 6000, 12000))):
+        cq.copy_(i32(*a))
+        ck.copy_(i32(*b))
+        want = []
+        for kk in (k, k2):
+            out = torch.full_like(q, 7.0)
+            want.append(W.prompt_attention(q, kk, v, cq, ck, out=out))
+            assert (out[:a[0]] == 7.0).all() and (out[a[2]:] == 7.0).all()
+        s = torch.cuda.Stream(dev)
+        s.wait_stream(torch.cuda.current_stream(dev))
+        for o in outs:
+            o.fill_(7.0)
+        graphs[0].replay()
+        graphs[1].replay()
+        with torch.cuda.stream(s):
+            side = W.prompt_attention(q, k, v, cq, ck, out=torch.full_like(q, 7.0))
+        torch.cuda.synchronize(dev)
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(side, want[0])
+    # bounds that overlap or run backwards: every access stays inside, rows of one owner are right
+    W.prompt_attention(q, k, v, i32(0, 200, 0, 200, 0, 200), i32(0, 12000, 0, 12000, 0, 12000))
+    good = W.prompt_attention(q, k, v, i32(0, 200, 0, 0), i32(0, 12000, 0, 0))
+    ref = A.attend(f64(q), f64(k), f64(v), 128 ** -0.5, True)
+    check_out(good, ref, 128)
+
+
 # ------------------------------------------------------------ append, evict --
 
 @pytest.mark.parametrize("fmt", FMTS)

@@ -66,7 +66,8 @@ SIGNATURES = {
                         _P],
     "wattn_decode_workspace_size": [_I, _I, _I, _I, _I, _I, _I, _I],
     "wattn_decode": [_P, _I64, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _F, _P, _P, _P, _P, _SZ, _P],
-    "wattn_prompt": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
+    "wattn_prompt_workspace_size": [_I, _I, _I, _I, _I, _I],
+    "wattn_prompt": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _SZ, _P],
     "wmoe_router_topk": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _P],
     "wmoe_topk_scores": [_P, _P, _I, _I, _I, _I, _F, _F, _P, _P, _P],
     "wmoe_router_topk_static": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P],
@@ -85,7 +86,8 @@ SIGNATURES = {
 }
 _RESTYPE = {"w_last_error": ctypes.c_char_p, "wmoe_workspace_size": ctypes.c_size_t,
             "wkv_scores_workspace_size": ctypes.c_size_t, "wmx_linear_workspace_size": ctypes.c_size_t,
-            "wkv_evict_workspace_size": ctypes.c_size_t, "wattn_decode_workspace_size": ctypes.c_size_t}
+            "wkv_evict_workspace_size": ctypes.c_size_t, "wattn_decode_workspace_size": ctypes.c_size_t,
+            "wattn_prompt_workspace_size": ctypes.c_size_t}
 
 _lib = None
 _lock = threading.Lock()

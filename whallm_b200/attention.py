@@ -50,6 +50,11 @@ def _decode_bytes(*shape):
     return L.lib().wattn_decode_workspace_size(*shape)
 
 
+@functools.lru_cache(maxsize=256)
+def _prompt_bytes(*shape):
+    return L.lib().wattn_prompt_workspace_size(*shape)
+
+
 def _at(name, t, dtype, shape, dev):
     """Address of a contiguous tensor of a given type, shape and device (None: 0)."""
     if t is None:
@@ -235,8 +240,10 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     if out is None:
         out = q.new_empty((Tq, Hq, d))
     lse = q.new_empty((Tq, Hq), dtype=_F32) if return_lse else None
+    nbytes = _prompt_bytes(B, Tq, Tk, Hq, Hkv, d)
+    ws = q.new_empty((nbytes,), dtype=_U8) if nbytes else None     # only few rows on many keys need one
     _call("wattn_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
           _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev), _at("cu_seqlens_k", cu_seqlens_k, _INT, (B + 1,), dev), B, Tq,
           Tk, Hq, Hkv, d, scale, 1 if causal else 0, _at("out", out, _BF16, (Tq, Hq, d), dev),
-          lse.data_ptr() if return_lse else None)
+          lse.data_ptr() if return_lse else None, ws.data_ptr() if nbytes else None, nbytes)
     return (out, lse) if return_lse else out

@@ -38,6 +38,10 @@
 // not finite; such values (there are none in a healthy model) are added to the
 // rows that do see them at the end.  The check hides under the step's softmax.
 //
+// Few rows on many keys.  Where the blocks do not fill the GPU their keys are split
+// into parts (find_item), each of which leaves its reference point, sum and
+// unnormalised output in a workspace; a second kernel joins them.
+//
 // Measured (events, back to back): 8192 tokens without a mask, 32/8 heads, D = 64
 // 730 us (750 TF/s), D = 128 845 us (1300 TF/s), 16/2 heads, D = 256 795 us (1380
 // TF/s; cuBLAS sustains 1406 on the same GPU); causal 16384 tokens 1450, 1715 and
@@ -47,6 +51,7 @@
 // last product and the next block's (1 PV, 1.5 output, the rest the first S and
 // its softmax).
 #include <algorithm>
+#include <type_traits>
 
 #include "wm_tc.cuh"
 
@@ -77,7 +82,14 @@ struct PromptArgs {
   float scale2;
   wm_bf16 *out;
   float *lse;
+  // few blocks on long histories: their keys are split, item x leaves its sums in slot x
+  int slots, sms;           // work items at most, 0: no block is split; SMs
+  float *part_o;            // [slots, kRows, D]
+  float2 *part_ml;          // [slots, kRows]: reference point (log2) and sum
 };
+
+constexpr int kLeastTiles = 2;          // key tiles of a part
+constexpr int kSplitKeys = 2048;        // fewer keys in all, or half of it per sequence, are not split
 
 template <int D>
 struct Cfg {
@@ -98,10 +110,11 @@ struct Cfg {
 // One block of packed rows of one (sequence, key-value head).
 struct Item {
   int valid;                // 0: no more work
-  int q0, k0;               // first row and key of the sequence
-  int nq, nk;
+  int q0, k0;               // first row of the sequence, first key of the item
+  int nq, nk, skip;         // rows and keys of the sequence, its keys before the item's
   int h, blk;
   int tiles, first;         // key tiles; the first of them that holds a key some row does not see
+  int part, parts, slot;    // of the block's keys; where the part's sums go
   uint32_t odd[16];         // keys of tiles first .. first + 3 with values that are not finite (128 bits each)
 };
 
@@ -221,7 +234,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void store32(wm_bf16 *p, const uint32_t (&r)[8]) {
+__device__ __forceinline__ void store32(void *p, const uint32_t (&r)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), WM_U8(r, 0) : "memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -290,17 +303,45 @@ __device__ __forceinline__ int read_next(Shared *sh) {
 // Work item number x by one warp: blocks of all sequences from the last block of
 // the last sequence backwards (within a causal sequence the longest first), heads
 // innermost.
-template <int D>
+//
+// SP: blocks are split over their keys, every block of a sequence into the same
+// number of equal parts of at most c key tiles.  With c = (all blocks' tiles) /
+// (SMs - blocks) there are at most as many parts as SMs, in whatever proportions
+// the sequences' lengths stand: one wave.  With more blocks than half of the SMs
+// the divisor stays there: equal blocks are then not split (two waves of halves
+// take as long), and long ones among short ones are cut down to twice the mean load.
+template <int D, bool SP>
 __device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out) {
   using C = Cfg<D>;
   const int lane = threadIdx.x & 31;
+  auto blocks = [&](int nq) { return (static_cast<unsigned>(nq) * static_cast<unsigned>(a.G) + (C::kRows - 1)) / C::kRows; };
+  auto key_tiles = [&](int nk) { return (static_cast<unsigned>(nk) + (C::kN - 1)) / C::kN; };
+  unsigned c = 1u;
+  if constexpr (SP) {
+    int64_t nb = 0, nt = 0;
+    for (int b = x < 0 ? a.B : lane; b < a.B; b += 32) {
+      int q0, nq, k0, nk;
+      seq_bounds(a, b, q0, nq, k0, nk);
+      nb += blocks(nq);
+      nt += static_cast<int64_t>(blocks(nq)) * key_tiles(nk);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      nb += __shfl_xor_sync(0xffffffffu, nb, d);
+      nt += __shfl_xor_sync(0xffffffffu, nt, d);
+    }
+    const int64_t room = max(max(a.sms - nb * a.Hkv, static_cast<int64_t>(a.sms / 2)), static_cast<int64_t>(1));
+    c = static_cast<unsigned>(max((nt * a.Hkv + room - 1) / room, static_cast<int64_t>(kLeastTiles)));
+  }
   unsigned blk = static_cast<unsigned>(x) / static_cast<unsigned>(a.Hkv);
   const int h = static_cast<int>(static_cast<unsigned>(x) - blk * static_cast<unsigned>(a.Hkv));
   for (int hi = x < 0 ? 0 : a.B; hi > 0; hi -= 32) {  // lane l: sequence hi - 1 - l
     const int b = hi - 1 - lane;
     int q0 = 0, nq = 0, k0 = 0, nk = 0;
     if (b >= 0) seq_bounds(a, b, q0, nq, k0, nk);
-    unsigned s = (static_cast<unsigned>(nq) * static_cast<unsigned>(a.G) + (C::kRows - 1)) / C::kRows;
+    unsigned parts = 1u;
+    if constexpr (SP) parts = min(max((key_tiles(nk) + c - 1u) / c, 1u), static_cast<unsigned>(a.slots));
+    unsigned s = blocks(nq) * parts;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const unsigned o = __shfl_up_sync(0xffffffffu, s, d);
@@ -309,19 +350,35 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out)
     const unsigned hit = __ballot_sync(0xffffffffu, s > blk);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
-        const int k = static_cast<int>(s - 1 - blk);  // block within the sequence, last first
+        int k = static_cast<int>(s - 1 - blk);        // block within the sequence, last first
+        unsigned part = 0u;
+        if constexpr (SP) {
+          part = static_cast<unsigned>(k) % parts;
+          k = static_cast<int>(static_cast<unsigned>(k) / parts);
+        }
         const int R0 = k * C::kRows;
         const int R1 = min(R0 + C::kRows, nq * a.G) - 1;
         const int n0 = visible(a, nq, nk, R0), n1 = visible(a, nq, nk, R1);
+        int j0 = 0, j1 = (n1 + C::kN - 1) / C::kN, first = n0 / C::kN;
+        if constexpr (SP) {
+          const unsigned n = static_cast<unsigned>(j1), each = n / parts, more = n % parts;   // the first `more` parts have one more
+          j0 = static_cast<int>(part * each + min(part, more));
+          j1 = j0 + static_cast<int>(each + (part < more ? 1u : 0u));
+          first = max(first - j0, 0);
+        }
         out->valid = 1;
         out->q0 = q0;
-        out->k0 = k0;
+        out->k0 = k0 + j0 * C::kN;
         out->nq = nq;
         out->nk = nk;
+        out->skip = j0 * C::kN;
         out->h = h;
         out->blk = k;
-        out->tiles = (n1 + C::kN - 1) / C::kN;
-        out->first = n0 / C::kN;
+        out->tiles = j1 - j0;
+        out->first = first;
+        out->part = static_cast<int>(part);
+        out->parts = static_cast<int>(parts);
+        out->slot = x;
       }
       if (lane < 16) out->odd[lane] = 0u;
       return;
@@ -331,7 +388,7 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out)
   if (lane == 0) out->valid = 0;                      // x < 0 or past the last block
 }
 
-template <int D>
+template <int D, bool SP>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_prompt(PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v) {
@@ -395,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int sl = it & 1;
         if (!wait(&sh, &bar.item_empty[sl], ((it >> 1) & 1) ^ 1)) break;
         Item *item = &sh.item[sl];
-        find_item<D>(a, x, item);
+        find_item<D, SP>(a, x, item);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.item_full[sl]);
         if (!item->valid) break;
@@ -572,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         Item *item = &sh.item[sl];
         if (!item->valid) break;
-        const int n = item->tiles, first = item->first, nk = item->nk;
+        const int n = item->tiles, first = item->first, nk = item->nk - item->skip;
         const int64_t rows = static_cast<int64_t>(item->nq) * a.G;
         for (int w = 0; ok && w < C::kTiles; ++w) {
           ok = wait(&sh, &bar.q_empty[w], (it & 1) ^ 1);
@@ -666,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int steps = n * C::kTiles;
       const int R = item->blk * C::kRows + (C::kChain ? 0 : w * 128) + r;
       const bool live = R < static_cast<int64_t>(nq) * a.G;
-      const int see = live ? visible(a, nq, nk, R) : 0;
+      const int see = live ? visible(a, nq, nk, R) - item->skip : 0;     // of the item's keys
       float m = kNegInf, l = 0.0f;
 
       for (int s = w; ok && s < steps; s += 2) {
@@ -824,6 +881,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
         }
+        if (SP && item->parts > 1) {
+          uint32_t *dst = reinterpret_cast<uint32_t *>(a.part_o) +
+                          (static_cast<int64_t>(item->slot) * C::kRows + (R - item->blk * C::kRows)) * D + c;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t y[8];
+#pragma unroll
+            for (int z = 0; z < 8; ++z) y[z] = o[8 * e + z];
+            if (live) store32(dst + 8 * e, y);
+          }
+          __syncwarp();
+          continue;
+        }
         // whole 32-byte sectors: 16-byte stores to 32 rows at a time took twice as long
         wm_bf16 *dst = a.out + head * D + c;
 #pragma unroll
@@ -838,7 +908,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();                                 // the TMEM loads are whole-warp instructions
       }
-      if (live && a.lse && (!C::kChain || w == 0)) a.lse[head] = see > 0 ? (m + log2f(l)) * kLn2 : kNegInf;
+      if (SP && item->parts > 1) {
+        if (live && (!C::kChain || w == 0))
+          a.part_ml[static_cast<int64_t>(item->slot) * C::kRows + (R - item->blk * C::kRows)] = make_float2(m, l);
+      } else if (live && a.lse && (!C::kChain || w == 0)) a.lse[head] = see > 0 ? (m + log2f(l)) * kLn2 : kNegInf;
       tc_fence_before();
       mbar_arrive(&bar.o_free);
       __syncwarp();
@@ -849,10 +922,74 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (*reinterpret_cast<volatile int *>(&sh.abort)) { // a wait ran out: no result passes for one
     const int64_t n = static_cast<int64_t>(a.Tq) * a.Hq * D;
     for (int64_t i = tid; i < n; i += kThreads) a.out[i] = 0x7FC0;
+    if constexpr (SP)
+      for (int64_t i = tid; i < static_cast<int64_t>(a.slots) * C::kRows; i += kThreads)
+        a.part_ml[i] = make_float2(0.0f, __uint_as_float(0x7fc00000u));
   }
   if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// The parts of split blocks joined with weights 2^(m_part - m).  A CTA per work
+// item: those of one block share its rows, a warp takes one row at a time.
+constexpr int kJoinThreads = 512;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) k_attn_prompt_join(PromptArgs a) {
+  using C = Cfg<D>;
+  constexpr int kV = D / 32;                          // values of a lane, in pieces of kW
+  constexpr int kW = kV < 4 ? kV : 4;
+  using Piece = typename std::conditional<kW == 2, float2, float4>::type;
+  __shared__ Item item;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  WM_PDL_WAIT();
+  if (warp == 0) find_item<D, true>(a, static_cast<int>(blockIdx.x), &item);
+  __syncthreads();
+  if (!item.valid || item.parts < 2) return;
+  // part y is in slot slot0 - y Hkv; of malformed, overlapping sequences some have no slot
+  const int64_t slot0 = item.slot + static_cast<int64_t>(item.part) * a.Hkv;
+  const int y0 = slot0 < a.slots ? 0 : static_cast<int>((slot0 - a.slots) / a.Hkv) + 1;
+  const int r1 = static_cast<int>(static_cast<int64_t>(C::kRows) * (item.part + 1) / item.parts);
+  for (int r = static_cast<int>(static_cast<int64_t>(C::kRows) * item.part / item.parts) + warp; r < r1; r += kJoinThreads / 32) {
+    const int R = item.blk * C::kRows + r;
+    if (R >= static_cast<int64_t>(item.nq) * a.G) break;
+    auto at = [&](int y) { return (slot0 - static_cast<int64_t>(y) * a.Hkv) * C::kRows + r; };
+    float m = kNegInf;
+    for (int y = y0 + lane; y < item.parts; y += 32) m = fmaxf(m, a.part_ml[at(y)].x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float l = 0.0f, o[kV] = {};
+#pragma unroll 4
+    for (int y = y0; y < item.parts; ++y) {
+      const float2 ml = a.part_ml[at(y)];
+      const Piece *po = reinterpret_cast<const Piece *>(a.part_o + at(y) * D) + lane;
+      // never 0 for a seen part, so that an infinite value shows as such
+      const float f = ml.x == kNegInf ? 0.0f : fmaxf(ex2(ml.x - m), 1.17549435e-38f);
+      l += ml.x == kNegInf ? ml.y : f * ml.y;         // no key of the part seen: 0, or NaN of NaN scores
+#pragma unroll
+      for (int i = 0; i < kV / kW; ++i) {
+        const Piece v = po[32 * i];
+        if (ml.x == kNegInf) continue;
+        o[kW * i] += f * v.x;
+        o[kW * i + 1] += f * v.y;
+        if constexpr (kW == 4) {
+          o[kW * i + 2] += f * v.z;
+          o[kW * i + 3] += f * v.w;
+        }
+      }
+    }
+    const bool sees = visible(a, item.nq, item.nk, R) > 0;
+    const float inv = sees ? 1.0f / l : 0.0f;
+    const int t = R / a.G;
+    const int64_t head = (static_cast<int64_t>(item.q0) + t) * a.Hq + item.h * a.G + (R - t * a.G);
+#pragma unroll
+    for (int i = 0; i < kV / kW; ++i)
+#pragma unroll
+      for (int e = 0; e < kW; e += 2)
+        *reinterpret_cast<uint32_t *>(a.out + head * D + 32 * kW * i + kW * lane + e) =
+            sees ? bf16x2(o[kW * i + e] * inv, o[kW * i + e + 1] * inv) : 0u;
+    if (a.lse && lane == 0) a.lse[head] = sees ? (m + log2f(l)) * kLn2 : kNegInf;
   }
 }
 
@@ -873,6 +1010,39 @@ int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t toke
   return WM_OK;
 }
 
+// Work items of a call without splitting, at most: one partial block per sequence
+// beyond the rows' own blocks.
+int64_t most_items(int B, int Tq, int Hq, int Hkv, int D) {
+  const int rows = D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows;
+  return (static_cast<int64_t>(Tq) * (Hq / Hkv) / rows + B) * Hkv;
+}
+
+// Slots for the parts of split blocks, 0 where none is split.  With fewer blocks
+// than SMs the rest would idle (32/8 heads of 128, us): 64 rows on 32,768 keys 453
+// -> 52, 512 rows 460 -> 257; 16 rows on 4096 keys 63 -> 20, on 2048 36 -> 20; two
+// sequences on 1024 each 22 -> 23, hence the least count.  The join costs 6 us where
+// nothing turns out to be split, so one sequence with more blocks than half of the
+// SMs, which never is, goes without; several may be ragged (16 rows each, 15
+// sequences of 500 and one of 32,768 keys: 453 -> 91; 16 of 2000 to 3500: 61 -> 67).
+int split_slots(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+  const int64_t most = most_items(B, Tq, Hq, Hkv, D), sms = wm::sm_count();
+  if (Tk < kSplitKeys || Tk / (kSplitKeys / 2) < B || 2 * most >= (B == 1 ? sms : 3 * sms)) return 0;
+  return static_cast<int>(std::max(sms, most + sms / 2));
+}
+
+size_t slot_bytes(int D) { return static_cast<size_t>(D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows) * (D + 2) * sizeof(float); }
+
+template <int D, bool SP>
+int launch_as(const PromptArgs &a, int64_t grid, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
+  cudaError_t e = wm::allow_smem<k_attn_prompt<D, SP>>(smem_bytes<D>());
+  if (e == cudaSuccess)
+    e = wm::launch_pdl(k_attn_prompt<D, SP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem_bytes<D>(), stream, a, mq, mk, mv);
+  if constexpr (SP)
+    if (e == cudaSuccess) e = wm::launch_pdl(k_attn_prompt_join<D>, dim3(static_cast<unsigned>(grid)), dim3(kJoinThreads), 0, stream, a);
+  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
+  return wm::check_launch("wattn_prompt");
+}
+
 template <int D>
 int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t stream) {
   using C = Cfg<D>;
@@ -882,24 +1052,24 @@ int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t
   const bool any = a.Tk > 0;
   if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, 1, C::kN)) return rc;
   if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, 1, C::kVKeys)) return rc;
-  // at most one partial block per sequence beyond the rows' own blocks
-  const int64_t most = (static_cast<int64_t>(a.Tq) * a.G / C::kRows + a.B) * a.Hkv;
+  if (a.slots) return launch_as<D, true>(a, a.slots, mq, mk, mv, stream);
+  const int64_t most = most_items(a.B, a.Tq, a.Hq, a.Hkv, D);
   WM_REQUIRE(most <= INT32_MAX, "prompt attention: too many rows");
-  const int grid = static_cast<int>(std::max<int64_t>(most, 1));
-  const cudaError_t e = wm::allow_smem<k_attn_prompt<D>>(smem_bytes<D>());
-  if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
-  const cudaError_t l = wm::launch_pdl(k_attn_prompt<D>, dim3(grid), dim3(kThreads), smem_bytes<D>(), stream, a, mq, mk, mv);
-  if (l != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(l));
-  return wm::check_launch("wattn_prompt");
+  return launch_as<D, false>(a, std::max<int64_t>(most, 1), mq, mk, mv, stream);
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t wattn_prompt_workspace_size(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
+  if (B <= 0 || Tq <= 0 || Tk < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128 && D != 256)) return 0;
+  return split_slots(B, Tq, Tk, Hq, Hkv, D) * slot_bytes(D);
+}
+
 int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                  const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int B, int Tq, int Tk, int Hq, int Hkv, int D,
-                 float scale, int causal, wm_bf16 *out, float *lse, wm_stream_t stream) {
+                 float scale, int causal, wm_bf16 *out, float *lse, void *workspace, size_t ws_bytes, wm_stream_t stream) {
   wm::clear_error();
   WM_REQUIRE(B >= 0 && Tq >= 0 && Tk >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0,
              "prompt attention: the query heads must be a multiple of the key-value heads");
@@ -912,8 +1082,13 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
                  wm::aligned(q, 16) && wm::aligned(k, 16) && wm::aligned(v, 16) && wm::aligned(out, 32),
              "prompt attention: token rows must be 16-byte aligned and hold their heads, the output 32-byte aligned");
   WM_REQUIRE(static_cast<int64_t>(Tq) * (Hq / Hkv) <= INT32_MAX - 256, "prompt attention: too many rows per key-value head");
+  const int slots = split_slots(B, Tq, Tk, Hq, Hkv, D);
+  if (ws_bytes < slots * slot_bytes(D)) return wm::fail(WM_ERR_WORKSPACE, "prompt attention: workspace too small");
+  WM_REQUIRE(slots == 0 || (workspace && wm::aligned(workspace, 256)), "prompt attention: the workspace must be 256-byte aligned");
+  float *ws = static_cast<float *>(workspace);
+  const int64_t sums = static_cast<int64_t>(slots) * (D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows);
   const PromptArgs a{q, v, q_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, Hq / Hkv, causal,
-                     128 % (Hq / Hkv) == 0, scale * kLog2e, out, lse};
+                     128 % (Hq / Hkv) == 0, scale * kLog2e, out, lse, slots, wm::sm_count(), ws, slots ? reinterpret_cast<float2 *>(ws + sums * D) : nullptr};
   if (D == 64) return launch<64>(a, k, k_stride, stream);
   if (D == 128) return launch<128>(a, k, k_stride, stream);
   return launch<256>(a, k, k_stride, stream);
