@@ -533,6 +533,18 @@ def test_prompt_few_rows_on_many_keys(dev, D, nq, nk, Hq, Hkv):
     run_prompt(dev, nq, nk, Hq, Hkv, D, seed=40 + D)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nq,nk,Hq,Hkv", [
+    ([32] * 20, [700 + 3 * i for i in range(20)], 8, 2),                 # one full tile each, several keys' tiles
+    ([1] * 30 + [400], [300] * 30 + [900], 12, 3),                       # a long one among single rows: several blocks
+    ([5, 0, 1, 33, 2], [5, 9, 0, 33, 128], 7, 1),                        # q not by TMA; no rows, no keys
+    ([100] * 150, [129] * 150, 1, 1),                                    # more blocks than SMs
+])
+def test_prompt_one_tile_blocks(dev, D, nq, nk, Hq, Hkv):
+    run_prompt(dev, nq, nk, Hq, Hkv, D, seed=50 + D)
+    run_prompt(dev, nq, nk, Hq, Hkv, D, causal=False, seed=51 + D)
+
+
 def test_prompt_split_full_and_many_sequences(dev):
     run_prompt(dev, [5, 129], [6000, 4097], 4, 1, 128, causal=False, seed=41)
     nq = [3] * 40                                                        # more sequences than a warp's lanes

@@ -17,9 +17,10 @@
 // of two TMEM buffers; a softmax warpgroup, one thread per row, reads its row,
 // writes P = exp2(S scale log2e - m) as bf16 over S; O += P V with P from TMEM.
 // Up to D = 128 the block has two tiles of 128 rows and step s works on tile
-// s & 1 (two softmax warpgroups in turn, each with its own O); at D = 256 TMEM
-// holds one O of 256 columns, the block has one tile, step s takes the s-th key
-// tile and the two warpgroups hand the running maximum to each other.
+// s & 1 (two softmax warpgroups in turn, each with its own O).  At D = 256, where
+// TMEM holds one O of 256 columns, and for sequences of few rows the block has one
+// tile, step s takes the s-th key tile and the two warpgroups hand the running
+// maximum to each other.
 // The MMA warp issues PV(s), S(s + 2), PV(s + 1), ...: instructions of one thread
 // execute in order, so S(s + 2) may overwrite the buffer that PV(s) read.
 //
@@ -91,15 +92,16 @@ struct PromptArgs {
 constexpr int kLeastTiles = 2;          // key tiles of a part
 constexpr int kSplitKeys = 2048;        // fewer keys in all, or half of it per sequence, are not split
 
-template <int D>
+// ONE: one tile of 128 rows, which the warpgroups share, in place of two
+template <int D, bool ONE>
 struct Cfg {
-  static constexpr bool kChain = D == 256;            // one tile, the warpgroups share its rows
+  static constexpr bool kChain = ONE;
   static constexpr int kTiles = kChain ? 1 : 2;       // 128-row tiles of a block
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kN = 128;                      // keys of a tile
   static constexpr int kQBytes = kRows * D * 2;
   // K and V tiles come in pieces of one slot: at D = 256 two, half of the dimensions of K or half of the keys of V
-  static constexpr int kParts = kChain ? 2 : 1;
+  static constexpr int kParts = D == 256 ? 2 : 1;
   static constexpr int kSlot = kN * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 5;
   static constexpr int kKDims = D / kParts, kVKeys = kN / kParts;
@@ -138,9 +140,9 @@ struct Shared {
 
 // The tiles need 1024-byte alignment: the kernel has no static shared memory, so
 // its dynamic part begins at such an address (else the call ends with NaN).
-template <int D>
-constexpr int smem_bytes() { return Cfg<D>::kQBytes + Cfg<D>::kSlots * Cfg<D>::kSlot + static_cast<int>(sizeof(Shared)); }
-static_assert(smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "shared memory of a CTA");
+template <int D, bool ONE>
+constexpr int smem_bytes() { return Cfg<D, ONE>::kQBytes + Cfg<D, ONE>::kSlots * Cfg<D, ONE>::kSlot + static_cast<int>(sizeof(Shared)); }
+static_assert(smem_bytes<128, false>() <= 232448 && smem_bytes<128, true>() <= 232448 && smem_bytes<256, true>() <= 232448, "shared memory of a CTA");
 
 // try_wait without a suspend hint: with the hint of the other kernels' waits a
 // warp saw a completed phase 400 to 500 cycles late, which is on the critical
@@ -270,8 +272,8 @@ __device__ __forceinline__ void seq_bounds(const PromptArgs &a, int b, int &q0, 
 
 // Position of value tile j among the 2 n tiles of an item, which come in the order
 // in which the MMA warp needs them.
-template <int D>
-__device__ __forceinline__ int pos_v(int j, int n) { return Cfg<D>::kChain ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; }
+template <bool ONE>
+__device__ __forceinline__ int pos_v(int j, int n) { return ONE ? (j == n - 1 ? 2 * n - 1 : 2 * j + 2) : 2 * j + 1; }
 
 // Work items are the blocks of the grid: a CTA that has started its item asks the
 // hardware for a block that has not been launched yet and takes its number over
@@ -310,9 +312,9 @@ __device__ __forceinline__ int read_next(Shared *sh) {
 // the sequences' lengths stand: one wave.  With more blocks than half of the SMs
 // the divisor stays there: equal blocks are then not split (two waves of halves
 // take as long), and long ones among short ones are cut down to twice the mean load.
-template <int D, bool SP>
+template <int D, bool ONE, bool SP>
 __device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out) {
-  using C = Cfg<D>;
+  using C = Cfg<D, ONE>;
   const int lane = threadIdx.x & 31;
   auto blocks = [&](int nq) { return (static_cast<unsigned>(nq) * static_cast<unsigned>(a.G) + (C::kRows - 1)) / C::kRows; };
   auto key_tiles = [&](int nk) { return (static_cast<unsigned>(nk) + (C::kN - 1)) / C::kN; };
@@ -388,11 +390,11 @@ __device__ __forceinline__ void find_item(const PromptArgs &a, int x, Item *out)
   if (lane == 0) out->valid = 0;                      // x < 0 or past the last block
 }
 
-template <int D, bool SP>
+template <int D, bool ONE, bool SP>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_prompt(PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v) {
-  using C = Cfg<D>;
+  using C = Cfg<D, ONE>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Shared &sh = *reinterpret_cast<Shared *>(smem + C::kQBytes + C::kSlots * C::kSlot);
   const uint32_t q_s = smem_u32(smem), kv_s = q_s + C::kQBytes;
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int sl = it & 1;
         if (!wait(&sh, &bar.item_empty[sl], ((it >> 1) & 1) ^ 1)) break;
         Item *item = &sh.item[sl];
-        find_item<D, SP>(a, x, item);
+        find_item<D, ONE, SP>(a, x, item);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.item_full[sl]);
         if (!item->valid) break;
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma_ts(o, p + kp * 8, vb + kv * (2048 >> 4), id_o, (j | kp) != 0);
               }
               if (half == 1 && (C::kChain || s >= steps - 2)) tc_commit(&bar.o_done[buf]);
-              if (C::kChain || (half == 1 && w == 1)) tc_commit(&bar.kv_empty[at.slot]);
+              if (C::kParts == 2 || (half == 1 && (C::kChain || w == 1))) tc_commit(&bar.kv_empty[at.slot]);
             }
             __syncwarp();
           }
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int y = first * C::kParts; ok && y < n * C::kParts; ++y) {
           const int j = y / C::kParts, part = y % C::kParts;
-          const int slot = static_cast<int>((g0 + pos_v<D>(j, n) * C::kParts + part) % C::kSlots);
+          const int slot = static_cast<int>((g0 + pos_v<ONE>(j, n) * C::kParts + part) % C::kSlots);
           ok = wait(&sh, &bar.v_edge[slot], (edge_ph >> slot) & 1u);
           if (!ok) break;
           edge_ph ^= 1u << slot;
@@ -935,16 +937,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 // The parts of split blocks joined with weights 2^(m_part - m).  A CTA per work
 // item: those of one block share its rows, a warp takes one row at a time.
 constexpr int kJoinThreads = 512;
-template <int D>
+template <int D, bool ONE>
 __global__ void __launch_bounds__(kJoinThreads) k_attn_prompt_join(PromptArgs a) {
-  using C = Cfg<D>;
+  using C = Cfg<D, ONE>;
   constexpr int kV = D / 32;                          // values of a lane, in pieces of kW
   constexpr int kW = kV < 4 ? kV : 4;
   using Piece = typename std::conditional<kW == 2, float2, float4>::type;
   __shared__ Item item;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   WM_PDL_WAIT();
-  if (warp == 0) find_item<D, true>(a, static_cast<int>(blockIdx.x), &item);
+  if (warp == 0) find_item<D, ONE, true>(a, static_cast<int>(blockIdx.x), &item);
   __syncthreads();
   if (!item.valid || item.parts < 2) return;
   // part y is in slot slot0 - y Hkv; of malformed, overlapping sequences some have no slot
@@ -1010,52 +1012,64 @@ int make_map3(CUtensorMap *map, const void *base, int D, int heads, int64_t toke
   return WM_OK;
 }
 
+// Rows of a block.  D = 256 has TMEM for one tile.  At D = 64 and 128 a block takes
+// one tile where the sequences' rows fill no more than that on average: the second
+// tile's products would be wasted.
+// Two tiles -> one (32/8 heads of 128, us): 37 sequences of 32 rows on 4096 keys 151
+// -> 107, 32 of 4 rows on 4000 and one of 512 190 -> 123; at 64 rows of 4 heads each
+// on their own keys 17 -> 21, 8 sequences of 2048 289 -> 392, as K and V are read
+// twice as often and each step waits for one softmax.
+int block_rows(int B, int Tq, int Hq, int Hkv, int D) {
+  return D == 256 || static_cast<int64_t>(Tq) * (Hq / Hkv) <= 128ll * B ? 128 : 256;
+}
+
 // Work items of a call without splitting, at most: one partial block per sequence
 // beyond the rows' own blocks.
 int64_t most_items(int B, int Tq, int Hq, int Hkv, int D) {
-  const int rows = D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows;
-  return (static_cast<int64_t>(Tq) * (Hq / Hkv) / rows + B) * Hkv;
+  return (static_cast<int64_t>(Tq) * (Hq / Hkv) / block_rows(B, Tq, Hq, Hkv, D) + B) * Hkv;
 }
 
 // Slots for the parts of split blocks, 0 where none is split.  With fewer blocks
 // than SMs the rest would idle (32/8 heads of 128, us): 64 rows on 32,768 keys 453
-// -> 52, 512 rows 460 -> 257; 16 rows on 4096 keys 63 -> 20, on 2048 36 -> 20; two
-// sequences on 1024 each 22 -> 23, hence the least count.  The join costs 6 us where
+// -> 52, 512 rows 460 -> 257; 16 rows on 4096 keys 63 -> 19, on 2048 36 -> 17; two
+// sequences on 1024 each 22 -> 19, hence the least count.  The join costs 6 us where
 // nothing turns out to be split, so one sequence with more blocks than half of the
 // SMs, which never is, goes without; several may be ragged (16 rows each, 15
-// sequences of 500 and one of 32,768 keys: 453 -> 91; 16 of 2000 to 3500: 61 -> 67).
+// sequences of 500 and one of 32,768 keys: 453 -> 63).
 int split_slots(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   const int64_t most = most_items(B, Tq, Hq, Hkv, D), sms = wm::sm_count();
   if (Tk < kSplitKeys || Tk / (kSplitKeys / 2) < B || 2 * most >= (B == 1 ? sms : 3 * sms)) return 0;
   return static_cast<int>(std::max(sms, most + sms / 2));
 }
 
-size_t slot_bytes(int D) { return static_cast<size_t>(D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows) * (D + 2) * sizeof(float); }
 
-template <int D, bool SP>
+size_t slot_bytes(int rows, int D) { return static_cast<size_t>(rows) * (D + 2) * sizeof(float); }
+
+template <int D, bool ONE, bool SP>
 int launch_as(const PromptArgs &a, int64_t grid, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
-  cudaError_t e = wm::allow_smem<k_attn_prompt<D, SP>>(smem_bytes<D>());
+  cudaError_t e = wm::allow_smem<k_attn_prompt<D, ONE, SP>>(smem_bytes<D, ONE>());
   if (e == cudaSuccess)
-    e = wm::launch_pdl(k_attn_prompt<D, SP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem_bytes<D>(), stream, a, mq, mk, mv);
+    e = wm::launch_pdl(k_attn_prompt<D, ONE, SP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem_bytes<D, ONE>(), stream, a, mq, mk,
+                       mv);
   if constexpr (SP)
-    if (e == cudaSuccess) e = wm::launch_pdl(k_attn_prompt_join<D>, dim3(static_cast<unsigned>(grid)), dim3(kJoinThreads), 0, stream, a);
+    if (e == cudaSuccess) e = wm::launch_pdl(k_attn_prompt_join<D, ONE>, dim3(static_cast<unsigned>(grid)), dim3(kJoinThreads), 0, stream, a);
   if (e != cudaSuccess) return wm::fail(WM_ERR_CUDA, std::string("wattn_prompt: ") + cudaGetErrorString(e));
   return wm::check_launch("wattn_prompt");
 }
 
-template <int D>
+template <int D, bool ONE>
 int launch(const PromptArgs &a, const wm_bf16 *k, int64_t k_stride, cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, ONE>;
   CUtensorMap mq, mk, mv;
   if (int rc = make_map3(&mq, a.q, D, a.Hq, a.Tq, a.q_stride, a.q_tma ? a.G : 1, a.q_tma ? 128 / a.G : 128)) return rc;
   // without keys no tile is loaded; the maps then describe one row of q
   const bool any = a.Tk > 0;
   if (int rc = make_map3(&mk, any ? k : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? k_stride : D, 1, C::kN)) return rc;
   if (int rc = make_map3(&mv, any ? a.v : a.q, D, any ? a.Hkv : 1, any ? a.Tk : 1, any ? a.v_stride : D, 1, C::kVKeys)) return rc;
-  if (a.slots) return launch_as<D, true>(a, a.slots, mq, mk, mv, stream);
+  if (a.slots) return launch_as<D, ONE, true>(a, a.slots, mq, mk, mv, stream);
   const int64_t most = most_items(a.B, a.Tq, a.Hq, a.Hkv, D);
   WM_REQUIRE(most <= INT32_MAX, "prompt attention: too many rows");
-  return launch_as<D, false>(a, std::max<int64_t>(most, 1), mq, mk, mv, stream);
+  return launch_as<D, ONE, false>(a, std::max<int64_t>(most, 1), mq, mk, mv, stream);
 }
 
 }  // namespace
@@ -1064,7 +1078,7 @@ extern "C" {
 
 size_t wattn_prompt_workspace_size(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   if (B <= 0 || Tq <= 0 || Tk < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128 && D != 256)) return 0;
-  return split_slots(B, Tq, Tk, Hq, Hkv, D) * slot_bytes(D);
+  return split_slots(B, Tq, Tk, Hq, Hkv, D) * slot_bytes(block_rows(B, Tq, Hq, Hkv, D), D);
 }
 
 int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -1083,15 +1097,17 @@ int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q
              "prompt attention: token rows must be 16-byte aligned and hold their heads, the output 32-byte aligned");
   WM_REQUIRE(static_cast<int64_t>(Tq) * (Hq / Hkv) <= INT32_MAX - 256, "prompt attention: too many rows per key-value head");
   const int slots = split_slots(B, Tq, Tk, Hq, Hkv, D);
-  if (ws_bytes < slots * slot_bytes(D)) return wm::fail(WM_ERR_WORKSPACE, "prompt attention: workspace too small");
+  const int rows = block_rows(B, Tq, Hq, Hkv, D);
+  if (ws_bytes < slots * slot_bytes(rows, D)) return wm::fail(WM_ERR_WORKSPACE, "prompt attention: workspace too small");
   WM_REQUIRE(slots == 0 || (workspace && wm::aligned(workspace, 256)), "prompt attention: the workspace must be 256-byte aligned");
   float *ws = static_cast<float *>(workspace);
-  const int64_t sums = static_cast<int64_t>(slots) * (D == 256 ? Cfg<256>::kRows : Cfg<128>::kRows);
+  const int64_t sums = static_cast<int64_t>(slots) * rows;
   const PromptArgs a{q, v, q_stride, v_stride, cu_seqlens_q, cu_seqlens_k, B, Tq, Tk, Hq, Hkv, Hq / Hkv, causal,
                      128 % (Hq / Hkv) == 0, scale * kLog2e, out, lse, slots, wm::sm_count(), ws, slots ? reinterpret_cast<float2 *>(ws + sums * D) : nullptr};
-  if (D == 64) return launch<64>(a, k, k_stride, stream);
-  if (D == 128) return launch<128>(a, k, k_stride, stream);
-  return launch<256>(a, k, k_stride, stream);
+  const bool one = rows == 128;
+  if (D == 64) return one ? launch<64, true>(a, k, k_stride, stream) : launch<64, false>(a, k, k_stride, stream);
+  if (D == 128) return one ? launch<128, true>(a, k, k_stride, stream) : launch<128, false>(a, k, k_stride, stream);
+  return launch<256, true>(a, k, k_stride, stream);
 }
 
 }  // extern "C"
