@@ -222,7 +222,8 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     ``cu_seqlens_k`` is given, keys of their own; causal row i of nq then sees the
     keys up to i + nk - nq (a prompt that continues a history).  Tokens may be
     strided (slices of one projection).  A row that sees no key gets zeros (lse
-    -inf); rows outside every sequence are not written."""
+    -inf); rows outside every sequence are not written.  Equal calls give equal
+    bits; how a sequence's keys are summed may depend on the batch around it."""
     dev = q.get_device()
     Tq, Hq, d, qs = _tokens("q", q, None, None, None)
     Tk, Hkv, _, ks = _tokens("k", k, None, d, dev)
