@@ -1,0 +1,56 @@
+"""Attention over scores, sums and scales at the ends of their ranges, vs 64-bit results.
+
+The bounds are those of test_gpu_attention.  A key whose score is minus infinity
+weighs nothing, so its reference is the same call without that key.
+"""
+import numpy as np
+import pytest
+import torch
+
+import whallm_b200 as W
+from oracle import attention as A
+from tests.test_gpu_attention import Cache, check_lse, check_mass, check_out, f64, gen, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+def forbid(c, b, keys):
+    """Give keys of sequence b a first block of dimensions whose score with a negative query is minus infinity in 32
+    bits: an infinite component in bf16 rows, the largest e4m3 values under the largest scale in the others."""
+    dev = c.k.device
+    e = torch.tensor(keys)
+    at, slot = c.table.cpu()[b][e // c.page].long().to(dev), (e % c.page).to(dev)
+    if c.fmt == "bf16":
+        c.k[at, :, slot, 5] = float("inf")
+    else:
+        c.k[at, :, slot, :32] = 0x7e                                     # 448
+        c.ks[at, :, slot, 0] = 254 if c.fmt == "mxfp8" else 3e38         # 448 x 32 x 2^127 is behind 2^128
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp8_f32_b64", "mxfp8"])
+@pytest.mark.parametrize("D,G", [(64, 2), (128, 4), (256, 12), (128, 17)])
+@pytest.mark.parametrize("max_pages,mass", [(None, False), (200, False), (None, True)])
+def test_decode_keys_of_minus_infinity(dev, fmt, D, G, max_pages, mass):
+    # single keys at a tile's start and end, a tile's only key, whole tiles and units, all but the last key; over a
+    # cluster and over the line
+    lens = [17, 33, 2, 200, 1000, 130, 65, 64]
+    dead = [[16], [32], [0], range(16), [*range(0, 400), 999], [*range(0, 64), *range(80, 96), 128, 129], range(64),
+            [*range(16, 32), 63]]
+    Hkv = 2
+    c = Cache(dev, lens, Hkv, D, 64, fmt, seed=D + G, max_pages=max_pages)
+    for b, keys in enumerate(dead):
+        forbid(c, b, list(keys))
+    q = rnd(gen(7, dev), len(lens), G * Hkv, D, std=2.0, dev=dev)
+    q[:, :, :64] = -q[:, :, :64].abs() - 0.25
+    m = torch.rand((len(lens), Hkv, c.width * 64), generator=gen(8, dev), device=dev) if mass else None
+    before = m.clone() if mass else None
+    out, lse = W.decode_attention(q, *c.args, mass=m, return_lse=True)
+    for b, n in enumerate(lens):
+        live = [j for j in range(n) if j not in set(dead[b])]
+        ref = A.attend(f64(q[b:b + 1]), *(x[live] for x in c.rows[b]), D ** -0.5)
+        check_out(out[b:b + 1], ref, D)
+        check_lse(lse[b:b + 1], ref, D)
+        if mass:
+            check_mass(f64(m[b, :, live]), ref, D, f64(before[b, :, live]))
+            gone = list(dead[b])
+            assert torch.equal(m[b, :, gone], before[b, :, gone])

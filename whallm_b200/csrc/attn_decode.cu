@@ -510,10 +510,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       }
 #pragma unroll
       for (int nh = 0; nh < NH; ++nh) {
-        s[nh][0] = ex2(s[nh][0] - m[nh][0]);
-        s[nh][1] = ex2(s[nh][1] - m[nh][1]);
-        s[nh][2] = ex2(s[nh][2] - m[nh][0]);
-        s[nh][3] = ex2(s[nh][3] - m[nh][1]);
+        // while every score so far is -inf the weights are 2^-inf, not 2^(-inf + inf)
+        const float m0 = m[nh][0] == kNegInf ? 0.0f : m[nh][0], m1 = m[nh][1] == kNegInf ? 0.0f : m[nh][1];
+        s[nh][0] = ex2(s[nh][0] - m0);
+        s[nh][1] = ex2(s[nh][1] - m1);
+        s[nh][2] = ex2(s[nh][2] - m0);
+        s[nh][3] = ex2(s[nh][3] - m1);
         l[nh][0] += s[nh][0] + s[nh][2];
         l[nh][1] += s[nh][1] + s[nh][3];
       }
