@@ -276,7 +276,8 @@ WM_API int wkv_paged_append(const wm_bf16 *k, const wm_bf16 *v, int64_t k_stride
  * updated in place (mass_out == mass and positions_out == positions) or written
  * to arrays of their own; lengths_out [B] (not lengths) gets min(length, budget).
  * A sequence with a length or a page id out of range is left as it is.  Pages
- * shared between sequences must not be evicted from.  Workspace:
+ * shared between sequences must not be evicted from.  The capacity and one page
+ * must stay 8192 entries below 2^31.  Workspace:
  * wkv_evict_workspace_size(B, Hkv, min(budget, capacity)). */
 WM_API size_t wkv_evict_workspace_size(int B, int Hkv, int budget);
 WM_API int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k_scales, void *v_scales, int fmt,

@@ -198,3 +198,13 @@ def test_paged_cache_refusals():
         c.append(x, x)
     assert c.offsets == [0, 0]                   # the refused call added no entry
     assert c.lengths.tolist() == [0, 0] and c.seen.tolist() == [0, 0]
+
+
+def test_evict_refuses_what_32_bits_cannot_count():
+    """The eviction kernel's indexes run past the last entry by up to a round of loads or a page, in 32 bits."""
+    f, big = "wkv_paged_evict", dict(bytes=1 << 60)
+    expect(f, evict_args(page=16, width=(1 << 27) - 1, **big), "below 2^31")        # 2^31 - 16 entries
+    expect(f, evict_args(page=16, width=(1 << 27) - 512, **big), "below 2^31")
+    expect(f, evict_args(page=(1 << 30) + 16, width=1, **big), "below 2^31")        # length + page - 1 behind 2^31
+    expect(f, evict_args(page=16, width=(1 << 27) - 514, mass=None, **big), "missing array")     # the most that is taken
+    expect(f, evict_args(page=1 << 29, width=2, mass=None, **big), "missing array")

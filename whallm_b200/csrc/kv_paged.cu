@@ -141,6 +141,10 @@ constexpr int kBins = 256;         // bins of a digit
 constexpr int kKeySmem = 40960;    // keys held per CTA (160 KB); longer slices read them again
 constexpr int kTableSmem = 2048;   // page numbers held per CTA
 constexpr int kMoveCtas = 4;       // CTAs per SM of the move kernel
+constexpr int kBatch = 4;          // loads in flight per thread
+constexpr int kMostCtas = 8;       // CTAs of a cluster
+constexpr int kPastEnd = 8192;     // an index runs less than this past the last entry
+static_assert(kMostCtas * kET <= kPastEnd && 2 * kBatch * kET <= kPastEnd, "evict: indexes past the end");
 
 struct EvictArgs {
   Pool pool;
@@ -306,7 +310,6 @@ __global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
   auto key_at = [&](int i) { return held ? sk[i - s0] : evict_key(mass[i], pos[i], from, a.sinks); };
   if (tid < kBins) hist[0][tid] = 0u;
   __syncthreads();
-  constexpr int kBatch = 4;                            // loads in flight per thread
   for (int i0 = s0; i0 < s1; i0 += kBatch * kET) {
     float m[kBatch];
     int32_t p[kBatch];
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(kET) k_paged_evict(EvictArgs a) {
   };
   // ranks: each thread walks a run of consecutive entries
   const int E = (s1 - s0 + kET - 1) / kET;
-  const int r0 = min(s0 + tid * E, s1), r1 = min(r0 + E, s1);
+  const int r0 = min(s0 + tid * E, s1), r1 = r0 + min(E, s1 - r0);
   int ties = 0;
   for (int i = r0; i < r1; ++i) ties += key_at(i) == prefix;
   int total, before, all, tie0 = block_scan(ties, warp_sums, &total);
@@ -484,11 +487,13 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   if (int rc = wm_paged::check_pool(pool, B, D, fmt)) return rc;
   WM_REQUIRE(budget > 0 && recent >= 0 && sinks >= 0 && static_cast<int64_t>(recent) + sinks <= budget,
              "evict: the budget must be positive and hold the recent and the first positions");
+  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
+  // the kernel counts entries in 32 bits: its indexes run up to a round of all threads' loads, or a page, past the last one
+  WM_REQUIRE(cap + page_size + kPastEnd <= INT32_MAX, "evict: the capacity and a page must stay 8192 entries below 2^31");
   if (B == 0) return WM_OK;
   WM_REQUIRE(lengths && seen && mass && positions && mass_out && positions_out && lengths_out, "evict: missing array");
   WM_REQUIRE(lengths_out != lengths, "evict: the new lengths need an array of their own");
   WM_REQUIRE((mass_out == mass) == (positions_out == positions), "evict: weights and positions are both in place or both not");
-  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
   const int n = static_cast<int>(std::min<int64_t>(budget, std::max<int64_t>(cap, 1)));
   if (ws_bytes < wkv_evict_workspace_size(B, Hkv, n)) return wm::fail(WM_ERR_WORKSPACE, "evict: workspace too small");
   WM_REQUIRE(workspace && wm::aligned(workspace, 8), "evict: the workspace must be 8-byte aligned");
@@ -496,7 +501,7 @@ int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, void *k
   // CTAs per (sequence, head): enough to fill the GPU, at least 2048 entries each, at most a portable cluster; up
   // to 4096 entries one CTA, whose barriers are cheaper than a cluster's and which needs no second launch
   int C = 1;
-  while (cap > 4096 && C < 8 && heads * C * 2 <= 2 * wm::sm_count() && cap > 2048 * C) C *= 2;
+  while (cap > 4096 && C < kMostCtas && heads * C * 2 <= 2 * wm::sm_count() && cap > 2048 * C) C *= 2;
   const int64_t slice = ((cap + C - 1) / C + 3) & ~int64_t{3};
   const int key_cap = static_cast<int>(std::min<int64_t>(slice, kKeySmem));
   const size_t smem = static_cast<size_t>(key_cap) * 4;
