@@ -54,3 +54,25 @@ def test_decode_keys_of_minus_infinity(dev, fmt, D, G, max_pages, mass):
             check_mass(f64(m[b, :, live]), ref, D, f64(before[b, :, live]))
             gone = list(dead[b])
             assert torch.equal(m[b, :, gone], before[b, :, gone])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("nq,nk,Hq,Hkv", [
+    ([4], [256], 8, 2), ([4, 3], [257, 390], 4, 1),                      # blocks of one tile
+    ([300], [256], 4, 4), ([300, 140], [256, 384], 8, 4),                # blocks of two
+    ([4], [4096], 4, 2), ([300], [5000], 2, 2),                          # keys in parts
+])
+@pytest.mark.parametrize("tile", [0, 1])
+def test_prompt_tile_of_nan_keys(dev, D, nq, nk, Hq, Hkv, tile):
+    """128 keys of NaN, before or behind finite ones: the rows that see them are NaN, their lse too."""
+    g = gen(60 + D, dev)
+    q, k, v = rnd(g, sum(nq), Hq, D, dev=dev), rnd(g, sum(nk), Hkv, D, dev=dev), rnd(g, sum(nk), Hkv, D, dev=dev)
+    at = 0
+    for n in nk:
+        k[at + 128 * tile:at + 128 * (tile + 1), 0] = float("nan")
+        at += n
+    cu = lambda n: torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=dev)  # noqa: E731
+    out, lse = W.prompt_attention(q, k, v, cu(nq), cu(nk), causal=False, return_lse=True)
+    G = Hq // Hkv
+    assert torch.isnan(out[:, :G]).all() and torch.isnan(lse[:, :G]).all()
+    assert torch.isfinite(out[:, G:]).all() and torch.isfinite(lse[:, G:]).all()

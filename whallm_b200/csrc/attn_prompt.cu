@@ -841,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if (steps > 0) {
           const float ml = *reinterpret_cast<volatile float *>(&sh.m[r]);
-          if (m != ml) l = m == kNegInf ? 0.0f : l * ex2(m - ml);
+          if (m != ml) l *= m == kNegInf ? 0.0f : ex2(m - ml);          // a sum of NaN scores stays NaN
           m = ml;
         }
         sh.l[w][r] = l;
