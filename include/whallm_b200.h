@@ -314,6 +314,8 @@ WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int H
  * tokens, a continuation also its history; else all nk keys.  out bf16
  * [Tq, Hq, D]; lse float32 [Tq, Hq] or NULL (natural logarithm).  A row that sees
  * no key gets zeros and lse -inf; rows outside every sequence are not written.
+ * The kernel's waits are bounded (2 s); a call in which one runs out fills the
+ * whole of out and lse with NaN, rows outside every sequence included.
  * D is 64, 128 or 256.  Workspace: wattn_prompt_workspace_size (0 unless few rows
  * meet many keys, which are then split over the GPU); calls that share one must
  * not overlap.  */

@@ -1,12 +1,15 @@
 """Argument checks of the attention and paged-cache calls, and the paged cache's
 host side, without a GPU: every refusal comes before any CUDA call."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
 
 import whallm_b200 as W
 from whallm_b200 import _lib as L
+from whallm_b200 import build
 
 P = ctypes.c_void_p(1 << 20)          # an aligned address that no refused call touches
 ODD = ctypes.c_void_p((1 << 20) + 2)
@@ -208,3 +211,28 @@ def test_evict_refuses_what_32_bits_cannot_count():
     expect(f, evict_args(page=(1 << 30) + 16, width=1, **big), "below 2^31")        # length + page - 1 behind 2^31
     expect(f, evict_args(page=16, width=(1 << 27) - 514, mass=None, **big), "missing array")     # the most that is taken
     expect(f, evict_args(page=1 << 29, width=2, mass=None, **big), "missing array")
+
+
+def test_a_wait_that_ran_out_leaves_nan(tmp_path):
+    """What the prompt kernel does when a bounded wait runs out, compiled for the host: every element of the output, the
+    log-sum-exp and the parts' sums is NaN, none beyond them is touched, and absent arrays are left alone."""
+    src = tmp_path / "giveup.cu"
+    src.write_text('#include "wm_giveup.cuh"\n'
+                   'extern "C" void poison(void *o, long n, void *l, long nl, void *p, long np, int first, int step) {\n'
+                   '  wm_giveup::poison((uint16_t *)o, n, (float *)l, nl, (float2 *)p, np, first, step);\n}\n')
+    lib = tmp_path / "giveup.so"
+    subprocess.run([build.NVCC, "-I", build.CSRC, "-Xcompiler", "-fPIC", "-shared", "-o", str(lib), str(src)], check=True)
+    poison = ctypes.CDLL(str(lib)).poison
+    out, lse, parts = torch.zeros(103, dtype=torch.bfloat16), torch.zeros(17), torch.zeros((9, 2))
+    at = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    n = ctypes.c_long
+    for t in range(4):
+        poison(at(out), n(100), None, n(16), None, n(8), t, 4)
+    assert torch.isnan(out[:100]).all() and (out[100:] == 0).all() and (lse == 0).all() and (parts == 0).all()
+    for t in range(4):
+        poison(at(out), n(0), at(lse), n(16), at(parts), n(8), t, 4)
+    assert torch.isnan(lse[:16]).all() and lse[16] == 0
+    assert torch.isnan(parts[:8, 1]).all() and (parts[:8, 0] == 0).all() and (parts[8] == 0).all()
+    # and the prompt kernel hands it all three
+    text = open(os.path.join(build.CSRC, "attn_prompt.cu")).read()
+    assert "poison(a.out, heads * D, a.lse, heads, SP ? a.part_ml : nullptr" in text

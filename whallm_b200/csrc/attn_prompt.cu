@@ -54,6 +54,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "wm_giveup.cuh"
 #include "wm_tc.cuh"
 
 namespace {
@@ -922,11 +923,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (*reinterpret_cast<volatile int *>(&sh.abort)) { // a wait ran out: no result passes for one
-    const int64_t n = static_cast<int64_t>(a.Tq) * a.Hq * D;
-    for (int64_t i = tid; i < n; i += kThreads) a.out[i] = 0x7FC0;
-    if constexpr (SP)
-      for (int64_t i = tid; i < static_cast<int64_t>(a.slots) * C::kRows; i += kThreads)
-        a.part_ml[i] = make_float2(0.0f, __uint_as_float(0x7fc00000u));
+    const int64_t heads = static_cast<int64_t>(a.Tq) * a.Hq;
+    wm_giveup::poison(a.out, heads * D, a.lse, heads, SP ? a.part_ml : nullptr, static_cast<int64_t>(a.slots) * C::kRows, tid, kThreads);
   }
   if (warp == 9) {
     tc_fence_after();
