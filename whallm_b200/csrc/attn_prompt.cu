@@ -128,6 +128,7 @@ struct Bars {
   // MMA warp for v_fixed.  Both advance only with edge tiles, so a phase cannot pass unseen
   uint64_t kv_full[8], kv_empty[8], v_edge[8], v_fixed[8];
   uint64_t s_full[2], p_half[2], p_ready[2], o_done[2], m_ready[2], o_free, both;
+  uint64_t mma_end;                                   // the MMAs of a CTA that gives up
 };
 
 struct Shared {
@@ -158,6 +159,11 @@ __device__ __forceinline__ bool try_wait(uint64_t *bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+// A last bounded wait, for what is still in flight when the others gave up.
+__device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
+  for (int tries = 0; tries < 1000 && !wm_tc::mbar_try(bar, parity); ++tries) {}
 }
 
 // Bounded wait of a whole warp: all its lanes return the same answer.  A wait
@@ -418,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&b.next_full, 1);
     mbar_init(&b.o_free, 256);
     mbar_init(&b.both, 256);
+    mbar_init(&b.mma_end, 1);
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&b.kv_full[i], 1);
       mbar_init(&b.kv_empty[i], 1);
@@ -449,6 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 8) {
       // ------------------------------------------------- items and TMA loads
       uint32_t g = 0u;                                // pieces loaded so far
+      uint32_t asked = 0u;                            // requests for another item
       uint32_t edge_ph = 0u, edge_last = 0u;          // per slot: phase of v_edge, and whether the last load was an edge tile
       int it = 0;
       for (int x = static_cast<int>(blockIdx.x);; ++it) {
@@ -460,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bar.item_full[sl]);
         if (!item->valid) break;
         if (elect_one()) ask_next(&sh);
+        ++asked;
         const int n = item->tiles, first = item->first;
         bool ok = true;
         for (int p = 0; ok && p < 2 * n; ++p) {
@@ -502,15 +511,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         x = read_next(&sh);
         __syncwarp();
       }
-      // loads in flight when the others gave up must land before the CTA leaves
-      if (*reinterpret_cast<volatile int *>(&sh.abort))
+      // loads and the request in flight when the others gave up must land before the CTA leaves
+      if (*reinterpret_cast<volatile int *>(&sh.abort)) {
+        if (asked) drain(&bar.next_full, (asked - 1) & 1u);
         for (uint32_t i = g > C::kSlots ? g - C::kSlots : 0u; i < g; ++i) {
           const int slot = static_cast<int>(i % C::kSlots);
           const bool edge = (edge_last >> slot) & 1u;
           uint64_t *full = edge ? &bar.v_edge[slot] : &bar.kv_full[slot];
           const uint32_t ph = edge ? ((edge_ph >> slot) & 1u) ^ 1u : (i / C::kSlots) & 1u;
-          for (int tries = 0; tries < 1000 && !wm_tc::mbar_try(full, ph); ++tries) {}
+          drain(full, ph);
         }
+      }
     } else if (warp == 9) {
       // ------------------------------------------------------------- MMAs
       // One thread issues, but the whole warp keeps the state, and what it reads from shared memory goes
@@ -621,10 +632,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (s + 2 < steps) ok = issue_s(s + 2);
         }
       }
+      if (*reinterpret_cast<volatile int *>(&sh.abort)) {
+        if (elect_one()) tc_commit(&bar.mma_end);
+        __syncwarp();
+        drain(&bar.mma_end, 0u);
+      }
     } else {
       // --------------------------------- query rows, and values of edge tiles
       const int ht = tid - 320;
       uint32_t g0 = 0u, edge_ph = 0u;                 // pieces before this item, phases of v_edge
+      uint32_t q_loads = 0u;                          // tiles of Q loaded by TMA so far
       bool ok = true;
       for (int it = 0; ok; ++it) {
         const int sl = it & 1;
@@ -648,6 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_3d(qt + d * 16384, &map_q, d * 64, item->h * a.G, item->q0 + R0 / a.G, &bar.q_full[w]);
             }
             __syncwarp();
+            ++q_loads;
             continue;
           }
           constexpr int per = D / 8;                  // 16-byte pieces of a row
@@ -703,6 +721,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
         g0 += 2 * n * C::kParts;
       }
+      if (*reinterpret_cast<volatile int *>(&sh.abort))
+        for (uint32_t i = q_loads > C::kTiles ? q_loads - C::kTiles : 0u; i < q_loads; ++i)
+          drain(&bar.q_full[i % C::kTiles], (i / C::kTiles) & 1u);
     }
   } else {
     // ------------------------------------------------- softmax, one row each
