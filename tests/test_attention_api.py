@@ -236,3 +236,26 @@ def test_a_wait_that_ran_out_leaves_nan(tmp_path):
     # and the prompt kernel hands it all three
     text = open(os.path.join(build.CSRC, "attn_prompt.cu")).read()
     assert "poison(a.out, heads * D, a.lse, heads, SP ? a.part_ml : nullptr" in text
+
+
+def test_paged_cache_follows_steps_on_the_device():
+    """Steps that advance ``lengths`` on the device, as a captured one does: after ``refresh`` the host hands out pages
+    from the new counts, and refuses counts that its pages do not hold."""
+    c = W.PagedKVCache(2, 2, 64, n_pages=8, page_size=16, max_pages=5, device="cpu")
+    c.reserve([16, 3])
+    c.lengths += torch.tensor([16, 3], dtype=torch.int32)
+    c.refresh()
+    assert c.offsets == [16, 3] and c.free_pages == 6
+    c.reserve([16, 16])
+    assert c.free_pages == 4 and (c.page_table[:, :2] >= 0).all()
+    c.lengths.fill_(0)                               # shortened on the device: its pages stay handed out
+    c.refresh()
+    c.reserve([32, 32])
+    assert c.offsets == [0, 0] and c.free_pages == 4
+    for bad in ([33, 0], [0, -1]):
+        c.lengths.copy_(torch.tensor(bad, dtype=torch.int32))
+        with pytest.raises(ValueError, match="reserve before"):
+            c.refresh()
+        assert c.offsets == [0, 0]
+    c.clear(0)
+    assert c.free_pages == 6 and c.offsets == [0, 0]

@@ -76,3 +76,58 @@ def test_prompt_tile_of_nan_keys(dev, D, nq, nk, Hq, Hkv, tile):
     G = Hq // Hkv
     assert torch.isnan(out[:, :G]).all() and torch.isnan(lse[:, :G]).all()
     assert torch.isfinite(out[:, G:]).all() and torch.isfinite(lse[:, G:]).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_captured_steps_go_on_with_the_class(dev, fmt):
+    """reserve, captured steps, refresh, reserve, more of them over page borders, evict, append: the same cache as one
+    that only the class's own calls filled."""
+    B, Hkv, Hq, D, page = 3, 2, 8, 64, 16
+    g = gen(71, dev)
+    a, b = (W.PagedKVCache(B, Hkv, D, n_pages=20, page_size=page, max_pages=8, fmt=fmt, track=True) for _ in range(2))
+    start = [rnd(g, 34, Hkv, D, dev=dev) for _ in range(2)]
+    for c in (a, b):
+        c.append(*start, [16, 15, 3])
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    q, k, v = (torch.zeros((B, h, D), dtype=torch.bfloat16, device=dev) for h in (Hq, Hkv, Hkv))
+
+    def step(c):
+        c.lengths.add_(1)
+        c.seen.add_(1)
+        W.paged_append(k, v, cu, c.keys, c.values, c.page_table, c.lengths, c.fmt, c.key_scales, c.value_scales, c.mass,
+                       c.positions, c.seen)
+        return W.decode_attention(q, c.keys, c.values, c.page_table, c.lengths, c.fmt, c.key_scales, c.value_scales,
+                                  mass=c.mass)
+
+    spare = W.PagedKVCache(B, Hkv, D, n_pages=3, page_size=page, max_pages=8, fmt=fmt, track=True)
+    spare.reserve([1] * B)
+    step(spare)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step(b)
+
+    def feed():
+        for t in (q, k, v):
+            t.copy_(rnd(g, *t.shape, dev=dev))
+
+    for _ in range(3):                               # 3 x 8 steps: each run of them ends in new pages
+        b.reserve([8] * B)
+        for _ in range(8):
+            feed()
+            a.append(k, v)
+            want = a.attend(q)
+            gr.replay()
+            assert torch.equal(out, want) and torch.isfinite(out).all()
+        b.refresh()
+        assert a.offsets == b.offsets == a.lengths.tolist()
+    for c in (a, b):
+        c.evict(24, recent=4, sinks=1)
+    assert a.offsets == b.offsets == [24, 24, 24] == b.lengths.tolist() and a.free_pages == b.free_pages
+    feed()
+    outs = []
+    for c in (a, b):
+        c.append(k, v)
+        outs.append(c.attend(q))
+    assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+    for x in range(B):
+        assert torch.equal(a.mass[x, :, :25], b.mass[x, :, :25]) and torch.equal(a.positions[x, :, :25], b.positions[x, :, :25])

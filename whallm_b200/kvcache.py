@@ -436,7 +436,9 @@ class PagedKVCache:
 
     ``append`` and ``evict`` change host state, so a captured step calls
     ``attention.paged_append`` and ``decode_attention`` on these tensors instead,
-    over pages handed out beforehand with ``reserve``."""
+    over pages handed out beforehand with ``reserve``, and advances ``lengths``
+    (and ``seen``) itself.  The host does not see that: call ``refresh`` before
+    the next ``reserve``, ``append``, ``evict`` or ``offsets``."""
 
     def __init__(self, batch: int, heads: int, dimension: int, n_pages: int, page_size: int = 64,
                  max_pages: int | None = None, fmt: str = "bf16", track: bool = False, device="cuda"):
@@ -466,12 +468,11 @@ class PagedKVCache:
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch)]
         self._len = [0] * batch
-        self._seen = [0] * batch
 
     # -------------------------------------------------------------- pages --
     @property
     def offsets(self):
-        """Entries of each sequence."""
+        """Entries of each sequence, as the host counts them (see ``refresh``)."""
         return list(self._len)
 
     @property
@@ -497,11 +498,23 @@ class PagedKVCache:
             self._pages[b] += [self._free.pop() for _ in range(n)]
         self._write_table([b for b, n in enumerate(more) if n])
 
+    def refresh(self):
+        """Read ``lengths`` back after steps that changed it on the device (waits for them on the current stream).
+
+        Raises ValueError, and changes nothing, where a sequence ran past the pages handed out: its last tokens were
+        not stored."""
+        lengths = self.lengths.tolist()
+        for b, (n, pages) in enumerate(zip(lengths, self._pages)):
+            if not 0 <= n <= len(pages) * self.page_size:
+                raise ValueError(f"sequence {b} counts {n} entries, its pages hold {len(pages) * self.page_size}: "
+                                 "reserve before the steps")
+        self._len = lengths
+
     def clear(self, sequence: int):
         """Forget a sequence and take back its pages."""
         self._free += reversed(self._pages[sequence])
         self._pages[sequence] = []
-        self._len[sequence] = self._seen[sequence] = 0
+        self._len[sequence] = 0
         self._write_table([sequence])
         self.lengths[sequence] = 0
         self.seen[sequence] = 0
@@ -532,7 +545,6 @@ class PagedKVCache:
             self.seen.sub_(new)
             raise
         self._len = [n + c for n, c in zip(self._len, counts)]
-        self._seen = [n + c for n, c in zip(self._seen, counts)]
 
     def attend(self, queries: torch.Tensor, scale: float | None = None, return_lse: bool = False, out=None):
         """Attention of one token per sequence, bf16 [batch, query heads, D]; adds to ``mass`` if tracked."""
