@@ -296,8 +296,8 @@ WM_API int wkv_paged_evict(int B, int Hkv, int D, void *k_cache, void *v_cache, 
  * [0, capacity] or that reaches a page id outside [0, n_pages) gets NaN.
  * Workspace: wattn_decode_workspace_size (with a mass array it also holds the
  * scores, 4 bytes per entry of the capacity and query head, the heads of a kv
- * head rounded up to 2, above 16 to a multiple of 16); calls that share one must
- * not overlap. */
+ * head rounded up to 2, above 16 to a multiple of 16); the size follows the
+ * current device, as the call does; calls that share one must not overlap. */
 WM_API size_t wattn_decode_workspace_size(int B, int Hq, int Hkv, int D, int fmt, int page_size, int max_pages,
                                           int with_mass);
 WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int Hkv, int D, const void *k_cache,
@@ -317,8 +317,8 @@ WM_API int wattn_decode(const wm_bf16 *q, int64_t q_stride, int B, int Hq, int H
  * The kernel's waits are bounded (2 s); a call in which one runs out fills the
  * whole of out and lse with NaN, rows outside every sequence included.
  * D is 64, 128 or 256.  Workspace: wattn_prompt_workspace_size (0 unless few rows
- * meet many keys, which are then split over the GPU); calls that share one must
- * not overlap.  */
+ * meet many keys, which are then split over the GPU); the size follows the current
+ * device, as the call does; calls that share one must not overlap.  */
 WM_API size_t wattn_prompt_workspace_size(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 WM_API int wattn_prompt(const wm_bf16 *q, const wm_bf16 *k, const wm_bf16 *v, int64_t q_stride, int64_t k_stride,
                         int64_t v_stride, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int B, int Tq,

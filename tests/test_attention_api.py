@@ -259,3 +259,51 @@ def test_paged_cache_follows_steps_on_the_device():
         assert c.offsets == [0, 0]
     c.clear(0)
     assert c.free_pages == 6 and c.offsets == [0, 0]
+
+
+def test_workspaces_are_planned_on_the_tensors_device(monkeypatch):
+    """Two devices of different sizes, stood in for on the host: each call's workspace is the one that its own device
+    asks for, whichever is current and whichever came first."""
+    from whallm_b200 import attention as A
+
+    class Tensor:
+        def __init__(self, dev, dtype, *shape):
+            self.dev, self.dtype, self.shape, self.is_cuda = dev, dtype, torch.Size(shape), True
+
+        def stride(self):
+            return torch.empty(self.shape, device="meta").stride()
+
+        def new_empty(self, shape, dtype=None):
+            return Tensor(self.dev, dtype or self.dtype, *shape)
+
+        get_device, is_contiguous, data_ptr = lambda s: s.dev, lambda s: True, lambda s: 1 << 20
+        numel = lambda s: s.shape.numel()  # noqa: E731
+
+    current, calls = [0], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.dev
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            if name.endswith("_size"):
+                return lambda *shape: 1000 * (current[0] + 1)
+            return lambda *args: calls.append((name, current[0], args[-2])) or 0
+
+    monkeypatch.setattr(L, "_lib", Lib())
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(A, "_raw_stream", lambda dev: dev)
+    bf, i32 = torch.bfloat16, torch.int32
+    for dev in (1, 0, 2, 1):
+        t = lambda dtype, *shape: Tensor(dev, dtype, *shape)  # noqa: E731, B023
+        W.decode_attention(t(bf, 7, 8, 64), t(bf, 4, 2, 16, 64), t(bf, 4, 2, 16, 64), t(i32, 7, 300), t(i32, 7))
+        W.prompt_attention(t(bf, 7, 8, 64), t(bf, 9001, 2, 64), t(bf, 9001, 2, 64), t(i32, 2), t(i32, 2))
+        assert calls[-2:] == [("wattn_decode", dev, 1000 * (dev + 1)), ("wattn_prompt", dev, 1000 * (dev + 1))]

@@ -45,14 +45,13 @@ def _call(name, dev, *args):
         L.fail(name, rc)
 
 
-@functools.lru_cache(maxsize=256)
-def _decode_bytes(*shape):
-    return L.lib().wattn_decode_workspace_size(*shape)
-
-
-@functools.lru_cache(maxsize=256)
-def _prompt_bytes(*shape):
-    return L.lib().wattn_prompt_workspace_size(*shape)
+@functools.lru_cache(maxsize=512)
+def _bytes(name, dev, *shape):
+    """Workspace of a call on device number ``dev``: the plan behind it follows that device's SMs."""
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return getattr(L.lib(), name)(*shape)
+    return getattr(L.lib(), name)(*shape)
 
 
 def _at(name, t, dtype, shape, dev):
@@ -205,7 +204,7 @@ def decode_attention(q, k_cache, v_cache, page_table, lengths, fmt="bf16", k_sca
     if out is None:
         out = q.new_empty((B, Hq, d))
     lse = q.new_empty((B, Hq), dtype=_F32) if return_lse else None
-    nbytes = _decode_bytes(B, Hq, heads, d, f, size, width, mass is not None)
+    nbytes = _bytes("wattn_decode_workspace_size", dev, B, Hq, heads, d, f, size, width, mass is not None)
     ws = q.new_empty((nbytes,), dtype=_U8) if nbytes else None     # short caches need none
     _call("wattn_decode", dev, q.data_ptr(), qs, B, Hq, heads, d, kc, vc, ksc, vsc, f, pages, size, table, width,
           _at("lengths", lengths, _INT, (B,), dev), scale, _at("out", out, _BF16, (B, Hq, d), dev),
@@ -241,7 +240,7 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, causal=
     if out is None:
         out = q.new_empty((Tq, Hq, d))
     lse = q.new_empty((Tq, Hq), dtype=_F32) if return_lse else None
-    nbytes = _prompt_bytes(B, Tq, Tk, Hq, Hkv, d)
+    nbytes = _bytes("wattn_prompt_workspace_size", dev, B, Tq, Tk, Hq, Hkv, d)
     ws = q.new_empty((nbytes,), dtype=_U8) if nbytes else None     # only few rows on many keys need one
     _call("wattn_prompt", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs,
           _at("cu_seqlens", cu_seqlens, _INT, (B + 1,), dev), _at("cu_seqlens_k", cu_seqlens_k, _INT, (B + 1,), dev), B, Tq,
