@@ -78,6 +78,33 @@ def test_prompt_tile_of_nan_keys(dev, D, nq, nk, Hq, Hkv, tile):
     assert torch.isfinite(out[:, G:]).all() and torch.isfinite(lse[:, G:]).all()
 
 
+@pytest.mark.parametrize("fmt,D", [("fp8_f32_b64", 128), ("fp8_f32_b64", 256), ("mxfp8", 64), ("mxfp8", 128), ("mxfp8", 256)])
+@pytest.mark.parametrize("G,max_pages,mass", [(4, None, False), (9, None, False), (4, 300, False), (16, 300, True)])
+def test_decode_blocks_of_far_apart_scales(dev, fmt, D, G, max_pages, mass):
+    # every block of value dimensions in a range of its own, up to 2^100 apart: each is as exact as alone
+    lens = [1, 16, 17, 100, 700]
+    Hkv = 2
+    c = Cache(dev, lens, Hkv, D, 64, fmt, seed=D + G, max_pages=max_pages)
+    blocks = c.vs.shape[-1]
+    e = np.random.RandomState(D + G).randint(-60, 41, (len(lens), Hkv, blocks))
+    e[:, :, 0], e[:, :, 1] = 40, -60
+    for b, n in enumerate(lens):
+        f = torch.tensor(e[b], device=dev)
+        for p in c.table[b, :-(-n // 64)].tolist():
+            if fmt == "mxfp8":
+                c.vs[p] = (c.vs[p].int() + f[:, None, :]).clamp(0, 254).to(torch.uint8)
+            else:
+                c.vs[p] *= torch.exp2(f.double()).float()[:, None, :]
+        c.rows[b][1] = (c.rows[b][1].reshape(n, Hkv, blocks, -1) * 2.0 ** e[b][None, :, :, None]).reshape(n, Hkv, D)
+    q = rnd(gen(9, dev), len(lens), G * Hkv, D, std=2.0, dev=dev)
+    m = torch.zeros((len(lens), Hkv, c.width * 64), device=dev) if mass else None
+    out, lse = W.decode_attention(q, *c.args, mass=m, return_lse=True)
+    for b in range(len(lens)):
+        ref = A.attend(f64(q[b:b + 1]), *c.rows[b], D ** -0.5)
+        check_out(out[b:b + 1], ref, D)
+        check_lse(lse[b:b + 1], ref, D)
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
 def test_captured_steps_go_on_with_the_class(dev, fmt):
     """reserve, captured steps, refresh, reserve, more of them over page borders, evict, append: the same cache as one

@@ -30,10 +30,11 @@
 // of two per head that puts its largest magnitude into [2^14, 2^15): exact for
 // values within 2^-28 of it, off by less than 2^-39 of it below.  A key's block
 // scales multiply its partial scores.  A value's block scales multiply its weight
-// before the rounding, in units of the largest power of two seen among the warp's
-// scales (O is rescaled when that grows, as for the maximum) and times 2^15: the
-// weights are f16 values of at most 2^15, rounded to 11 bits down to 2^-29 of the
-// largest, and no dequantized row is ever rounded.
+// before the rounding, times a power of two for the block's dimensions that keeps
+// the product at most 2^15.  It starts at 2^115 and falls when a scale of the warp's
+// values needs it, then to 2^13 so that this happens once or twice per part (O is
+// rescaled as for the maximum): the weights are rounded to 11 bits down to 2^-26 of
+// the largest of their block, and no dequantized row is ever rounded.
 //
 // Measured (CUDA graphs, three input sets in turn): 64 sequences of 90 to 8190
 // entries, 32/8 heads of 128, bf16: 166 us, 6.7 TB/s (a plain copy: 6.5); two of
@@ -58,6 +59,7 @@ constexpr int kUnit = kWarps * kTile;   // keys of a unit of work
 constexpr int kMaxCluster = 8;
 constexpr int kClusterKeys = 1024;      // capacity per CTA up to which a cluster joins a pair
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTopWeight = 32768.0f;  // of a weight in f16
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -233,6 +235,9 @@ struct Shape {
   static constexpr int kChunks = kRow / 16;
   static constexpr int kScale = wm_paged::scale_bytes(FMT, D);    // bytes of a row's scales
   static constexpr int kBlocks = FMT == WKV_BF16 ? 1 : (FMT == WKV_FP8_F32_B64 ? D / 64 : D / 32);
+  // 16 heads of 256 fill the registers: the blocks' factors are held in shared memory (87 -> 79 us for two of 130,000
+  // MXFP8 entries, 32/2 heads; smaller shapes lose 1 %)
+  static constexpr bool kFar = D == 256 && NH == 2 && FMT != WKV_BF16;
   static constexpr int kStage = 2 * kTile * (kRow + kScale);      // keys, values and their scales
   static constexpr int kStages = D == 64 && FMT != WKV_BF16 ? 4 : 3;
   static constexpr int kHeads = 8 * NH;
@@ -254,6 +259,9 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
 // finite score keeps its sum (zero, or NaN).
 __device__ __forceinline__ float part_factor(float m, float top) { return m == kNegInf ? 1.0f : ex2(m - top); }
 
+// 1 / x for a power of two in [2^-126, 2^126]
+__device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // CL: a cluster of CTAs per pair instead of a share of the line (see launch()).
 template <int D, int FMT, int NH, bool CL>
 __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
@@ -261,6 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[kWarps][S::kHeads], sm_l[kWarps][S::kHeads];
   __shared__ float2 sm_part[S::kHeads];               // the CTA's maximum and sum
+  __shared__ __align__(16) float sm_factor[kWarps][S::kFar ? S::kBlocks : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i2 = (lane & 3) * 2;
   uint8_t *ring = smem + warp * (S::kStages * S::kStage);
   const uint32_t ring_u = wm_tc::smem_u32(ring);
@@ -327,7 +336,26 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
 
     float o[D / 16][NH][4];
     float m[NH][2], l[NH][2];
-    float unit = 0.0f, per_unit = 0.0f;               // e4m3: O is in units of `unit`; 2^15 / unit
+    float factor[S::kBlocks];                         // e4m3: of the weights and O of a block's dimensions, a power of two
+#pragma unroll
+    for (int blk = 0; blk < S::kBlocks; ++blk) factor[blk] = 0x1p115f;
+    auto keep_factors = [&] {                         // where registers are short: in shared memory between their uses
+      if constexpr (S::kFar) {
+        __syncwarp();
+        if (lane == 0)
+#pragma unroll
+          for (int blk = 0; blk < S::kBlocks; ++blk) sm_factor[warp][blk] = factor[blk];
+        __syncwarp();
+      }
+    };
+    auto fetch_factors = [&] {
+      if constexpr (S::kFar) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int blk = 0; blk < S::kBlocks; ++blk) factor[blk] = sm_factor[warp][blk];
+      }
+    };
+    keep_factors();
 #pragma unroll
     for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -405,8 +433,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
       if constexpr (FMT != WKV_BF16) {
         load_scales<FMT>(sc + g * S::kScale, ka);
         load_scales<FMT>(sc + (g + 8) * S::kScale, kb);
-        load_scales<FMT>(sc + (kTile + g) * S::kScale, va);
-        load_scales<FMT>(sc + (kTile + g + 8) * S::kScale, vb);
       }
 
       // scores: rows are keys (g, g + 8), columns heads (i2, i2 + 1)
@@ -458,6 +484,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
             s[nh][3] = fmaf(t[nh][3], kb[blk], s[nh][3]);
           }
         }
+      }
+      if constexpr (FMT != WKV_BF16) {
+        load_scales<FMT>(sc + (kTile + g) * S::kScale, va);
+        load_scales<FMT>(sc + (kTile + g + 8) * S::kScale, vb);
       }
       const int key = (t0 + i * kWarps) * kTile;
       const int rows = min(kTile, len - key);
@@ -537,36 +567,49 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
           for (int nh = 0; nh < NH; ++nh) mma(o[mt][nh], f, p[nh][0], p[nh][1]);
         }
       } else {
-        // the unit follows the largest scale of the warp's values
-        float big = 0.0f;
+        float s0[S::kBlocks], s1[S::kBlocks], big = 0.0f;
+        fetch_factors();
 #pragma unroll
-        for (int blk = 0; blk < S::kBlocks; ++blk) big = fmaxf(big, fmaxf(va[blk], vb[blk]));
-        if (__any_sync(0xffffffffu, big > unit)) {
-          big = fmaxf(big, unit);
+        for (int blk = 0; blk < S::kBlocks; ++blk) {
+          s0[blk] = va[blk] * factor[blk];
+          s1[blk] = vb[blk] * factor[blk];
+          big = fmaxf(big, fmaxf(s0[blk], s1[blk]));
+        }
+        if (__any_sync(0xffffffffu, big > kTopWeight)) {
+          asm volatile("" ::: "memory");              // all read again: none is held in a register for this
+          fetch_factors();
+          load_scales<FMT>(sc + (kTile + g) * S::kScale, va);
+          load_scales<FMT>(sc + (kTile + g + 8) * S::kScale, vb);
 #pragma unroll
-          for (int x = 16; x; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-          // the next power of two, within what has a reciprocal
-          const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 126, -100), 127);
-          const float u = wm_stream::pow2f(e), f = unit / u;
-          unit = u;
-          per_unit = 32768.0f / u;
+          for (int blk = 0; blk < S::kBlocks; ++blk) {
+            float x = fmaxf(va[blk], vb[blk]);        // the largest scale of the block's values
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt)
+            for (int y = 16; y; y >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+            // to less than 2^13: a scale has to grow four times before the next change
+            const bool low = x * factor[blk] > kTopWeight;
+            const float next = low ? wm_stream::pow2f(139 - static_cast<int>(__float_as_uint(x) >> 23)) : factor[blk];
+            const float f = low ? next * inverse(factor[blk]) : 1.0f;
+            factor[blk] = next;
+            s0[blk] = va[blk] * next;
+            s1[blk] = vb[blk] * next;
 #pragma unroll
-            for (int nh = 0; nh < NH; ++nh)
+            for (int y = 0; y < D / 16 / S::kBlocks; ++y)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) o[mt][nh][x] *= f;
+              for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[blk * (D / 16 / S::kBlocks) + y][nh][j] *= f;
+          }
+          keep_factors();
         }
         constexpr int per = D / 16 / S::kBlocks;
         const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
 #pragma unroll
         for (int blk = 0; blk < S::kBlocks; ++blk) {
-          const float s0 = va[blk] * per_unit, s1 = vb[blk] * per_unit;
           uint32_t p[NH][2];
 #pragma unroll
           for (int nh = 0; nh < NH; ++nh) {
-            p[nh][0] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][0] * s0, s[nh][1] * s0));
-            p[nh][1] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][2] * s1, s[nh][3] * s1));
+            p[nh][0] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][0] * s0[blk], s[nh][1] * s0[blk]));
+            p[nh][1] = transpose8(wm_stream::f32x2_to_f16x2(s[nh][2] * s1[blk], s[nh][3] * s1[blk]));
           }
 #pragma unroll
           for (int x = 0; x < per; x += 2) {
@@ -615,20 +658,21 @@ __global__ void __launch_bounds__(kWarps * 32) k_attn_decode(DecodeArgs a) {
         }
     __syncthreads();                                  // all rings are drained
     float *mg = reinterpret_cast<float *>(smem);      // [warp][head][D]
+    fetch_factors();
 #pragma unroll
     for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int hd = nh * 8 + i2 + j;
         const float top = fmaxf(fmaxf(sm_m[0][hd], sm_m[1][hd]), fmaxf(sm_m[2][hd], sm_m[3][hd]));
-        float f = m[nh][j] == kNegInf ? (n > 0 ? 1.0f : 0.0f) : ex2(m[nh][j] - top);
-        if constexpr (FMT != WKV_BF16) f *= unit * 0x1p-15f;
+        const float f = m[nh][j] == kNegInf ? (n > 0 ? 1.0f : 0.0f) : ex2(m[nh][j] - top);
         float *row = mg + (warp * S::kHeads + hd) * D;
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) {
           const int d0 = FMT == WKV_BF16 ? 16 * mt + g : 16 * mt + 2 * g, d1 = FMT == WKV_BF16 ? d0 + 8 : d0 + 1;
-          row[d0] = o[mt][nh][j] * f;
-          row[d1] = o[mt][nh][j + 2] * f;
+          const float to = FMT == WKV_BF16 ? f : f * inverse(factor[mt / (D / 16 / S::kBlocks)]);
+          row[d0] = o[mt][nh][j] * to;
+          row[d1] = o[mt][nh][j + 2] * to;
         }
       }
     __syncthreads();
