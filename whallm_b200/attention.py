@@ -194,7 +194,9 @@ def decode_attention(q, k_cache, v_cache, page_table, lengths, fmt="bf16", k_sca
     (float32 [B, Hkv, capacity]) collects every entry's attention weight, summed
     over the query heads of its key-value head.  ``scale`` defaults to D^-1/2.  A
     sequence without entries gets zeros (lse -inf); one whose length or pages are
-    out of range gets NaN."""
+    out of range gets NaN.  A key whose score is -inf weighs nothing.  With ``mass``
+    time and workspace grow with the capacity (the table's width), so keep that near
+    the longest sequence."""
     f, pages, heads, size, d, B, width, dev, kc, vc, ksc, vsc, table = _pool(k_cache, v_cache, k_scales, v_scales,
                                                                              page_table, fmt)
     Bq, Hq, _, qs = _tokens("q", q, None, d, dev)

@@ -3,8 +3,8 @@
 //   s_j = scale q.k_j,  lse = log sum_j exp(s_j),  out = sum_j exp(s_j - lse) v_j
 //
 // for the G = Hq / Hkv query heads of each key-value head at once.  The call is
-// HBM bound: every cached row is read once, 4 D bytes (bf16) per entry and head
-// against 4 D G operations.
+// HBM bound: every cached row is read once for each 16 of these heads, 4 D bytes (bf16)
+// per entry and head against 4 D G operations.
 //
 // Work split.  The entries of all (sequence, head) pairs form one line of units
 // of 64 keys; every CTA takes a share of the line (struct Line), found from the

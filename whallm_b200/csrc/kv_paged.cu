@@ -19,11 +19,14 @@ namespace {
 // lane and piece, all issued first).  Its lanes then find, one token each, where
 // the tokens it touches go: binary search in cu_seqlens (held in shared memory),
 // length, page.  The pieces get their token's row by shuffle; a quantized row's
-// scale blocks are 2 or 4 adjacent lanes, as in k_kv_fp8_quantize.  Bound by HBM
-// for bf16 rows (2 B read, 2 B written per value) and by the quantizer's
-// arithmetic for e4m3 rows: with a search per piece it took 475 instructions per
-// 16 values, 59 % of the issue slots.  13,200 tokens of 2 x 256 values to e4m3: 15.6
-// us (22.5 with one piece per lane and a search each); 64 tokens of 8 x 128: 2.5 us.
+// scale blocks are 2 or 4 adjacent lanes, as in k_kv_fp8_quantize.  Bound by the
+// waves of CTAs (2.8 of them below) and, for e4m3 rows, the quantizer's arithmetic:
+// with a search per piece it took 475 instructions per 16 values, 59 % of the issue
+// slots.  16,784 tokens of 2 x 256 values: bf16 rows 14.1 us (4.9 TB/s read and
+// written), e4m3 with float32 scales 15.1, MXFP8 15.0, each 0.7 to 0.9 more with weights
+// and positions (e4m3 22.5 with one piece per lane and a search each); 64 tokens of 8 x
+// 128: 2.5 us.  Five CTAs per SM cap the registers at 48, at which the float32-scale form
+// with two pieces spills 76 bytes.
 
 constexpr int kSeqSmem = 512;          // sequences searched in shared memory
 

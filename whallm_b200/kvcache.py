@@ -427,6 +427,8 @@ class PagedKVCache:
     """Keys and values of up to ``batch`` sequences in one pool of ``n_pages``
     pages of ``page_size`` entries, read by ``attention.decode_attention``.
 
+    A sequence holds up to ``max_pages`` of them (default: all), by which launches,
+    ``mass`` and workspaces are sized: give the longest that is needed.
     ``fmt`` is a format of ``attention.PAGED_FORMATS``; with ``track`` every
     entry also has its position and the attention weight it received (``mass``),
     by which ``evict`` reduces the sequences to a budget.  Pages are handed out
