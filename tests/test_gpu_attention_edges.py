@@ -9,7 +9,7 @@ import torch
 
 import whallm_b200 as W
 from oracle import attention as A
-from tests.test_gpu_attention import Cache, check_lse, check_mass, check_out, f64, gen, rnd
+from tests.test_gpu_attention import Cache, check_lse, check_mass, check_out, f64, gen, rnd, run_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -76,6 +76,25 @@ def test_prompt_tile_of_nan_keys(dev, D, nq, nk, Hq, Hkv, tile):
     G = Hq // Hkv
     assert torch.isnan(out[:, :G]).all() and torch.isnan(lse[:, :G]).all()
     assert torch.isfinite(out[:, G:]).all() and torch.isfinite(lse[:, G:]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("nq,nk,Hq,Hkv", [
+    ([1, 2, 1, 0, 1] * 8, [0, 1, 0, 3, 0] * 8, 8, 8),                    # one-tile blocks, most of them without keys
+    ([1] * 60, [0] * 60, 64, 8),
+    ([300, 5, 260] * 12, [0, 5, 0] * 12, 8, 8),                          # two-tile blocks
+    ([900, 700], [100, 650], 32, 8),                                     # rows in front of a sequence's keys
+])
+def test_prompt_blocks_without_keys_in_a_row(dev, D, nq, nk, Hq, Hkv):
+    # more blocks than SMs, so that a CTA gets several without a key, one after the other; each call once more while
+    # the caches are warm
+    q, k, v, out, lse = run_prompt(dev, nq, nk, Hq, Hkv, D, seed=70)
+    cu = lambda n: torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=dev)  # noqa: E731
+    cq, ck = cu(nq), cu(nk)
+    for _ in range(300):
+        again, lse2 = W.prompt_attention(q, k, v, cq, ck, return_lse=True)
+        torch.cuda.synchronize()
+        assert torch.equal(lse2, lse) and torch.equal(again, out)
 
 
 @pytest.mark.parametrize("fmt,D", [("fp8_f32_b64", 128), ("fp8_f32_b64", 256), ("mxfp8", 64), ("mxfp8", 128), ("mxfp8", 256)])

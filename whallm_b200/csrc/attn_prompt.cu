@@ -541,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       Ring base{0, 0u};                               // slot of this item's first piece
+      uint32_t o_ph = 1u;                             // phase of o_free: of the last item that had keys
       uint32_t fixed = 0u, pph = 0u;                  // phase bits: v_fixed per slot, P per buffer
       const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
       bool ok = true;
@@ -591,7 +592,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && lane == 0) mbar_arrive(&bar.q_empty[w]);
           }
         for (int s = 0; ok && s < 2 && s < steps; ++s) ok = issue_s(s);
-        if (ok && it > 0) ok = wait(&sh, &bar.o_free, (it - 1) & 1);  // the last item's O has been read
+        // The last O has been read.  Items without keys have none and take no part in this: the softmax warps run
+        // through them without this warp, two of them would pass two phases before it looks
+        if (ok && steps > 0) {
+          ok = wait(&sh, &bar.o_free, o_ph);
+          o_ph ^= 1u;
+        }
         for (int s = 0; ok && s < steps; ++s) {
           const int j = C::kChain ? s : s >> 1, w = C::kChain ? 0 : s & 1, buf = s & 1;
           // the keys of P's first half are multiplied while the softmax still works on the second
@@ -937,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           a.part_ml[static_cast<int64_t>(item->slot) * C::kRows + (R - item->blk * C::kRows)] = make_float2(m, l);
       } else if (live && a.lse && (!C::kChain || w == 0)) a.lse[head] = see > 0 ? (m + log2f(l)) * kLn2 : kNegInf;
       tc_fence_before();
-      mbar_arrive(&bar.o_free);
+      if (steps > 0) mbar_arrive(&bar.o_free);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.item_empty[sl]);
     }
