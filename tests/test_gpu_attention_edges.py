@@ -56,6 +56,31 @@ def test_decode_keys_of_minus_infinity(dev, fmt, D, G, max_pages, mass):
             assert torch.equal(m[b, :, gone], before[b, :, gone])
 
 
+@pytest.mark.parametrize("D,G", [(64, 3), (128, 4), (256, 12)])
+@pytest.mark.parametrize("max_pages", [None, 300])
+def test_decode_values_that_are_not_finite(dev, D, G, max_pages):
+    # a live value shows in its dimension and its kv head's rows, a NaN key in its kv head's; nowhere else
+    Hkv, lens = 2, [40, 500, 17]
+    c = Cache(dev, lens, Hkv, D, 64, "bf16", seed=D, max_pages=max_pages)
+    q = rnd(gen(10, dev), len(lens), G * Hkv, D, dev=dev)
+    want, lse = W.decode_attention(q, *c.args, return_lse=True)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        v = c.v.clone()
+        v[c.table[1, 3], 1, 9, D - 2] = bad
+        got, l2 = W.decode_attention(q, c.k, v, *c.args[2:], return_lse=True)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[1, G:, D - 2] = True
+        assert torch.equal(got[~hit], want[~hit]) and torch.equal(l2, lse)
+        assert (torch.isnan(got[hit]) if bad != bad else got[hit] == bad).all()
+    k = c.k.clone()
+    k[c.table[1, 3], 1, 9, 0] = float("nan")
+    got, l2 = W.decode_attention(q, k, c.v, *c.args[2:], return_lse=True)
+    hit = torch.zeros_like(lse, dtype=torch.bool)
+    hit[1, G:] = True
+    assert torch.equal(got[~hit], want[~hit]) and torch.equal(l2[~hit], lse[~hit])
+    assert torch.isnan(got[hit]).all() and torch.isnan(l2[hit]).all()
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("nq,nk,Hq,Hkv", [
     ([4], [256], 8, 2), ([4, 3], [257, 390], 4, 1),                      # blocks of one tile
